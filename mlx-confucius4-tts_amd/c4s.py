@@ -1,4 +1,5 @@
-"""Python binding of libc4s_sampling.so (C ABI in include/c4s_sampling.h).
+"""Python binding of libc4s_sampling.so (C ABI in include/c4s_sampling.h and,
+for the decoder layer's operators, include/c4s_layers.h).
 
 ctypes only; torch supplies device memory and streams, nothing else. Loading
 fails loudly when the library has not been built or no gfx950 device is
@@ -16,6 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "lib", "libc4s_sampling.so")
 HEADER = os.path.join(REPO, "include", "c4s_sampling.h")
+LAYERS_HEADER = os.path.join(REPO, "include", "c4s_layers.h")
 
 OK, EINVAL, EHIP, ENOMEM, ETIMEOUT = 0, 1, 2, 3, 4
 F32, BF16 = 0, 1
@@ -26,7 +28,10 @@ MODE_CUSTOM = 256
 STAT_PATH, STAT_TOPP_EXACT, STAT_DRAW_EXACT, STAT_KEPT = 0, 1, 2, 3
 STREAM_SEQUENTIAL = 1
 STREAM_NO_SPECULATION = 2
-W_BF16, W_F32, W_Q8 = 0, 1, 2   # c4s_head.wdtype
+W_BF16, W_F32, W_Q8 = 0, 1, 2   # c4s_head.wdtype, c4s_linear_desc.wdtype
+NORM_LAYER, NORM_RMS = 0, 1
+ACTS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3}   # c4s_linear_desc.act
+KV_BF16, KV_Q8 = 0, 1
 
 _vp = C.c_void_p
 
@@ -62,9 +67,42 @@ class HeadWeights(C.Structure):
                 ("wbias", _vp), ("D", C.c_int32), ("V", C.c_int32), ("wdtype", C.c_int32), ("group", C.c_int32)]
 
 
-def header_functions() -> list[str]:
-    """Names of every function the public header declares."""
-    txt = open(HEADER).read()
+class Norm(C.Structure):
+    _fields_ = [("M", C.c_int32), ("D", C.c_int32), ("kind", C.c_int32), ("eps", C.c_float),
+                ("x", _vp), ("ldx", C.c_int64), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32),
+                ("y", _vp), ("ldy", C.c_int64), ("post", C.c_int32), ("gate_rows", C.c_int32),
+                ("post_gamma", _vp), ("post_beta", _vp), ("gate", _vp), ("ld_gate", C.c_int64),
+                ("res_scale", C.c_float), ("out_dtype", C.c_int32), ("gamma", _vp), ("beta", _vp),
+                ("x_out", _vp), ("ld_x_out", C.c_int64), ("out", _vp), ("ld_out", C.c_int64)]
+
+
+class Linear(C.Structure):
+    _fields_ = [("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("act", C.c_int32),
+                ("x", _vp), ("ldx", C.c_int64), ("weight", _vp), ("wdtype", C.c_int32), ("group", C.c_int32),
+                ("wscale", _vp), ("wbias", _vp), ("bias", _vp), ("residual", _vp), ("ld_res", C.c_int64),
+                ("res_dtype", C.c_int32), ("out_dtype", C.c_int32), ("out", _vp), ("ld_out", C.c_int64)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("block_table", _vp),
+                ("table_ld", C.c_int64), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("store", C.c_int32)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("ldk", C.c_int64), ("ldv", C.c_int64), ("lens", _vp), ("rows_off", _vp),
+                ("n_rows", C.c_int32), ("dtype", C.c_int32)]
+
+
+class Attn(C.Structure):
+    _fields_ = [("q", _vp), ("ldq", C.c_int64), ("out", _vp), ("ld_out", C.c_int64), ("lse", _vp), ("lens", _vp),
+                ("rows_off", _vp), ("first", _vp), ("n_rows", C.c_int32), ("max_new", C.c_int32),
+                ("n_heads", C.c_int32), ("scale", C.c_float)]
+
+
+def header_functions(header: str = HEADER) -> list[str]:
+    """Names of every function a public header declares."""
+    txt = open(header).read()
     txt = re.sub(r"/\*.*?\*/", "", txt, flags=re.S)
     return sorted(set(re.findall(r"\b(c4s_[a-z0-9_]+)\s*\(", txt)))
 
@@ -119,6 +157,11 @@ def lib() -> C.CDLL:
     L.c4s_head_weights_load.argtypes = [C.c_char_p, C.c_int32, C.c_int32, C.POINTER(HeadWeights)]
     L.c4s_head_weights_free.argtypes = [C.POINTER(HeadWeights)]
     L.c4s_weights_last_error.restype = C.c_char_p
+    L.c4s_block_norm.argtypes = [_vp, C.POINTER(Norm), _vp]
+    L.c4s_linear.argtypes = [_vp, C.POINTER(Linear), _vp]
+    L.c4s_kv_append.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(KvRows), _vp]
+    L.c4s_kv_read.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(KvRows), _vp]
+    L.c4s_attn.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(Attn), _vp]
     _lib = L
     return L
 
@@ -192,6 +235,97 @@ def load_head_weights(root: str, wdtype: int = W_BF16, group: int = 64) -> HeadW
 
 def free_head_weights(hw: HeadWeights) -> None:
     lib().c4s_head_weights_free(C.byref(hw))
+
+
+def _dtype(t) -> int:
+    """C4S_DTYPE_* of a tensor that is bf16 or float32."""
+    import torch
+    if t.dtype == torch.bfloat16:
+        return BF16
+    if t.dtype == torch.float32:
+        return F32
+    raise ValueError(f"expected a bfloat16 or float32 tensor, got {t.dtype}")
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _vector(t, n, what):
+    """The address of a contiguous float32 vector of n values, or None."""
+    import torch
+    if t is None:
+        return None
+    _need(t.dtype == torch.float32 and t.dim() == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1),
+          f"{what}: expected a contiguous float32 vector of {n}")
+    return t.data_ptr()
+
+
+def _i32(t, n, what):
+    """The address of a contiguous int32 vector of n values, or None."""
+    import torch
+    if t is None:
+        return None
+    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1),
+          f"{what}: expected a contiguous int32 vector of {n}")
+    return t.data_ptr()
+
+
+def _rows(t, what):
+    """(address, row stride) of a [rows][width] tensor whose rows are contiguous."""
+    _need(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what}: expected rows of contiguous values")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _heads(t, heads, dim, what):
+    """(address, row stride) of a [rows][heads][dim] tensor whose rows are contiguous."""
+    _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == dim and (t.stride(2) == 1 or dim <= 1) and
+          (heads == 1 or t.stride(1) == dim), f"{what}: expected [rows][{heads}][{dim}], a row contiguous")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else heads * dim)
+
+
+class KvCache:
+    """The tensors of one layer's paged cache (c4s_kv_cache in include/c4s_layers.h):
+
+    k            [n_pages][n_kv_heads][page_size][head_dim]  bfloat16, or int8 codes
+    v            [n_pages][n_kv_heads][head_dim][page_size]  as k
+    k_scale, v_scale  [n_pages][n_kv_heads][page_size]       float32, with int8 codes
+    block_table  [n_seqs][max_pages]                         int32, shared by the layers
+
+    The object keeps the tensors and their addresses; their contents may change
+    at any time."""
+
+    def __init__(self, k, v, block_table, k_scale=None, v_scale=None):
+        import torch
+        _need(k.dim() == 4 and k.is_contiguous() and v.is_contiguous(), "KvCache: k and v must be contiguous, 4-d")
+        pages, heads, size, dim = k.shape
+        _need(tuple(v.shape) == (pages, heads, dim, size), "KvCache: v must be [n_pages][n_kv_heads][head_dim][page_size]")
+        _need(k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.int8), "KvCache: k and v must be bfloat16 or int8")
+        q8 = k.dtype == torch.int8
+        _need(q8 == (k_scale is not None) and q8 == (v_scale is not None), "KvCache: scales go with int8 codes")
+        for s in (k_scale, v_scale):
+            _need(s is None or (s.dtype == torch.float32 and s.is_contiguous() and tuple(s.shape) == (pages, heads, size)),
+                  "KvCache: scales must be contiguous float32 [n_pages][n_kv_heads][page_size]")
+        _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and
+              (block_table.shape[1] <= 1 or block_table.stride(1) == 1), "KvCache: block_table must be int32 rows")
+        n_seqs, max_pages = block_table.shape
+        self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
+        self.n_seqs, self.n_kv_heads, self.head_dim, self.page_size = n_seqs, heads, dim, size
+        self.desc = KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), _p(block_table),
+                                block_table.stride(0) if n_seqs > 1 else max_pages, n_seqs, max_pages, pages, size,
+                                heads, dim, KV_Q8 if q8 else KV_BF16)
+        self.ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, q8=False):
+        """A cache of its own on block_table's device; nothing in it is set."""
+        import torch
+        t, d = torch.int8 if q8 else torch.bfloat16, block_table.device
+        k = torch.empty((n_pages, n_kv_heads, page_size, head_dim), dtype=t, device=d)
+        v = torch.empty((n_pages, n_kv_heads, head_dim, page_size), dtype=t, device=d)
+        scales = [torch.empty((n_pages, n_kv_heads, page_size), device=d) for _ in range(2)] if q8 else [None, None]
+        return cls(k, v, block_table, *scales)
 
 
 class Context:
@@ -336,6 +470,106 @@ class Context:
                  out_stats=_p(out_stats), mode=MODE_CHAIN, hist_bits=_p(hist_bits), stop_token=stop_token)
         self._check(lib().c4s_lmhead_sample_noalloc(self._h, C.byref(h), C.byref(r), _stream_handle(stream)),
                     "lmhead_sample_noalloc")
+
+    # ---- the decoder layer's operators (include/c4s_layers.h) ---------------------------
+    def block_norm(self, x, gamma, beta, out, y=None, x_out=None, post=False, post_gamma=None, post_beta=None,
+                   gate=None, gate_rows=1, scale=1.0, eps=1e-5, rms=False, stream=None):
+        """r = x + scale * gate (.) u with u = y, or norm(y) when post; x_out = r;
+        out = norm(r). x, y, x_out, out: [rows][D], bfloat16 or float32; gate:
+        float32 [ceil(rows / gate_rows)][D]; without y, r = x."""
+        M, D = x.shape
+        for name, t in (("y", y), ("x_out", x_out), ("out", out)):
+            _need(t is None or tuple(t.shape) == (M, D), f"block_norm: {name} must be [{M}][{D}]")
+        _need(x_out is None or x_out.dtype == x.dtype, "block_norm: x_out must have x's dtype")
+        g, ldg = (None, 0)
+        if gate is not None:
+            _need(gate_rows >= 1 and gate.shape[0] * gate_rows >= M and gate.shape[1] == D and _dtype(gate) == F32,
+                  "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+            g, ldg = _rows(gate, "block_norm: gate")
+        xp, ldx = _rows(x, "block_norm: x")
+        yp, ldy = (None, 0) if y is None else _rows(y, "block_norm: y")
+        xo, ldxo = (None, 0) if x_out is None else _rows(x_out, "block_norm: x_out")
+        op, ldo = (None, 0) if out is None else _rows(out, "block_norm: out")
+        d = Norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, _dtype(x), F32 if y is None else _dtype(y), yp,
+                 ldy, 1 if post else 0, gate_rows, _vector(post_gamma, D, "block_norm: post_gamma"),
+                 _vector(post_beta, D, "block_norm: post_beta"), g, ldg, scale, F32 if out is None else _dtype(out),
+                 _vector(gamma, D, "block_norm: gamma"), _vector(beta, D, "block_norm: beta"), xo, ldxo, op, ldo)
+        rc = lib().c4s_block_norm(self._h, C.byref(d), _stream_handle(stream))
+        if rc:
+            self._check(rc, "block_norm")
+
+    def linear(self, x, weight, out, bias=None, residual=None, act="none", quant=None, stream=None):
+        """out = residual + act(x @ weight^T + bias). x: bfloat16 [M][K]; weight:
+        [N][K], bfloat16, or uint8 codes with quant=(scales, offsets, group);
+        residual, out: [M][N], bfloat16 or float32; act: none, gelu, silu, relu."""
+        import torch
+        M, K = x.shape
+        N = weight.shape[0]
+        _need(x.dtype == torch.bfloat16 and weight.dim() == 2 and weight.shape[1] == K and weight.is_contiguous(),
+              "linear: x must be bfloat16 [M][K], weight contiguous [N][K]")
+        _need(tuple(out.shape) == (M, N) and (residual is None or tuple(residual.shape) == (M, N)),
+              f"linear: out and residual must be [{M}][{N}]")
+        _need(weight.dtype == (torch.bfloat16 if quant is None else torch.uint8),
+              "linear: weights are bfloat16, or uint8 with quant=(scales, offsets, group)")
+        ws, wb, group = quant if quant is not None else (None, None, 0)
+        for t in (ws, wb):
+            _need(t is None or (group > 0 and t.dtype == torch.float32 and t.is_contiguous() and
+                                tuple(t.shape) == (N, K // group)), "linear: scales and offsets must be float32 [N][K / group]")
+        _need(act in ACTS, f"linear: act must be one of {', '.join(ACTS)}")
+        xp, ldx = _rows(x, "linear: x")
+        op, ldo = _rows(out, "linear: out")
+        rp, ldr = (None, 0) if residual is None else _rows(residual, "linear: residual")
+        d = Linear(M, N, K, ACTS[act], xp, ldx, weight.data_ptr(), W_BF16 if quant is None else W_Q8, group, _p(ws),
+                   _p(wb), _vector(bias, N, "linear: bias"), rp, ldr, F32 if residual is None else _dtype(residual),
+                   _dtype(out), op, ldo)
+        rc = lib().c4s_linear(self._h, C.byref(d), _stream_handle(stream))
+        if rc:
+            self._check(rc, "linear")
+
+    def _kv_rows(self, cache, k, v, lens, rows_off, what):
+        heads, dim = cache.n_kv_heads, cache.head_dim
+        _need(k.shape[0] == v.shape[0] and k.dtype == v.dtype, f"{what}: k and v must be alike")
+        kp, ldk = _heads(k, heads, dim, f"{what}: k")
+        vp, ldv = _heads(v, heads, dim, f"{what}: v")
+        return KvRows(kp, vp, ldk, ldv, _i32(lens, cache.n_seqs, f"{what}: lens"),
+                      _i32(rows_off, cache.n_seqs + 1, f"{what}: rows_off"), k.shape[0], _dtype(k))
+
+    def kv_append(self, cache, k, v, lens, rows_off=None, stream=None):
+        """The rows k, v (bfloat16 [rows][n_kv_heads][head_dim]) into the cache, as
+        the last positions of lens[b]; rows_off as in include/c4s_layers.h."""
+        r = self._kv_rows(cache, k, v, lens, rows_off, "kv_append")
+        rc = lib().c4s_kv_append(self._h, cache.ref, C.byref(r), _stream_handle(stream))
+        if rc:
+            self._check(rc, "kv_append")
+
+    def kv_read(self, cache, k, v, lens, rows_off=None, stream=None):
+        """The cache's values at the last positions of lens[b] into the rows k, v
+        (bfloat16 or float32)."""
+        r = self._kv_rows(cache, k, v, lens, rows_off, "kv_read")
+        rc = lib().c4s_kv_read(self._h, cache.ref, C.byref(r), _stream_handle(stream))
+        if rc:
+            self._check(rc, "kv_read")
+
+    def attn(self, q, cache, lens, out, rows_off=None, max_new=None, scale=None, first=None, lse=None, stream=None):
+        """Attention of the rows q (bfloat16 [rows][n_heads][head_dim], the last
+        positions of lens[b]) over the cache, into out. max_new: the most rows a
+        sequence has (default: all rows); scale: 1 / sqrt(head_dim) by default."""
+        import torch
+        rows, heads, dim = q.shape
+        _need(q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and out.shape == q.shape,
+              "attn: q and out must be bfloat16 [rows][n_heads][head_dim]")
+        _need(dim == cache.head_dim, f"attn: q has head_dim {dim}, the cache {cache.head_dim}")
+        _need(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (rows, heads)),
+              "attn: lse must be contiguous float32 [rows][n_heads]")
+        qp, ldq = _heads(q, heads, dim, "attn: q")
+        op, ldo = _heads(out, heads, dim, "attn: out")
+        n = cache.n_seqs
+        d = Attn(qp, ldq, op, ldo, _p(lse), _i32(lens, n, "attn: lens"), _i32(rows_off, n + 1, "attn: rows_off"),
+                 _i32(first, n, "attn: first"), rows, rows if max_new is None else min(max_new, rows), heads,
+                 dim ** -0.5 if scale is None else scale)
+        rc = lib().c4s_attn(self._h, cache.ref, C.byref(d), _stream_handle(stream))
+        if rc:
+            self._check(rc, "attn")
 
     def hbm_probe(self, src, dst, nbytes, mode=0, stream=None):
         self._check(lib().c4s_hbm_probe(self._h, _p(src), _p(dst), nbytes, mode,
