@@ -87,7 +87,7 @@ typedef struct c4s_linear_desc {
   int32_t M, N, K;          /* N and K up to 4194304 */
   int32_t act;              /* C4S_ACT_* */
   const uint16_t* x;        /* [M][ldx] bf16 */
-  int64_t ldx;
+  int64_t ldx;              /* up to 4194304 */
   const void* weight;       /* [N][K] in wdtype */
   int32_t wdtype;           /* C4S_W_BF16 or C4S_W_Q8 */
   int32_t group;            /* C4S_W_Q8: 32, 64 or 128 */

@@ -237,19 +237,23 @@ def free_head_weights(hw: HeadWeights) -> None:
     lib().c4s_head_weights_free(C.byref(hw))
 
 
-def _dtype(t) -> int:
-    """C4S_DTYPE_* of a tensor that is bf16 or float32."""
-    import torch
-    if t.dtype == torch.bfloat16:
-        return BF16
-    if t.dtype == torch.float32:
-        return F32
-    raise ValueError(f"expected a bfloat16 or float32 tensor, got {t.dtype}")
-
+# The layer calls come once a layer and AR step, so what they check is checked
+# in few Python operations: messages are constants, nothing is formatted.
 
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
+
+
+def _dtype(t, what) -> int:
+    """C4S_DTYPE_* of a tensor that is bfloat16 or float32."""
+    import torch
+    d = t.dtype
+    if d is torch.bfloat16:
+        return BF16
+    if d is torch.float32:
+        return F32
+    raise ValueError(what)
 
 
 def _vector(t, n, what):
@@ -257,9 +261,9 @@ def _vector(t, n, what):
     import torch
     if t is None:
         return None
-    _need(t.dtype == torch.float32 and t.dim() == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1),
-          f"{what}: expected a contiguous float32 vector of {n}")
-    return t.data_ptr()
+    if t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(what)
 
 
 def _i32(t, n, what):
@@ -267,22 +271,30 @@ def _i32(t, n, what):
     import torch
     if t is None:
         return None
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1),
-          f"{what}: expected a contiguous int32 vector of {n}")
-    return t.data_ptr()
+    if t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(what)
 
 
-def _rows(t, what):
-    """(address, row stride) of a [rows][width] tensor whose rows are contiguous."""
-    _need(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what}: expected rows of contiguous values")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+def _rows(t, shape, what):
+    """(address, row stride) of a [rows][width] tensor of this shape whose rows are
+    contiguous; (None, 0) of None."""
+    if t is None:
+        return None, 0
+    if t.shape == shape:
+        ld, one = t.stride()
+        if one == 1 or shape[1] <= 1:
+            return t.data_ptr(), (ld if shape[0] > 1 else shape[1])
+    raise ValueError(what)
 
 
-def _heads(t, heads, dim, what):
-    """(address, row stride) of a [rows][heads][dim] tensor whose rows are contiguous."""
-    _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == dim and (t.stride(2) == 1 or dim <= 1) and
-          (heads == 1 or t.stride(1) == dim), f"{what}: expected [rows][{heads}][{dim}], a row contiguous")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else heads * dim)
+def _heads(t, shape, what):
+    """(address, row stride) of a [rows][heads][dim] tensor of this shape whose rows are contiguous."""
+    if t.shape == shape:
+        ld, dim, one = t.stride()
+        if one == 1 and (dim == shape[2] or shape[1] == 1):
+            return t.data_ptr(), (ld if shape[0] > 1 else shape[1] * shape[2])
+    raise ValueError(what)
 
 
 class KvCache:
@@ -472,29 +484,40 @@ class Context:
                     "lmhead_sample_noalloc")
 
     # ---- the decoder layer's operators (include/c4s_layers.h) ---------------------------
+    def _queue(self, stream):
+        """The HIP stream of a call: the given one, or this device's current one."""
+        if stream is None:
+            import torch
+            return torch._C._cuda_getCurrentRawStream(self.device)
+        return _stream_handle(stream)
+
     def block_norm(self, x, gamma, beta, out, y=None, x_out=None, post=False, post_gamma=None, post_beta=None,
                    gate=None, gate_rows=1, scale=1.0, eps=1e-5, rms=False, stream=None):
         """r = x + scale * gate (.) u with u = y, or norm(y) when post; x_out = r;
         out = norm(r). x, y, x_out, out: [rows][D], bfloat16 or float32; gate:
         float32 [ceil(rows / gate_rows)][D]; without y, r = x."""
-        M, D = x.shape
-        for name, t in (("y", y), ("x_out", x_out), ("out", out)):
-            _need(t is None or tuple(t.shape) == (M, D), f"block_norm: {name} must be [{M}][{D}]")
-        _need(x_out is None or x_out.dtype == x.dtype, "block_norm: x_out must have x's dtype")
-        g, ldg = (None, 0)
+        shape = x.shape
+        M, D = shape
+        xt = _dtype(x, "block_norm: x must be bfloat16 or float32")
+        yt = F32 if y is None else _dtype(y, "block_norm: y must be bfloat16 or float32")
+        ot = F32 if out is None else _dtype(out, "block_norm: out must be bfloat16 or float32")
+        if x_out is not None and x_out.dtype is not x.dtype:
+            raise ValueError("block_norm: x_out must have x's dtype")
+        g, ldg = None, 0
         if gate is not None:
-            _need(gate_rows >= 1 and gate.shape[0] * gate_rows >= M and gate.shape[1] == D and _dtype(gate) == F32,
-                  "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
-            g, ldg = _rows(gate, "block_norm: gate")
-        xp, ldx = _rows(x, "block_norm: x")
-        yp, ldy = (None, 0) if y is None else _rows(y, "block_norm: y")
-        xo, ldxo = (None, 0) if x_out is None else _rows(x_out, "block_norm: x_out")
-        op, ldo = (None, 0) if out is None else _rows(out, "block_norm: out")
-        d = Norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, _dtype(x), F32 if y is None else _dtype(y), yp,
-                 ldy, 1 if post else 0, gate_rows, _vector(post_gamma, D, "block_norm: post_gamma"),
-                 _vector(post_beta, D, "block_norm: post_beta"), g, ldg, scale, F32 if out is None else _dtype(out),
-                 _vector(gamma, D, "block_norm: gamma"), _vector(beta, D, "block_norm: beta"), xo, ldxo, op, ldo)
-        rc = lib().c4s_block_norm(self._h, C.byref(d), _stream_handle(stream))
+            if not (gate_rows >= 1 and gate.shape[0] * gate_rows >= M and _dtype(gate, "block_norm: gate must be float32") == F32):
+                raise ValueError("block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+            g, ldg = _rows(gate, (gate.shape[0], D), "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+        xp, ldx = _rows(x, shape, "block_norm: rows of x must be contiguous")
+        yp, ldy = _rows(y, shape, "block_norm: y must have x's shape, its rows contiguous")
+        xo, ldxo = _rows(x_out, shape, "block_norm: x_out must have x's shape, its rows contiguous")
+        op, ldo = _rows(out, shape, "block_norm: out must have x's shape, its rows contiguous")
+        d = Norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, xt, yt, yp, ldy, 1 if post else 0, gate_rows,
+                 _vector(post_gamma, D, "block_norm: post_gamma must be a float32 vector of D"),
+                 _vector(post_beta, D, "block_norm: post_beta must be a float32 vector of D"), g, ldg, scale, ot,
+                 _vector(gamma, D, "block_norm: gamma must be a float32 vector of D"),
+                 _vector(beta, D, "block_norm: beta must be a float32 vector of D"), xo, ldxo, op, ldo)
+        rc = lib().c4s_block_norm(self._h, C.byref(d), self._queue(stream))
         if rc:
             self._check(rc, "block_norm")
 
@@ -505,48 +528,57 @@ class Context:
         import torch
         M, K = x.shape
         N = weight.shape[0]
-        _need(x.dtype == torch.bfloat16 and weight.dim() == 2 and weight.shape[1] == K and weight.is_contiguous(),
-              "linear: x must be bfloat16 [M][K], weight contiguous [N][K]")
-        _need(tuple(out.shape) == (M, N) and (residual is None or tuple(residual.shape) == (M, N)),
-              f"linear: out and residual must be [{M}][{N}]")
-        _need(weight.dtype == (torch.bfloat16 if quant is None else torch.uint8),
-              "linear: weights are bfloat16, or uint8 with quant=(scales, offsets, group)")
-        ws, wb, group = quant if quant is not None else (None, None, 0)
-        for t in (ws, wb):
-            _need(t is None or (group > 0 and t.dtype == torch.float32 and t.is_contiguous() and
-                                tuple(t.shape) == (N, K // group)), "linear: scales and offsets must be float32 [N][K / group]")
-        _need(act in ACTS, f"linear: act must be one of {', '.join(ACTS)}")
-        xp, ldx = _rows(x, "linear: x")
-        op, ldo = _rows(out, "linear: out")
-        rp, ldr = (None, 0) if residual is None else _rows(residual, "linear: residual")
-        d = Linear(M, N, K, ACTS[act], xp, ldx, weight.data_ptr(), W_BF16 if quant is None else W_Q8, group, _p(ws),
-                   _p(wb), _vector(bias, N, "linear: bias"), rp, ldr, F32 if residual is None else _dtype(residual),
-                   _dtype(out), op, ldo)
-        rc = lib().c4s_linear(self._h, C.byref(d), _stream_handle(stream))
+        if not (x.dtype is torch.bfloat16 and weight.shape == (N, K) and weight.is_contiguous()):
+            raise ValueError("linear: x must be bfloat16 [M][K], weight contiguous [N][K]")
+        ws = wb = None
+        wt, group = W_BF16, 0
+        if quant is not None:
+            ws, wb, group = quant
+            wt = W_Q8
+            if not (group > 0 and ws.dtype is torch.float32 and wb.dtype is torch.float32 and
+                    ws.shape == wb.shape == (N, K // group) and ws.is_contiguous() and wb.is_contiguous()):
+                raise ValueError("linear: scales and offsets must be contiguous float32 [N][K / group]")
+            ws, wb = ws.data_ptr(), wb.data_ptr()
+        if weight.dtype is not (torch.bfloat16 if quant is None else torch.uint8):
+            raise ValueError("linear: weights are bfloat16, or uint8 with quant=(scales, offsets, group)")
+        if act not in ACTS:
+            raise ValueError("linear: act must be none, gelu, silu or relu")
+        xp, ldx = _rows(x, (M, K), "linear: rows of x must be contiguous")
+        op, ldo = _rows(out, (M, N), "linear: out must be [M][N], its rows contiguous")
+        rp, ldr = _rows(residual, (M, N), "linear: residual must be [M][N], its rows contiguous")
+        d = Linear(M, N, K, ACTS[act], xp, ldx, weight.data_ptr(), wt, group, ws, wb,
+                   _vector(bias, N, "linear: bias must be a float32 vector of N"), rp, ldr,
+                   F32 if residual is None else _dtype(residual, "linear: residual must be bfloat16 or float32"),
+                   _dtype(out, "linear: out must be bfloat16 or float32"), op, ldo)
+        rc = lib().c4s_linear(self._h, C.byref(d), self._queue(stream))
         if rc:
             self._check(rc, "linear")
 
-    def _kv_rows(self, cache, k, v, lens, rows_off, what):
-        heads, dim = cache.n_kv_heads, cache.head_dim
-        _need(k.shape[0] == v.shape[0] and k.dtype == v.dtype, f"{what}: k and v must be alike")
-        kp, ldk = _heads(k, heads, dim, f"{what}: k")
-        vp, ldv = _heads(v, heads, dim, f"{what}: v")
-        return KvRows(kp, vp, ldk, ldv, _i32(lens, cache.n_seqs, f"{what}: lens"),
-                      _i32(rows_off, cache.n_seqs + 1, f"{what}: rows_off"), k.shape[0], _dtype(k))
+    @staticmethod
+    def _kv_rows(cache, k, v, lens, rows_off):
+        shape = (k.shape[0], cache.n_kv_heads, cache.head_dim)
+        kp, ldk = _heads(k, shape, "kv rows: k must be [rows][n_kv_heads][head_dim], a row contiguous")
+        vp, ldv = _heads(v, shape, "kv rows: v must be [rows][n_kv_heads][head_dim], a row contiguous")
+        t = _dtype(k, "kv rows: k and v must be bfloat16 or float32")
+        if v.dtype is not k.dtype:
+            raise ValueError("kv rows: k and v must have one dtype")
+        return KvRows(kp, vp, ldk, ldv, _i32(lens, cache.n_seqs, "kv rows: lens must be an int32 vector of n_seqs"),
+                      _i32(rows_off, cache.n_seqs + 1, "kv rows: rows_off must be an int32 vector of n_seqs + 1"),
+                      shape[0], t)
 
     def kv_append(self, cache, k, v, lens, rows_off=None, stream=None):
         """The rows k, v (bfloat16 [rows][n_kv_heads][head_dim]) into the cache, as
         the last positions of lens[b]; rows_off as in include/c4s_layers.h."""
-        r = self._kv_rows(cache, k, v, lens, rows_off, "kv_append")
-        rc = lib().c4s_kv_append(self._h, cache.ref, C.byref(r), _stream_handle(stream))
+        r = self._kv_rows(cache, k, v, lens, rows_off)
+        rc = lib().c4s_kv_append(self._h, cache.ref, C.byref(r), self._queue(stream))
         if rc:
             self._check(rc, "kv_append")
 
     def kv_read(self, cache, k, v, lens, rows_off=None, stream=None):
         """The cache's values at the last positions of lens[b] into the rows k, v
         (bfloat16 or float32)."""
-        r = self._kv_rows(cache, k, v, lens, rows_off, "kv_read")
-        rc = lib().c4s_kv_read(self._h, cache.ref, C.byref(r), _stream_handle(stream))
+        r = self._kv_rows(cache, k, v, lens, rows_off)
+        rc = lib().c4s_kv_read(self._h, cache.ref, C.byref(r), self._queue(stream))
         if rc:
             self._check(rc, "kv_read")
 
@@ -555,19 +587,22 @@ class Context:
         positions of lens[b]) over the cache, into out. max_new: the most rows a
         sequence has (default: all rows); scale: 1 / sqrt(head_dim) by default."""
         import torch
-        rows, heads, dim = q.shape
-        _need(q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16 and out.shape == q.shape,
-              "attn: q and out must be bfloat16 [rows][n_heads][head_dim]")
-        _need(dim == cache.head_dim, f"attn: q has head_dim {dim}, the cache {cache.head_dim}")
-        _need(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (rows, heads)),
-              "attn: lse must be contiguous float32 [rows][n_heads]")
-        qp, ldq = _heads(q, heads, dim, "attn: q")
-        op, ldo = _heads(out, heads, dim, "attn: out")
+        shape = q.shape
+        rows, heads, dim = shape
+        if not (q.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and dim == cache.head_dim):
+            raise ValueError("attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's")
+        if lse is not None and not (lse.dtype is torch.float32 and lse.shape == (rows, heads) and lse.is_contiguous()):
+            raise ValueError("attn: lse must be contiguous float32 [rows][n_heads]")
+        qp, ldq = _heads(q, shape, "attn: rows of q must be contiguous")
+        op, ldo = _heads(out, shape, "attn: out must have q's shape, its rows contiguous")
         n = cache.n_seqs
-        d = Attn(qp, ldq, op, ldo, _p(lse), _i32(lens, n, "attn: lens"), _i32(rows_off, n + 1, "attn: rows_off"),
-                 _i32(first, n, "attn: first"), rows, rows if max_new is None else min(max_new, rows), heads,
+        d = Attn(qp, ldq, op, ldo, None if lse is None else lse.data_ptr(),
+                 _i32(lens, n, "attn: lens must be an int32 vector of n_seqs"),
+                 _i32(rows_off, n + 1, "attn: rows_off must be an int32 vector of n_seqs + 1"),
+                 _i32(first, n, "attn: first must be an int32 vector of n_seqs"), rows,
+                 rows if max_new is None or max_new > rows else max_new, heads,
                  dim ** -0.5 if scale is None else scale)
-        rc = lib().c4s_attn(self._h, cache.ref, C.byref(d), _stream_handle(stream))
+        rc = lib().c4s_attn(self._h, cache.ref, C.byref(d), self._queue(stream))
         if rc:
             self._check(rc, "attn")
 

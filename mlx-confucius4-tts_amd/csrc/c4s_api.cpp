@@ -235,6 +235,7 @@ int c4s_destroy(c4s_ctx* ctx) {
     if (p) (void)hipFree(p);
   ctx->rows_ws.clear();
   ctx->logits_ws.clear();
+  ctx->layer_ws.clear();
   if (ctx->host_stream) (void)hipStreamDestroy(ctx->host_stream);
   if (ctx->side) (void)hipStreamDestroy(ctx->side);
   if (ctx->scan_s) (void)hipStreamDestroy(ctx->scan_s);

@@ -88,11 +88,11 @@ __device__ __forceinline__ void part_odd(uint32_t& w, uint32_t& odd) {
 constexpr int kRows = 16;
 constexpr int kKeys = 64;    // positions a wave takes at a time
 constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kAttnThreads = 64 * kWaves;
 
 // DH: the head's dims rounded up to 64, 128 or 256.
 template <int DH, bool Q8>
-__global__ __launch_bounds__(kThreads) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads) void k_attn(AttnArgs a) {
   constexpr int kSteps = DH / 32, kTiles = DH / 16;
   __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
   __shared__ __align__(16) float so[kWaves - 1][kRows][DH + 4];
@@ -299,14 +299,14 @@ hipError_t launch_attn(const AttnArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(((int64_t)a.max_new * a.shared + kRows - 1) / kRows * a.c.n_heads), a.c.n_seqs);
   const bool q8 = a.c.store == C4S_KV_Q8;
   if (a.c.dim <= 64) {
-    if (q8) hipLaunchKernelGGL((k_attn<64, true>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<64, false>), grid, dim3(kThreads), 0, s, a);
+    if (q8) hipLaunchKernelGGL((k_attn<64, true>), grid, dim3(kAttnThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<64, false>), grid, dim3(kAttnThreads), 0, s, a);
   } else if (a.c.dim <= 128) {
-    if (q8) hipLaunchKernelGGL((k_attn<128, true>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<128, false>), grid, dim3(kThreads), 0, s, a);
+    if (q8) hipLaunchKernelGGL((k_attn<128, true>), grid, dim3(kAttnThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<128, false>), grid, dim3(kAttnThreads), 0, s, a);
   } else {
-    if (q8) hipLaunchKernelGGL((k_attn<256, true>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<256, false>), grid, dim3(kThreads), 0, s, a);
+    if (q8) hipLaunchKernelGGL((k_attn<256, true>), grid, dim3(kAttnThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<256, false>), grid, dim3(kAttnThreads), 0, s, a);
   }
   return hipGetLastError();
 }

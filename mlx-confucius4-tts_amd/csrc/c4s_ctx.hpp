@@ -35,6 +35,31 @@ struct HipRt {
   bool wait(hipStream_t s, hipEvent_t e) { return ok(hipStreamWaitEvent(s, e, 0)); }
 };
 
+// That of a pool whose workspaces begin zeroed: by a kernel on a stream of its
+// own, which is never captured.
+struct ZeroedRt : HipRt {
+  hipStream_t stream = nullptr;
+  bool alloc(void** p, size_t bytes) {
+    if (!HipRt::alloc(p, bytes)) return false;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    bool fine = ok(hipThreadExchangeStreamCaptureMode(&mode));
+    if (fine) {
+      fine = ok(c4s::launch_zero(*p, bytes < c4s::kLayerZeroed ? bytes : c4s::kLayerZeroed, stream)) &&
+             ok(hipStreamSynchronize(stream));
+      const hipError_t e = err;
+      (void)hipThreadExchangeStreamCaptureMode(&mode);
+      err = e;
+    }
+    if (!fine) {
+      const hipError_t e = err;
+      (void)hipFree(*p);
+      *p = nullptr;
+      err = e;
+    }
+    return fine;
+  }
+};
+
 struct c4s_ctx {
   int device = 0;
   std::string err;
@@ -43,6 +68,7 @@ struct c4s_ctx {
   size_t ws_bytes = 0;
   c4s::StreamPool<HipRt> rows_ws;     // large-vocabulary rows: slices, lists, exact-pass keys
   c4s::StreamPool<HipRt> logits_ws;   // LM head + sample: logits when the caller gives none
+  c4s::StreamPool<ZeroedRt> layer_ws; // decoder layer: counters, split sums' parts
   // host-helper staging: pinned host memory that the device maps
   void* hstage = nullptr;
   size_t hstage_bytes = 0;
@@ -109,7 +135,8 @@ inline bool is_capturing(hipStream_t s) {
 }
 
 // The stream's workspace of `pool` for a call about to be queued on `s`.
-inline int pool_take(c4s_ctx* ctx, c4s::StreamPool<HipRt>& pool, hipStream_t s, size_t need, const char* what, void** out) {
+template <class Rt>
+int pool_take(c4s_ctx* ctx, c4s::StreamPool<Rt>& pool, hipStream_t s, size_t need, const char* what, void** out) {
   switch (pool.take(s, is_capturing(s), need, out)) {
     case c4s::PoolResult::kOk: return C4S_OK;
     case c4s::PoolResult::kWouldGrow:

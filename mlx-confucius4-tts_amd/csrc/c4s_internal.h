@@ -135,6 +135,11 @@ constexpr size_t kNoAllocBytes = (size_t)8 << 20;
 // This device's address of that scratch (the current device).
 hipError_t noalloc_scratch(void** ptr);
 
+// Bytes at the start of a decoder layer's workspace that are zero between calls.
+constexpr size_t kLayerZeroed = (size_t)1 << 18;
+// Zeroes `bytes` (a multiple of 4) from p on.
+hipError_t launch_zero(void* p, size_t bytes, hipStream_t s);
+
 size_t rows_lds_bytes(int vocab);
 size_t rows_global_lds_bytes(int vocab);
 size_t stream_lds_bytes(int vocab, int unused);

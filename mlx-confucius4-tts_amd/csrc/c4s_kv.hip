@@ -16,7 +16,7 @@ namespace c4s {
 namespace {
 
 constexpr int kTile = 16;          // rows a workgroup takes
-constexpr int kThreads = 256;
+constexpr int kKvThreads = 256;
 constexpr int kMaxDim = 256;
 
 // Where packed row r lies in the cache: its page and place in it, or -1 when
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t to_bf16(float f) {   // round to nearest eve
   return __builtin_bit_cast(uint16_t, (__bf16)f);
 }
 
-__global__ __launch_bounds__(kThreads) void k_kv_append(KvArgs c, KvRowsArgs rows) {
+__global__ __launch_bounds__(kKvThreads) void k_kv_append(KvArgs c, KvRowsArgs rows) {
   __shared__ __align__(16) uint16_t tile[kMaxDim][kTile + 2];
   __shared__ Place places[kTile];
   const int head = blockIdx.y, row = threadIdx.x / 16, l = threadIdx.x % 16;
@@ -124,14 +124,14 @@ __global__ __launch_bounds__(kThreads) void k_kv_append(KvArgs c, KvRowsArgs row
   const Place pv = places[threadIdx.x % 16];
   if (pv.page < 0) return;
   const int64_t base = (pv.page * c.n_heads + head) * (int64_t)ps * dim + pv.at;
-  for (int d = threadIdx.x / 16; d < dim; d += kThreads / 16) {
+  for (int d = threadIdx.x / 16; d < dim; d += kKvThreads / 16) {
     const uint16_t h = tile[d][threadIdx.x % 16];
     if (q8) static_cast<uint8_t*>(c.v)[base + (int64_t)d * ps] = (uint8_t)h;
     else static_cast<uint16_t*>(c.v)[base + (int64_t)d * ps] = h;
   }
 }
 
-__global__ __launch_bounds__(kThreads) void k_kv_read(KvArgs c, KvRowsArgs rows) {
+__global__ __launch_bounds__(kKvThreads) void k_kv_read(KvArgs c, KvRowsArgs rows) {
   __shared__ __align__(16) float tile[kMaxDim][kTile + 1];
   __shared__ Place places[kTile];
   const int head = blockIdx.y, row = threadIdx.x / 16, l = threadIdx.x % 16;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(KvArgs c, KvRowsArgs rows)
     const int64_t slot = (pv.page * c.n_heads + head) * (int64_t)ps + pv.at;
     const int64_t base = (pv.page * c.n_heads + head) * (int64_t)ps * dim + pv.at;
     const float scale = q8 && pv.page >= 0 ? c.v_scale[slot] : 1.0f;
-    for (int d = threadIdx.x / 16; d < dim; d += kThreads / 16) {
+    for (int d = threadIdx.x / 16; d < dim; d += kKvThreads / 16) {
       float v = 0.0f;
       if (pv.page >= 0)
         v = q8 ? (float)static_cast<const int8_t*>(c.v)[base + (int64_t)d * ps] * scale
@@ -195,12 +195,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(KvArgs c, KvRowsArgs rows)
 }  // namespace
 
 hipError_t launch_kv_append(const KvArgs& c, const KvRowsArgs& r, hipStream_t s) {
-  hipLaunchKernelGGL(k_kv_append, dim3((r.n_rows + kTile - 1) / kTile, c.n_heads), dim3(kThreads), 0, s, c, r);
+  hipLaunchKernelGGL(k_kv_append, dim3((r.n_rows + kTile - 1) / kTile, c.n_heads), dim3(kKvThreads), 0, s, c, r);
   return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvArgs& c, const KvRowsArgs& r, hipStream_t s) {
-  hipLaunchKernelGGL(k_kv_read, dim3((r.n_rows + kTile - 1) / kTile, c.n_heads), dim3(kThreads), 0, s, c, r);
+  hipLaunchKernelGGL(k_kv_read, dim3((r.n_rows + kTile - 1) / kTile, c.n_heads), dim3(kKvThreads), 0, s, c, r);
   return hipGetLastError();
 }
 

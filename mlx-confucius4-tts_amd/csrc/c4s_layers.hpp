@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/c4s_layers.h"
+#include "c4s_internal.h"
 
 namespace c4s {
 
@@ -44,8 +45,15 @@ struct AttnArgs {
   float scale;
 };
 
+// What a call needs of its stream's workspace: counters that are zero between
+// calls (a kernel that uses them leaves them so), and floats.
+struct LayerSpace {
+  int64_t counters = 0, floats = 0;
+};
+
 hipError_t launch_block_norm(const c4s_norm& a, hipStream_t s);
-hipError_t launch_linear(const c4s_linear_desc& a, hipStream_t s);
+LayerSpace linear_space(const c4s_linear_desc& a);
+hipError_t launch_linear(const c4s_linear_desc& a, uint32_t* counters, float* space, hipStream_t s);
 hipError_t launch_kv_append(const KvArgs& c, const KvRowsArgs& r, hipStream_t s);
 hipError_t launch_kv_read(const KvArgs& c, const KvRowsArgs& r, hipStream_t s);
 hipError_t launch_attn(const AttnArgs& a, hipStream_t s);

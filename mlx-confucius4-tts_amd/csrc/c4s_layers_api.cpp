@@ -36,6 +36,22 @@ int entry(c4s_ctx* ctx, const void* desc, const char* what, Body body) {
   }
 }
 
+// As queue(), with `need` of the stream's workspace: launch(counters, floats).
+template <class Launch>
+int queue_with(c4s_ctx* ctx, const c4s::LayerSpace& need, hipStream_t s, const char* what, Launch launch) {
+  DeviceGuard g(ctx->device);
+  if (g.err != hipSuccess) return hip_fail(ctx, g.err, "hipSetDevice");
+  if (need.floats == 0) return launched(ctx, launch(nullptr, nullptr), what);
+  if (need.counters * 4 > (int64_t)c4s::kLayerZeroed) return fail(ctx, C4S_EINVAL, std::string(what) + ": too many parts");
+  ctx->layer_ws.runtime().stream = ctx->host_stream;
+  void* ws = nullptr;
+  const int rc = c4s::pool_take(ctx, ctx->layer_ws, s, c4s::kLayerZeroed + (size_t)need.floats * 4, "layer workspace", &ws);
+  if (rc) return rc;
+  const hipError_t e = launch(static_cast<uint32_t*>(ws), reinterpret_cast<float*>(static_cast<char*>(ws) + c4s::kLayerZeroed));
+  ctx->layer_ws.queued(s, c4s::is_capturing(s));
+  return launched(ctx, e, what);
+}
+
 template <class Launch>
 int queue(c4s_ctx* ctx, const char* what, Launch launch) {
   DeviceGuard g(ctx->device);
@@ -72,6 +88,7 @@ int check_linear(c4s_ctx* ctx, const c4s_linear_desc* a) {
       return fail(ctx, C4S_EINVAL, "linear: group must be 32, 64 or 128 and divide K");
   }
   if (!is_dtype(a->out_dtype) || (a->residual && !is_dtype(a->res_dtype))) return fail(ctx, C4S_EINVAL, "linear: unknown dtype");
+  if (a->ldx > 1 << 22) return fail(ctx, C4S_EINVAL, "linear: ldx above 4194304");
   if (a->ldx < a->K || a->ld_out < a->N || (a->residual && a->ld_res < a->N))
     return fail(ctx, C4S_EINVAL, "linear: a row stride is below its row");
   if ((bits(a->x) & 15u) || (a->ldx & 7) || (bits(a->weight) & (a->wdtype == C4S_W_Q8 ? 7u : 15u)))
@@ -159,7 +176,9 @@ int c4s_linear(c4s_ctx* ctx, const c4s_linear_desc* lin, void* stream) {
   return entry(ctx, lin, "linear", [&] {
     const int rc = check_linear(ctx, lin);
     if (rc || lin->M == 0) return rc;
-    return queue(ctx, "linear launch", [&] { return c4s::launch_linear(*lin, static_cast<hipStream_t>(stream)); });
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return queue_with(ctx, c4s::linear_space(*lin), s, "linear launch",
+                      [&](uint32_t* n, float* f) { return c4s::launch_linear(*lin, n, f, s); });
   });
 }
 

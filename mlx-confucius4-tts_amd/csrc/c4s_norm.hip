@@ -114,11 +114,11 @@ struct Row {
   }
 };
 
-constexpr int kThreads = 256;
+constexpr int kNormThreads = 256;
 
 template <int T, int E, int V>
-__global__ __launch_bounds__(T > kThreads ? T : kThreads) void k_block_norm(c4s_norm a) {
-  constexpr int kRows = T < kThreads ? kThreads / T : 1;
+__global__ __launch_bounds__(T > kNormThreads ? T : kNormThreads) void k_block_norm(c4s_norm a) {
+  constexpr int kRows = T < kNormThreads ? kNormThreads / T : 1;
   __shared__ float part[16];
   const int m = blockIdx.x * kRows + (kRows > 1 ? (int)threadIdx.x / T : 0);
   if (m >= a.M) return;   // whole waves: with T > 64 a workgroup is one row
@@ -154,8 +154,8 @@ __global__ __launch_bounds__(T > kThreads ? T : kThreads) void k_block_norm(c4s_
 
 template <int T, int E, int V>
 hipError_t launch(const c4s_norm& a, hipStream_t s) {
-  constexpr int kRows = T < kThreads ? kThreads / T : 1;
-  hipLaunchKernelGGL((k_block_norm<T, E, V>), dim3((a.M + kRows - 1) / kRows), dim3(T > kThreads ? T : kThreads), 0, s, a);
+  constexpr int kRows = T < kNormThreads ? kNormThreads / T : 1;
+  hipLaunchKernelGGL((k_block_norm<T, E, V>), dim3((a.M + kRows - 1) / kRows), dim3(T > kNormThreads ? T : kNormThreads), 0, s, a);
   return hipGetLastError();
 }
 
@@ -164,7 +164,16 @@ bool by_four(const void* p, int64_t ld, int32_t dtype) {
   return !p || (ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (dtype == C4S_DTYPE_BF16 ? 8 : 16) == 0);
 }
 
+__global__ void k_zero(uint32_t* p, size_t n) {
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) p[i] = 0u;
+}
+
 }  // namespace
+
+hipError_t launch_zero(void* p, size_t bytes, hipStream_t s) {
+  hipLaunchKernelGGL(k_zero, dim3(64), dim3(256), 0, s, static_cast<uint32_t*>(p), bytes / 4);
+  return hipGetLastError();
+}
 
 hipError_t launch_block_norm(const c4s_norm& a, hipStream_t s) {
   const bool four = a.D % 4 == 0 && by_four(a.x, a.ldx, a.x_dtype) && by_four(a.y, a.ldy, a.y_dtype) &&

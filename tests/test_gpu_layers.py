@@ -125,6 +125,14 @@ LINEARS = [  # M, N, K, weight, group, act, residual, out, bias
     (1025, 515, 1288, "bf16", 0, "silu", "f32", "f32", True),
     (513, 1280, 1280, "q8", 32, "none", "bf16", "f32", True),
     (1500, 2560, 256, "bf16", 0, "none", "f32", "bf16", True),
+    # tiles of many rows: 128 and 256 wide, the last ones partial, inputs that end inside a stage
+    (2050, 1283, 1288, "bf16", 0, "silu", "f32", "f32", True),
+    (2049, 1300, 8, "bf16", 0, "none", None, "f32", False),
+    (4100, 2053, 72, "bf16", 0, "gelu", "bf16", "f32", True),
+    (4099, 2052, 200, "bf16", 0, "relu", "f32", "bf16", False),
+    (2600, 1281, 96, "q8", 32, "silu", "f32", "f32", True),
+    (1300, 2560, 256, "q8", 128, "none", None, "bf16", True),
+    (1411, 2564, 192, "q8", 64, "none", "bf16", "f32", False),
 ]
 
 
@@ -157,23 +165,23 @@ def test_linear(gpu_ctx, M, N, K, weight, group, act, res, ot, bias):
     assert (out[:, N:] == 7).all()
 
 
-@pytest.mark.parametrize("M", [3, 200])
-def test_linear_in_place_residual(gpu_ctx, M):
-    g, x, w, _ = _linear_inputs(M, 256, 512, "bf16", 0, 5)
-    r = torch.randn((M, 256), generator=g).cuda()
+@pytest.mark.parametrize("M,N", [(3, 256), (200, 256), (2100, 1400), (4100, 2100)])
+def test_linear_in_place_residual(gpu_ctx, M, N):
+    g, x, w, _ = _linear_inputs(M, N, 512, "bf16", 0, 5)
+    r = torch.randn((M, N), generator=g).cuda()
     out = torch.empty_like(r)
     gpu_ctx.linear(x.cuda(), w.cuda(), out, residual=r)
     gpu_ctx.linear(x.cuda(), w.cuda(), r, residual=r)
     assert torch.equal(out, r)
 
 
-@pytest.mark.parametrize("M", [5, 300])
+@pytest.mark.parametrize("M,N", [(5, 200), (300, 200), (2600, 1300), (4100, 2100)])
 @pytest.mark.parametrize("weight,group", [("bf16", 0), ("q8", 64)])
-def test_linear_rows_do_not_touch_each_other(gpu_ctx, M, weight, group):
+def test_linear_rows_do_not_touch_each_other(gpu_ctx, M, N, weight, group):
     """A row of NaN, inf or huge values leaves the other rows as they are, bit for bit."""
-    _, x, w, quant = _linear_inputs(M, 200, 256, weight, group, 9)
+    _, x, w, quant = _linear_inputs(M, N, 256, weight, group, 9)
     q = None if quant is None else (quant[0].cuda(), quant[1].cuda(), group)
-    a, b = (torch.empty((M, 200), device="cuda") for _ in "ab")
+    a, b = (torch.empty((M, N), device="cuda") for _ in "ab")
     gpu_ctx.linear(x.cuda(), w.cuda(), a, act="gelu", quant=q)
     x[2] = torch.tensor([np.nan, np.inf, -np.inf, 3e38] * 64).to(torch.bfloat16)
     gpu_ctx.linear(x.cuda(), w.cuda(), b, act="gelu", quant=q)
