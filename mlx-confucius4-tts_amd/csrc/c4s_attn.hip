@@ -1,25 +1,21 @@
 // Attention of new tokens over the paged cache (c4s_attn, include/c4s_layers.h).
 //
-// A workgroup has 16 rows (token, query head) of one sequence and key head; its
-// waves take blocks of 64 positions in turn, each with a running maximum and
-// sum of its own, and are joined at the end in LDS.
-//
 // Both products run transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane
-// always holds one row (column l % 16 of the results): the maximum, the sum and
-// the rescaling are a lane's own, but for two steps across the four lanes that
-// share a row. Which positions of the block a matrix row of S^T stands for is
-// free; row 4 g + i of tile t is position 16 g + 4 t + i, so that lane group g
-// ends up with the weights of positions 16 g .. 16 g + 15, which is what P^T wants
-// of it as the next product's operand, and which lie next to each other in a
-// page of the values. Nothing is shuffled or transposed in between, and keys
-// and values go from memory straight into the matrix engine's registers.
-//
-// The weights enter the second product as bf16 pairs (hi + lo, about 2^-17
-// relative): rounded once to bf16 they would add an error of the size of the
-// output's own rounding.
+// always holds one row (token, query head; column l % 16 of the results): the
+// maximum, the sum and the rescaling are a lane's own, but for two steps across
+// the four lanes that share a row. Which positions of a block a matrix row of
+// S^T stands for is free; in a block of B positions row 4 g + i of tile t is
+// position (B / 4) g + 4 t + i, so that lane group g ends up with the weights of
+// B / 4 positions in order, which is what P^T wants of it as the next product's
+// operand, and which lie next to each other in a page of the values. Nothing is
+// shuffled or transposed in between.
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cstdlib>
+
+#include "c4s_join.hpp"
 #include "c4s_layers.hpp"
 
 namespace c4s {
@@ -27,7 +23,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -49,10 +44,14 @@ __device__ __forceinline__ uint4 codes(uint2 q) {
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = i < 2 ? q.x : q.y;
     const float a = (float)(int8_t)(w >> (16 * (i & 1))), b = (float)(int8_t)(w >> (16 * (i & 1) + 8));
-    o[i] = (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xFFFF0000u);
+    o[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   // the upper halves
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
+
+// Keeps what is computed from w behind this place (the conversion of a block's
+// codes would otherwise move up to their load, at twice the registers).
+__device__ __forceinline__ void here(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
 
 // Over the four lanes that share a row.
 __device__ __forceinline__ float max4(float v) {
@@ -70,13 +69,13 @@ __device__ __forceinline__ uint4 keep(uint4 w, int at, int lo, int hi) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = at + 2 * i;
-    v[i] &= (j >= lo && j < hi ? 0xFFFFu : 0u) | (j + 1 >= lo && j + 1 < hi ? 0xFFFF0000u : 0u);
+    v[i] &= (((j >= lo) & (j < hi)) ? 0xFFFFu : 0u) | (((j + 1 >= lo) & (j + 1 < hi)) ? 0xFFFF0000u : 0u);
   }
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ bool odd_exp(uint32_t w) {   // either half inf or NaN
-  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+__device__ __forceinline__ int odd_exp(uint32_t w) {   // either half inf or NaN
+  return (int)((w & 0x7F80u) == 0x7F80u) | (int)((w & 0x7F800000u) == 0x7F800000u);
 }
 
 // The finite halves of w, and ones where the others were.
@@ -85,230 +84,421 @@ __device__ __forceinline__ void part_odd(uint32_t& w, uint32_t& odd) {
   w &= (odd & 0xFFFFu ? 0u : 0xFFFFu) | (odd >> 16 ? 0u : 0xFFFF0000u);
 }
 
-constexpr int kRows = 16;
-constexpr int kKeys = 64;    // positions a wave takes at a time
+// The rows of one sequence, and what they see.
+struct Seq {
+  int row0, n_new, past, fst, cap;   // n_new 0: nothing to do
+  __device__ __forceinline__ Seq(const AttnArgs& a, int seq) {
+    row0 = seq;
+    n_new = 1;
+    int n = 1;
+    if (a.off) {
+      row0 = a.off[seq];
+      n = a.off[seq + 1] - row0;
+      n_new = row0 < 0 ? 0 : min(min(n, a.n_rows - row0), a.max_new);
+    } else if (seq >= a.n_rows) {
+      n_new = 0;
+    }
+    past = a.lens[seq] - n;
+    cap = a.c.max_pages << a.c.page_shift;
+    fst = a.first ? min(max(a.first[seq], 0), cap) : 0;
+  }
+};
+
+constexpr int kRows = 16;   // rows of a workgroup
+
+// ---- few rows -----------------------------------------------------------------------------
+//
+// A single token's step reads the cache once and computes next to nothing: what
+// counts is how many bytes are on their way. A workgroup has 16 rows of one
+// sequence and key head and a chunk of its positions; its four waves take
+// blocks of KEYS positions in turn, each with a running maximum and sum of its
+// own. Keys and values go from memory straight into the matrix engine's
+// registers; a block's keys are asked for as soon as the block before it has
+// given its scores, its values as soon as the values before them have been
+// used, and its pages one block earlier still, so that a wave always has about
+// a block in flight and never waits for a table. The waves' parts meet in LDS,
+// the chunks' in the workspace, where the last workgroup of a row joins them
+// (c4s_join.hpp), in the chunks' order.
+//
+// The weights enter the second product as bf16 pairs (hi + lo, about 2^-17
+// relative), which costs nothing here: rounded once to bf16 they would add an
+// error of the size of the output's own rounding.
 constexpr int kWaves = 4;
 constexpr int kAttnThreads = 64 * kWaves;
+constexpr int kMaxParts = 128;   // chunks of a sequence
 
-// DH: the head's dims rounded up to 64, 128 or 256.
-template <int DH, bool Q8>
-__global__ __launch_bounds__(kAttnThreads) void k_attn(AttnArgs a) {
-  constexpr int kSteps = DH / 32, kTiles = DH / 16;
+struct FewArgs {
+  AttnArgs a;
+  int chunk, splits, tiles;   // positions a chunk (a multiple of 256); chunks at most; row tiles
+  uint32_t* arrived;          // [n_seqs][tiles][key heads]
+  float* part;                // [n_seqs][tiles][key heads][splits][kRows][dim + 4]
+};
+
+// DH: the head's dims rounded up to 64, 128 or 256; FULL: they are that many.
+template <int DH, bool Q8, bool FULL, int KEYS>
+__global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) void k_attn_few(FewArgs f) {
+  constexpr int kSteps = DH / 32, kTiles = DH / 16, kNT = KEYS / 16, kOwn = KEYS / 4;   // kOwn: a lane's positions of a block
+  constexpr int kKLoads = Q8 ? kNT * kSteps / 2 : kNT * kSteps, kVLoads = Q8 || KEYS == 32 ? kTiles : 2 * kTiles;
   __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
-  __shared__ __align__(16) float so[kWaves - 1][kRows][DH + 4];
+  __shared__ __align__(16) float so[kWaves][kRows][DH + 4];
+  const AttnArgs& a = f.a;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
-  const int head = blockIdx.x % a.c.n_heads, seq = blockIdx.y, dim = a.c.dim;
-  int row0 = seq, n_new = 1;
-  if (a.off) {
-    row0 = a.off[seq];
-    const int end = min(a.off[seq + 1], a.n_rows);
-    if (row0 < 0) return;
-    n_new = min(end - row0, a.max_new);
-  } else if (seq >= a.n_rows) {
-    return;
-  }
-  const int n_all = n_new * a.shared, r0 = blockIdx.x / a.c.n_heads * kRows;
+  const int dim = FULL ? DH : a.c.dim;
+  // blockIdx.x: (tile, chunk, key head), the heads of one chunk next to each other
+  const int head = blockIdx.x % a.c.n_heads, split = blockIdx.x / a.c.n_heads % f.splits, tile = blockIdx.x / a.c.n_heads / f.splits;
+  const int seq = blockIdx.y;
+  const Seq sq(a, seq);
+  const int n_all = sq.n_new * a.shared, r0 = tile * kRows;
   if (r0 >= n_all) return;
-  const int len = a.lens[seq];
-  const int past = len - (a.off ? a.off[seq + 1] - row0 : 1);
-  const int cap = a.c.max_pages << a.c.page_shift;
-  const int fst = a.first ? min(max(a.first[seq], 0), cap) : 0;
-  // lane's row
-  const int r = min(r0 + c, n_all - 1);
+  const int valid = min(kRows, n_all - r0);
+  const int r = r0 + min(c, valid - 1);
   const int token = r / a.shared, qh = head * a.shared + r % a.shared;
-  const int lim = min(past + token + 1, cap);           // positions this row sees end here
-  const int least = min(past + r0 / a.shared + 1, cap);   // ... the tile's first row
-  const int kend = min(past + min(r0 + kRows - 1, n_all - 1) / a.shared + 1, cap);
+  const int lim = min(sq.past + token + 1, sq.cap);                            // this row sees positions before it
+  const int least = min(sq.past + r0 / a.shared + 1, sq.cap);                  // ... the tile's first row
+  const int kend = min(sq.past + (r0 + valid - 1) / a.shared + 1, sq.cap);     // ... its last
+  const int fst = sq.fst;
+  const int first_chunk = fst / f.chunk, parts = kend > fst ? (kend - 1) / f.chunk + 1 - first_chunk : 1;
+  if (split >= parts) return;
+  const int begin = max((first_chunk + split) * f.chunk, fst & ~(KEYS - 1)), end = (int)min((int64_t)(first_chunk + split + 1) * f.chunk, (int64_t)kend);
 
   uint4 q[kSteps];
-  const uint16_t* qp = a.q + (int64_t)(row0 + token) * a.ldq + qh * dim;
+  {
+    const uint16_t* qp = a.q + (int64_t)(sq.row0 + token) * a.ldq + qh * dim;
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    // codes come 16 dims a lane at a time, which are two steps of 8
-    const int d = Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-    q[s] = d < dim ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < kSteps; ++s) {
+      // codes come 16 dims a lane at a time, which are two steps of 8
+      const int d = Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
+      q[s] = FULL || d < dim ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
+    }
   }
-
   const float c2 = a.scale * kLog2e;
-  float m = -__builtin_inff(), l = 0.0f;
-  f32x4 o[kTiles] = {};
-  const int ps = 1 << a.c.page_shift;
+  const int shift = a.c.page_shift, ps = 1 << shift;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
-  const int64_t page_elems = (int64_t)ps * dim;
+  constexpr int kSize = Q8 ? 1 : 2;
+  const int64_t page_bytes = (int64_t)ps * dim * kSize;
+  const char* kbase = static_cast<const char*>(a.c.k);
+  const char* vbase = static_cast<const char*>(a.c.v);
 
-  for (int t = (fst & ~(kKeys - 1)) + wave * kKeys; t < kend; t += kWaves * kKeys) {
-    // pages of the key row this lane loads, and of the 16 positions it weighs
-    const int kt = t + 16 * (c / 4), vt = t + 16 * g;
-    int kp = -1, vp = -1;
-    if ((kt >> a.c.page_shift) < a.c.max_pages) kp = table[kt >> a.c.page_shift];
-    if ((vt >> a.c.page_shift) < a.c.max_pages) vp = table[vt >> a.c.page_shift];
-    const bool there = vp >= 0 && vp < a.c.n_pages;
-    if (kp < 0 || kp >= a.c.n_pages) kp = 0;   // its scores are dropped
-    if (!there) vp = 0;
-    const int64_t kb = ((int64_t)kp * a.c.n_heads + head) * page_elems + (int64_t)((kt & (ps - 1)) + c % 4) * dim;
-    const int64_t vslot = ((int64_t)vp * a.c.n_heads + head) * ps + (vt & (ps - 1));
-    const int64_t vb = vslot * dim - (int64_t)(vt & (ps - 1)) * dim + (vt & (ps - 1));
-
-    f32x4 s[4] = {};
+  // A block's pages: of the key rows this lane loads, and of the positions it weighs.
+  struct Pages { int k, v; };
+  auto pages = [&](int t) {
+    const int ik = min((t + kOwn * (c / 4)) >> shift, a.c.max_pages - 1), iv = min((t + kOwn * g) >> shift, a.c.max_pages - 1);
+    return Pages{table[ik], table[iv]};
+  };
+  auto is_page = [&](int p) { return p >= 0 && p < a.c.n_pages; };
+  uint4 kr[kKLoads], vr[kVLoads];
+  float ks[Q8 ? kOwn : 1], vs[Q8 ? kOwn : 1];
+  auto load_keys = [&](int t, const Pages& p) {
+    const int kt = t + kOwn * (c / 4);
+    const int page = is_page(p.k) ? p.k : 0;   // its scores are dropped
+    const char* k = kbase + ((int64_t)page * a.c.n_heads + head) * page_bytes + (int64_t)(((kt & (ps - 1)) + c % 4) * dim) * kSize;
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      if constexpr (Q8) {
-        const uint8_t* k = static_cast<const uint8_t*>(a.c.k) + kb + (int64_t)(4 * tt) * dim;
+    for (int tt = 0; tt < kNT; ++tt)
 #pragma unroll
-        for (int st = 0; st < kSteps; st += 2) {
-          const int d = 32 * st + 16 * g;
-          const uint4 w = d < dim ? *reinterpret_cast<const uint4*>(k + d) : make_uint4(0, 0, 0, 0);
-          s[tt] = mfma(codes(make_uint2(w.x, w.y)), q[st], s[tt]);
-          s[tt] = mfma(codes(make_uint2(w.z, w.w)), q[st + 1], s[tt]);
-        }
-      } else {
-        const uint16_t* k = static_cast<const uint16_t*>(a.c.k) + kb + (int64_t)(4 * tt) * dim;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const int d = 32 * st + 8 * g;
-          s[tt] = mfma(d < dim ? *reinterpret_cast<const uint4*>(k + d) : make_uint4(0, 0, 0, 0), q[st], s[tt]);
-        }
+      for (int st = 0; st < kSteps / (Q8 ? 2 : 1); ++st) {
+        int d = (Q8 ? 64 * st + 16 * g : 32 * st + 8 * g);
+        if (!FULL && d >= dim) d = 0;          // times zeros of q
+        kr[tt * (kSteps / (Q8 ? 2 : 1)) + st] = *reinterpret_cast<const uint4*>(k + (4 * tt * dim + d) * kSize);
       }
+    if constexpr (Q8) {
+      const int vt = t + kOwn * g;
+      const float* s = a.c.k_scale + ((int64_t)(is_page(p.v) ? p.v : 0) * a.c.n_heads + head) * ps + (vt & (ps - 1));
+#pragma unroll
+      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&ks[j]) = *reinterpret_cast<const float4*>(s + j);
     }
-    // lane's 16 scores are positions vt .. vt + 15 of its row, in order
-    float p[16], vs[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float f = c2;
-      if constexpr (Q8) f *= a.c.k_scale[vslot + j];
-      p[j] = s[j / 4][j % 4] * f;
-      if constexpr (Q8) vs[j] = a.c.v_scale[vslot + j];
-    }
-    const bool edge = t < fst || t + kKeys > least || __any(!there);
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (!there || vt + j < fst || vt + j >= lim) p[j] = -__builtin_inff();
-    }
-    float top = p[0];
-#pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, p[j]);
-    top = fmaxf(max4(top), m);
-    const float base = top == -__builtin_inff() ? 0.0f : top;   // nothing seen yet
-    const float old = exp2f(m - base);
-    m = top;
-    l *= old;
-#pragma unroll
-    for (int d = 0; d < kTiles; ++d) o[d] *= old;
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      float x = exp2f(p[j] - base), y = exp2f(p[j + 1] - base);
-      l += x + y;
-      if constexpr (Q8) {   // 0 for a masked position, whatever its scale
-        x = x != 0.0f ? x * vs[j] : 0.0f;
-        y = y != 0.0f ? y * vs[j + 1] : 0.0f;
-      }
-      hi[j / 2] = pack(x, y);
-      lo[j / 2] = pack(x - low(hi[j / 2]), y - high(hi[j / 2]));
-    }
-    const int from = there ? fst - vt : 16, to = there ? kend - vt : 16;
+  };
+  auto load_values = [&](int t, const Pages& p) {
+    const int vt = t + kOwn * g;
+    const int64_t slot = (int64_t)(is_page(p.v) ? p.v : 0) * a.c.n_heads + head;
+    const char* v = vbase + slot * page_bytes + (vt & (ps - 1)) * kSize + (int64_t)(c * ps) * kSize;
 #pragma unroll
     for (int d = 0; d < kTiles; ++d) {
-      if (16 * d >= dim) break;
-      uint4 v[2];
+      const char* vd = v + (!FULL && 16 * d >= dim ? 0 : 16 * d * kSize) * ps;   // tiles behind the last dim are not used
       if constexpr (Q8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.c.v) + vb + (int64_t)(16 * d + c) * ps);
-        v[0] = codes(make_uint2(w.x, w.y));
-        v[1] = codes(make_uint2(w.z, w.w));
+        if constexpr (KEYS == 64) vr[d] = *reinterpret_cast<const uint4*>(vd);
+        else {
+          const uint2 w = *reinterpret_cast<const uint2*>(vd);
+          vr[d] = make_uint4(w.x, w.y, 0, 0);
+        }
       } else {
-        const uint16_t* vr = static_cast<const uint16_t*>(a.c.v) + vb + (int64_t)(16 * d + c) * ps;
-        v[0] = *reinterpret_cast<const uint4*>(vr);
-        v[1] = *reinterpret_cast<const uint4*>(vr + 8);
+#pragma unroll
+        for (int st = 0; st < KEYS / 32; ++st) vr[d * (KEYS / 32) + st] = *reinterpret_cast<const uint4*>(vd + 16 * st);
+      }
+    }
+    if constexpr (Q8) {
+      const float* s = a.c.v_scale + slot * ps + (vt & (ps - 1));
+#pragma unroll
+      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&vs[j]) = *reinterpret_cast<const float4*>(s + j);
+    }
+  };
+
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4 o[kTiles] = {};
+  constexpr int kStride = kWaves * KEYS;
+  int t = begin + wave * KEYS;
+  if (t < end) {
+    Pages now = pages(t), next = pages(t + kStride);
+    load_keys(t, now);
+    load_values(t, now);
+    for (; t < end; t += kStride) {
+      f32x4 s[kNT] = {};
+#pragma unroll
+      for (int tt = 0; tt < kNT; ++tt)
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          uint4 w;
+          if constexpr (Q8) {
+            uint4 x = kr[tt * (kSteps / 2) + st / 2];
+            here(x);
+            w = codes(st % 2 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
+          } else {
+            w = kr[tt * kSteps + st];
+          }
+          s[tt] = mfma(w, q[st], s[tt]);
+          if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      // lane's scores are positions vt .. vt + kOwn - 1 of its row, in order
+      const int vt = t + kOwn * g;
+      float p[kOwn];
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) p[j] = s[j / 4][j % 4] * (Q8 ? c2 * ks[j] : c2);
+      const bool there = is_page(now.v);
+      const bool edge = t < fst || t + KEYS > min(least, end) || __any(!there);
+      if (edge) {
+        const int from = max(fst - vt, 0), to = there ? min(lim, end) - vt : 0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) p[j] = ((j >= from) & (j < to)) ? p[j] : -__builtin_inff();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // The next block's loads; behind the last block that one's again, whose lines are near (a branch around
+      // them would make every wait behind it a wait for all of them).
+      const bool more = t + kStride < end;
+      const int tn = more ? t + kStride : t;
+      const Pages ahead = more ? next : now;
+      load_keys(tn, ahead);
+      next = pages(t + 2 * kStride);
+      __builtin_amdgcn_sched_barrier(0);
+      float top = p[0];
+#pragma unroll
+      for (int j = 1; j < kOwn; ++j) top = fmaxf(top, p[j]);
+      top = fmaxf(max4(top), m);
+      const float base = top == -__builtin_inff() ? 0.0f : top;   // nothing seen yet
+      const float old = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      l *= old;
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) o[d] *= old;
+      uint32_t hi[kOwn / 2], lo[kOwn / 2];
+#pragma unroll
+      for (int j = 0; j < kOwn; j += 2) {
+        float x = __builtin_amdgcn_exp2f(p[j] - base), y = __builtin_amdgcn_exp2f(p[j + 1] - base);
+        l += x + y;
+        if constexpr (Q8) {   // 0 for a masked position, whatever its scale
+          x = x != 0.0f ? x * vs[j] : 0.0f;
+          y = y != 0.0f ? y * vs[j + 1] : 0.0f;
+        }
+        hi[j / 2] = pack(x, y);
+        lo[j / 2] = pack(x - low(hi[j / 2]), y - high(hi[j / 2]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
+      if constexpr (!Q8) {
         if (edge) {
-          v[0] = keep(v[0], 0, from, to);
-          v[1] = keep(v[1], 8, from, to);
-          // A value that is not finite, in a block that some rows see in part:
-          // 0 times it would reach the rows that do not see it.
-          uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w}, odd[8];
-          bool any = false;
+          // What is not there or not for any row may hold anything: zeros. Where some of the rows see a
+          // position and others do not, 0 times a value that is not finite would reach those: such
+          // values are taken out, and the rows that see them become NaN.
+          const int from = there ? fst - vt : kOwn, to = there ? min(kend, end) - vt : kOwn;
+          int odd = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) any = any || odd_exp(w[i]);
-          if (__any(any)) {
+          for (int i = 0; i < kVLoads; ++i) {
+            vr[i] = keep(vr[i], 8 * (i % (KEYS / 32)), from, to);
+            odd |= odd_exp(vr[i].x) | odd_exp(vr[i].y) | odd_exp(vr[i].z) | odd_exp(vr[i].w);
+          }
+          if (least != kend && __any(odd)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) part_odd(w[i], odd[i]);
-            f32x4 seen = {};
+            for (int d = 0; d < kTiles; ++d) {
+              f32x4 seen = {};
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-              v[st] = make_uint4(w[4 * st], w[4 * st + 1], w[4 * st + 2], w[4 * st + 3]);
-              seen = mfma(make_uint4(odd[4 * st], odd[4 * st + 1], odd[4 * st + 2], odd[4 * st + 3]),
-                          make_uint4(hi[4 * st], hi[4 * st + 1], hi[4 * st + 2], hi[4 * st + 3]), seen);
+              for (int st = 0; st < KEYS / 32; ++st) {
+                uint4& v = vr[d * (KEYS / 32) + st];
+                uint4 ones;
+                part_odd(v.x, ones.x);
+                part_odd(v.y, ones.y);
+                part_odd(v.z, ones.z);
+                part_odd(v.w, ones.w);
+                seen = mfma(ones, quad(hi + 4 * st), seen);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (seen[i] != 0.0f) o[d][i] = __builtin_nanf("");
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (seen[i] != 0.0f) o[d][i] = __builtin_nanf("");
           }
         }
       }
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        o[d] = mfma(v[st], make_uint4(hi[4 * st], hi[4 * st + 1], hi[4 * st + 2], hi[4 * st + 3]), o[d]);
-        o[d] = mfma(v[st], make_uint4(lo[4 * st], lo[4 * st + 1], lo[4 * st + 2], lo[4 * st + 3]), o[d]);
+      for (int d = 0; d < kTiles; ++d) {
+#pragma unroll
+        for (int st = 0; st < KEYS / 32; ++st) {
+          uint4 v;
+          if constexpr (Q8) {
+            v = vr[d];
+            here(v);
+            v = codes(st ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y));
+          }
+          else v = vr[d * (KEYS / 32) + st];
+          o[d] = mfma(v, quad(hi + 4 * st), o[d]);
+          o[d] = mfma(v, quad(lo + 4 * st), o[d]);
+        }
+        if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(tn, ahead);
+      now = ahead;
     }
   }
 
-  // the waves' parts, joined by wave 0
+  // The waves' parts: of output quad (row, dims 4 i ..) by the thread that has it.
   l = sum4(l);
   if (g == 0) {
     sm[wave][c] = m;
     sl[wave][c] = l;
   }
-  if (wave > 0) {
 #pragma unroll
-    for (int d = 0; d < kTiles; ++d) *reinterpret_cast<f32x4*>(&so[wave - 1][c][16 * d + 4 * g]) = o[d];
+  for (int d = 0; d < kTiles; ++d) *reinterpret_cast<f32x4*>(&so[wave][c][16 * d + 4 * g]) = o[d];
+  __syncthreads();
+  const int quads = dim / 4;   // a row
+  const int64_t group = ((int64_t)seq * f.tiles + tile) * a.c.n_heads + head;
+  const int words = kRows * (quads + 1);   // quads a part: the rows', then (maximum, sum) of each row
+  float* mine = f.part + (group * f.splits + split) * words * 4;
+  auto finish = [&](int row, int i, f32x4 v, float top, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int rr = r0 + row, tok = sq.row0 + rr / a.shared, hh = head * a.shared + rr % a.shared;
+    *reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.ld_out + hh * dim + 4 * i) = make_uint2(pack(v[0] * inv, v[1] * inv), pack(v[2] * inv, v[3] * inv));
+    if (a.lse && i == 0) a.lse[(int64_t)tok * a.n_heads + hh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
+  };
+  for (int e = threadIdx.x; e < valid * quads; e += kAttnThreads) {
+    const int row = e / quads, i = e % quads;
+    float top = sm[0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][row]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float fw = __builtin_amdgcn_exp2f(sm[w][row] - base);
+      sum = __builtin_fmaf(sl[w][row], fw, sum);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&so[w][row][4 * i]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __builtin_fmaf(x[u], fw, v[u]);
+    }
+    if (parts == 1) {
+      finish(row, i, v, top, sum);
+    } else {
+      put_quad(mine, words, e, v);
+      if (i == 0) put_quad(mine, words, kRows * quads + row, f32x4{top, sum, 0.0f, 0.0f});
+    }
+  }
+  if (parts == 1 || !last_to_arrive(f.arrived + group, parts)) return;
+  const float* all = f.part + group * f.splits * words * 4;
+  // Every part's maximum and sum; what each part weighs, and the row's own.
+  float* tops = &so[0][0][0];            // [kRows][kMaxParts]
+  float* sums = tops + kRows * kMaxParts;
+  static_assert(sizeof(so) >= 2 * kRows * kMaxParts * sizeof(float), "the parts' statistics in LDS");
+  for (int e = threadIdx.x; e < valid * parts; e += kAttnThreads) {
+    const f32x4 x = get_quad(all + (int64_t)(e / valid) * words * 4, words, kRows * quads + e % valid);
+    tops[e % valid * kMaxParts + e / valid] = x[0];
+    sums[e % valid * kMaxParts + e / valid] = x[1];
   }
   __syncthreads();
-  if (wave > 0 || r0 + c >= n_all) return;
-  float top = m;
+  {
+    const int row = threadIdx.x / 16, j = threadIdx.x % 16;   // sixteen lanes a row
+    float top = -__builtin_inff();
+    if (row < valid)
+      for (int i = j; i < parts; i += 16) top = fmaxf(top, tops[row * kMaxParts + i]);
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][c]);
-  const float base = top == -__builtin_inff() ? 0.0f : top;
-  float f[kWaves], sum = 0.0f;
+    for (int x = 8; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 16));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    if (row < valid)
+      for (int i = j; i < parts; i += 16) {
+        const float w = __builtin_amdgcn_exp2f(tops[row * kMaxParts + i] - base);
+        tops[row * kMaxParts + i] = w;
+        sum = __builtin_fmaf(sums[row * kMaxParts + i], w, sum);
+      }
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    f[w] = exp2f(sm[w][c] - base);
-    sum += sl[w][c] * f[w];
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* out = a.out + (int64_t)(row0 + token) * a.ld_out + qh * dim;
-#pragma unroll
-  for (int d = 0; d < kTiles; ++d) {
-    if (16 * d >= dim) break;
-    f32x4 v = o[d] * f[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(&so[w - 1][c][16 * d + 4 * g]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(x[i], f[w], v[i]);
+    for (int x = 8; x; x >>= 1) sum += __shfl_xor(sum, x, 16);
+    if (j == 0) {
+      sm[0][row] = top;
+      sl[0][row] = sum;
     }
-    *reinterpret_cast<uint2*>(out + 16 * d + 4 * g) = make_uint2(pack(v[0] * inv, v[1] * inv), pack(v[2] * inv, v[3] * inv));
   }
-  if (a.lse && g == 0)
-    a.lse[(int64_t)(row0 + token) * a.n_heads + qh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
+  __syncthreads();
+  for (int e = threadIdx.x; e < valid * quads; e += kAttnThreads) {
+    const int row = e / quads;
+    f32x4 v = {};
+    for (int p = 0; p < parts; p += 8) {   // eight parts' loads in flight, added in order
+      f32x4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = get_quad(all + (int64_t)min(p + u, parts - 1) * words * 4, words, e);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = p + u < parts ? tops[row * kMaxParts + p + u] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p + u < parts ? __builtin_fmaf(x[u][i], w, v[i]) : v[i];
+      }
+    }
+    finish(row, e % quads, v, sm[0][row], sl[0][row]);
+  }
+}
+
+// Chunks: so many that the chip has work (kWant workgroups), not below 256
+// positions, at most kMaxParts of a sequence.
+constexpr int64_t kWant = 2048;
+FewArgs few_args(const AttnArgs& a) {
+  FewArgs f{};
+  f.a = a;
+  f.tiles = (int)(((int64_t)a.max_new * a.shared + kRows - 1) / kRows);
+  const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift, groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
+  int64_t want = kWant;
+  if (getenv("C4S_WANT")) want = atoi(getenv("C4S_WANT"));
+  int64_t chunk = std::max(cap * groups / want, (cap + kMaxParts - 1) / kMaxParts);
+  chunk = std::max<int64_t>((chunk + 255) / 256 * 256, 256);
+  f.chunk = (int)std::min<int64_t>(chunk, INT32_MAX / 2 / 256 * 256);
+  f.splits = (int)std::max<int64_t>((cap + f.chunk - 1) / f.chunk, 1);
+  return f;
+}
+
+template <int DH, bool Q8, bool FULL, int KEYS>
+hipError_t few(const FewArgs& f, hipStream_t s) {
+  hipLaunchKernelGGL((k_attn_few<DH, Q8, FULL, KEYS>), dim3((unsigned)((int64_t)f.tiles * f.splits * f.a.c.n_heads), f.a.c.n_seqs),
+                     dim3(kAttnThreads), 0, s, f);
+  return hipGetLastError();
+}
+template <int DH, int BKEYS, int QKEYS>
+hipError_t few(const FewArgs& f, hipStream_t s) {
+  const bool full = f.a.c.dim == DH;
+  if (f.a.c.store == C4S_KV_Q8) return full ? few<DH, true, true, QKEYS>(f, s) : few<DH, true, false, QKEYS>(f, s);
+  return full ? few<DH, false, true, BKEYS>(f, s) : few<DH, false, false, BKEYS>(f, s);
 }
 
 }  // namespace
 
-hipError_t launch_attn(const AttnArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.max_new * a.shared + kRows - 1) / kRows * a.c.n_heads), a.c.n_seqs);
-  const bool q8 = a.c.store == C4S_KV_Q8;
-  if (a.c.dim <= 64) {
-    if (q8) hipLaunchKernelGGL((k_attn<64, true>), grid, dim3(kAttnThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<64, false>), grid, dim3(kAttnThreads), 0, s, a);
-  } else if (a.c.dim <= 128) {
-    if (q8) hipLaunchKernelGGL((k_attn<128, true>), grid, dim3(kAttnThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<128, false>), grid, dim3(kAttnThreads), 0, s, a);
-  } else {
-    if (q8) hipLaunchKernelGGL((k_attn<256, true>), grid, dim3(kAttnThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<256, false>), grid, dim3(kAttnThreads), 0, s, a);
-  }
-  return hipGetLastError();
+LayerSpace attn_space(const AttnArgs& a) {
+  const FewArgs f = few_args(a);
+  if (f.splits == 1) return {};
+  const int64_t groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
+  return {groups, groups * f.splits * kRows * (a.c.dim + 4)};
+}
+
+hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipStream_t s) {
+  FewArgs f = few_args(a);
+  f.arrived = counters;
+  f.part = space;
+  if (a.c.dim <= 64) return few<64, 32, 32>(f, s);
+  if (a.c.dim <= 128) return few<128, 32, 32>(f, s);
+  return few<256, 32, 32>(f, s);
 }
 
 }  // namespace c4s

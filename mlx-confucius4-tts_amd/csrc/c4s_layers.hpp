@@ -56,6 +56,7 @@ LayerSpace linear_space(const c4s_linear_desc& a);
 hipError_t launch_linear(const c4s_linear_desc& a, uint32_t* counters, float* space, hipStream_t s);
 hipError_t launch_kv_append(const KvArgs& c, const KvRowsArgs& r, hipStream_t s);
 hipError_t launch_kv_read(const KvArgs& c, const KvRowsArgs& r, hipStream_t s);
-hipError_t launch_attn(const AttnArgs& a, hipStream_t s);
+LayerSpace attn_space(const AttnArgs& a);
+hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipStream_t s);
 
 }  // namespace c4s

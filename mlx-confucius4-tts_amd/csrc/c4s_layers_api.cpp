@@ -221,7 +221,9 @@ int c4s_attn(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_attn_desc* attn,
     a.n_heads = attn->n_heads;
     a.shared = attn->n_heads / cache->n_kv_heads;
     a.scale = attn->scale;
-    return queue(ctx, "attn launch", [&] { return c4s::launch_attn(a, static_cast<hipStream_t>(stream)); });
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return queue_with(ctx, c4s::attn_space(a), s, "attn launch",
+                      [&](uint32_t* n, float* f) { return c4s::launch_attn(a, n, f, s); });
   });
 }
 
