@@ -136,10 +136,10 @@ typedef struct c4s_kv_cache {
   const int32_t* block_table;   /* [n_seqs][table_ld] */
   int64_t table_ld;
   int32_t n_seqs;               /* up to 65535 */
-  int32_t max_pages;            /* entries of a row of block_table in use, <= table_ld */
+  int32_t max_pages;            /* entries of a row of block_table in use, <= table_ld; max_pages * page_size up to 2097152 */
   int32_t n_pages;
   int32_t page_size;            /* 16, 32, 64, 128 or 256 */
-  int32_t n_kv_heads;
+  int32_t n_kv_heads;           /* n_kv_heads * page_size * head_dim up to 536870912 */
   int32_t head_dim;             /* a multiple of 16, 16 .. 256 */
   int32_t store;                /* C4S_KV_* */
 } c4s_kv_cache;

@@ -13,7 +13,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "c4s_join.hpp"
 #include "c4s_layers.hpp"
@@ -125,7 +124,8 @@ constexpr int kRows = 16;   // rows of a workgroup
 // error of the size of the output's own rounding.
 constexpr int kWaves = 4;
 constexpr int kAttnThreads = 64 * kWaves;
-constexpr int kMaxParts = 128;   // chunks of a sequence
+constexpr int kMaxParts = 128;       // chunks of a sequence
+constexpr int kMaxChunk = 16384;     // positions of a chunk: its pages fit the table in LDS
 
 struct FewArgs {
   AttnArgs a;
@@ -147,6 +147,19 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   // blockIdx.x: (tile, chunk, key head), the heads of one chunk next to each other
   const int head = blockIdx.x % a.c.n_heads, split = blockIdx.x / a.c.n_heads % f.splits, tile = blockIdx.x / a.c.n_heads / f.splits;
   const int seq = blockIdx.y;
+  const int shift = a.c.page_shift, ps = 1 << shift;
+  // The chunk's part of the table (-1: no page), asked for while the lengths are on their way.
+  __shared__ int32_t pages[kMaxChunk / 16 + 16];
+  const int base = split * f.chunk;
+  auto fill = [&](int from) {
+    const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
+    for (int i = threadIdx.x; i < (f.chunk >> shift) + (KEYS >> 4); i += kAttnThreads) {
+      const int at = (from >> shift) + i;
+      const int p = at < a.c.max_pages ? table[at] : -1;
+      pages[i] = p < a.c.n_pages ? p : -1;
+    }
+  };
+  fill(base);
   const Seq sq(a, seq);
   const int n_all = sq.n_new * a.shared, r0 = tile * kRows;
   if (r0 >= n_all) return;
@@ -172,72 +185,74 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
     }
   }
   const float c2 = a.scale * kLog2e;
-  const int shift = a.c.page_shift, ps = 1 << shift;
-  const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
   constexpr int kSize = Q8 ? 1 : 2;
-  const int64_t page_bytes = (int64_t)ps * dim * kSize;
-  const char* kbase = static_cast<const char*>(a.c.k);
-  const char* vbase = static_cast<const char*>(a.c.v);
-
-  // A block's pages: of the key rows this lane loads, and of the positions it weighs.
+  const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;   // below 2^31
+  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head + (Q8 ? 16 : 16) * g + (c % 4) * dim * kSize;
+  const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head + (uint64_t)(uint32_t)((c * kSize) << shift);
+  const uint32_t scale_bytes = 4u * (uint32_t)a.c.n_heads << shift;
+  const uint32_t tile_bytes = (16u * kSize) << shift;
+  // A block's pages: of the key rows this lane loads, and of the positions it weighs (below 0: none).
+  const int origin = (first_chunk + split) * f.chunk >> shift;
   struct Pages { int k, v; };
-  auto pages = [&](int t) {
-    const int ik = min((t + kOwn * (c / 4)) >> shift, a.c.max_pages - 1), iv = min((t + kOwn * g) >> shift, a.c.max_pages - 1);
-    return Pages{table[ik], table[iv]};
+  auto pages_of = [&](int t) {
+    return Pages{pages[((t + kOwn * (c / 4)) >> shift) - origin], pages[((t + kOwn * g) >> shift) - origin]};
   };
-  auto is_page = [&](int p) { return p >= 0 && p < a.c.n_pages; };
   uint4 kr[kKLoads], vr[kVLoads];
   float ks[Q8 ? kOwn : 1], vs[Q8 ? kOwn : 1];
-  auto load_keys = [&](int t, const Pages& p) {
-    const int kt = t + kOwn * (c / 4);
-    const int page = is_page(p.k) ? p.k : 0;   // its scores are dropped
-    const char* k = kbase + ((int64_t)page * a.c.n_heads + head) * page_bytes + (int64_t)(((kt & (ps - 1)) + c % 4) * dim) * kSize;
+  auto load_keys = [&](int t, const Pages& p) {   // scores of what has no page are dropped
+    const uint32_t at = (uint32_t)((t + kOwn * (c / 4)) & (ps - 1)) * (uint32_t)(dim * kSize);
+    const char* k = kbase + (uint64_t)(uint32_t)max(p.k, 0) * page_bytes + at;
+    constexpr int kRow = kSteps / (Q8 ? 2 : 1);
 #pragma unroll
     for (int tt = 0; tt < kNT; ++tt)
 #pragma unroll
-      for (int st = 0; st < kSteps / (Q8 ? 2 : 1); ++st) {
-        int d = (Q8 ? 64 * st + 16 * g : 32 * st + 8 * g);
-        if (!FULL && d >= dim) d = 0;          // times zeros of q
-        kr[tt * (kSteps / (Q8 ? 2 : 1)) + st] = *reinterpret_cast<const uint4*>(k + (4 * tt * dim + d) * kSize);
+      for (int st = 0; st < kRow; ++st) {
+        int d = 64 * st / (Q8 ? 1 : 2);                                         // dims before this lane's
+        if (!FULL && d + (Q8 ? 16 : 8) * g >= dim) d = -(Q8 ? 16 : 8) * g;      // times zeros of q
+        kr[tt * kRow + st] = *reinterpret_cast<const uint4*>(k + (4 * tt * dim + d) * kSize);
       }
     if constexpr (Q8) {
       const int vt = t + kOwn * g;
-      const float* s = a.c.k_scale + ((int64_t)(is_page(p.v) ? p.v : 0) * a.c.n_heads + head) * ps + (vt & (ps - 1));
+      const char* s = reinterpret_cast<const char*>(a.c.k_scale) + (uint64_t)(uint32_t)max(p.v, 0) * scale_bytes + (uint32_t)(((head << shift) + (vt & (ps - 1))) * 4);
 #pragma unroll
-      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&ks[j]) = *reinterpret_cast<const float4*>(s + j);
+      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&ks[j]) = *reinterpret_cast<const float4*>(s + 4 * j);
     }
   };
   auto load_values = [&](int t, const Pages& p) {
-    const int vt = t + kOwn * g;
-    const int64_t slot = (int64_t)(is_page(p.v) ? p.v : 0) * a.c.n_heads + head;
-    const char* v = vbase + slot * page_bytes + (vt & (ps - 1)) * kSize + (int64_t)(c * ps) * kSize;
+    const uint32_t at = (uint32_t)((t + kOwn * g) & (ps - 1));
+    const char* v = vbase + (uint64_t)(uint32_t)max(p.v, 0) * page_bytes + at * kSize;
 #pragma unroll
     for (int d = 0; d < kTiles; ++d) {
-      const char* vd = v + (!FULL && 16 * d >= dim ? 0 : 16 * d * kSize) * ps;   // tiles behind the last dim are not used
       if constexpr (Q8) {
-        if constexpr (KEYS == 64) vr[d] = *reinterpret_cast<const uint4*>(vd);
+        if constexpr (KEYS == 64) vr[d] = *reinterpret_cast<const uint4*>(v);
         else {
-          const uint2 w = *reinterpret_cast<const uint2*>(vd);
+          const uint2 w = *reinterpret_cast<const uint2*>(v);
           vr[d] = make_uint4(w.x, w.y, 0, 0);
         }
       } else {
 #pragma unroll
-        for (int st = 0; st < KEYS / 32; ++st) vr[d * (KEYS / 32) + st] = *reinterpret_cast<const uint4*>(vd + 16 * st);
+        for (int st = 0; st < KEYS / 32; ++st) vr[d * (KEYS / 32) + st] = *reinterpret_cast<const uint4*>(v + 16 * st);
       }
+      if (FULL || 16 * (d + 1) < dim) v += tile_bytes;   // tiles behind the last dim are not used
     }
     if constexpr (Q8) {
-      const float* s = a.c.v_scale + slot * ps + (vt & (ps - 1));
+      const char* s = reinterpret_cast<const char*>(a.c.v_scale) + (uint64_t)(uint32_t)max(p.v, 0) * scale_bytes + ((uint32_t)(head << shift) + at) * 4;
 #pragma unroll
-      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&vs[j]) = *reinterpret_cast<const float4*>(s + j);
+      for (int j = 0; j < kOwn; j += 4) *reinterpret_cast<float4*>(&vs[j]) = *reinterpret_cast<const float4*>(s + 4 * j);
     }
   };
 
   float m = -__builtin_inff(), l = 0.0f;
   f32x4 o[kTiles] = {};
   constexpr int kStride = kWaves * KEYS;
+  if (first_chunk) {   // behind padding the chunk is another
+    __syncthreads();
+    fill((first_chunk + split) * f.chunk);
+  }
+  __syncthreads();
   int t = begin + wave * KEYS;
   if (t < end) {
-    Pages now = pages(t), next = pages(t + kStride);
+    Pages now = pages_of(t);
     load_keys(t, now);
     load_values(t, now);
     for (; t < end; t += kStride) {
@@ -263,7 +278,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       float p[kOwn];
 #pragma unroll
       for (int j = 0; j < kOwn; ++j) p[j] = s[j / 4][j % 4] * (Q8 ? c2 * ks[j] : c2);
-      const bool there = is_page(now.v);
+      const bool there = now.v >= 0;
       const bool edge = t < fst || t + KEYS > min(least, end) || __any(!there);
       if (edge) {
         const int from = max(fst - vt, 0), to = there ? min(lim, end) - vt : 0;
@@ -275,9 +290,8 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       // them would make every wait behind it a wait for all of them).
       const bool more = t + kStride < end;
       const int tn = more ? t + kStride : t;
-      const Pages ahead = more ? next : now;
+      const Pages ahead = pages_of(tn);
       load_keys(tn, ahead);
-      next = pages(t + 2 * kStride);
       __builtin_amdgcn_sched_barrier(0);
       float top = p[0];
 #pragma unroll
@@ -453,19 +467,22 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   }
 }
 
-// Chunks: so many that the chip has work (kWant workgroups), not below 256
-// positions, at most kMaxParts of a sequence.
-constexpr int64_t kWant = 2048;
+// How the positions are cut. A workgroup's way into its stream and out of it costs
+// some microseconds, so a sequence is cut only where the rows' tiles alone leave
+// the chip empty: into 512 workgroups together, or, in pieces of 1280 positions
+// or more, into 2048 (they even out what the lengths do not). Measured, in us,
+// for 512 / 1024 / 2048: 64 rows of 1024, 8 heads of 128: 54 / 72 / 68 (8-bit 32
+// / 41 / 44); 8 rows of 2000, 20 heads of 64: 17.7 / 18.5 / 19.9; 6 rows of 12000
+// to 50001, 8 heads of 128, 8-bit: 95 / 94 / 87.
 FewArgs few_args(const AttnArgs& a) {
   FewArgs f{};
   f.a = a;
   f.tiles = (int)(((int64_t)a.max_new * a.shared + kRows - 1) / kRows);
   const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift, groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
-  int64_t want = kWant;
-  if (getenv("C4S_WANT")) want = atoi(getenv("C4S_WANT"));
-  int64_t chunk = std::max(cap * groups / want, (cap + kMaxParts - 1) / kMaxParts);
-  chunk = std::max<int64_t>((chunk + 255) / 256 * 256, 256);
-  f.chunk = (int)std::min<int64_t>(chunk, INT32_MAX / 2 / 256 * 256);
+  const int64_t coarse = std::max<int64_t>(512 / groups, 1), fine = std::max<int64_t>(2048 / groups, 1);
+  int64_t chunk = std::min(cap / coarse, std::max<int64_t>(1280, cap / fine)) + 255;
+  chunk = std::max(chunk, (cap + kMaxParts - 1) / kMaxParts + 255) / 256 * 256;
+  f.chunk = (int)std::min<int64_t>(std::max<int64_t>(chunk, 256), kMaxChunk);
   f.splits = (int)std::max<int64_t>((cap + f.chunk - 1) / f.chunk, 1);
   return f;
 }
@@ -497,7 +514,7 @@ hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipS
   f.arrived = counters;
   f.part = space;
   if (a.c.dim <= 64) return few<64, 32, 32>(f, s);
-  if (a.c.dim <= 128) return few<128, 32, 32>(f, s);
+  if (a.c.dim <= 128) return few<128, 32, 64>(f, s);
   return few<256, 32, 32>(f, s);
 }
 

@@ -104,7 +104,8 @@ int check_cache(c4s_ctx* ctx, const c4s_kv_cache* c) {
   if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16)
     return fail(ctx, C4S_EINVAL, "kv_cache: head_dim must be a multiple of 16 up to 256");
   if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return fail(ctx, C4S_EINVAL, "kv_cache: n_kv_heads out of range");
-  if ((int64_t)c->max_pages * c->page_size > INT32_MAX - 1024) return fail(ctx, C4S_EINVAL, "kv_cache: max_pages out of range");
+  if ((int64_t)c->max_pages * c->page_size > 1 << 21) return fail(ctx, C4S_EINVAL, "kv_cache: more than 2097152 positions a sequence");
+  if ((int64_t)c->n_kv_heads * c->page_size * c->head_dim > 1 << 29) return fail(ctx, C4S_EINVAL, "kv_cache: more than 536870912 values a page");
   if (!c->k || !c->v || (c->max_pages && !c->block_table)) return fail(ctx, C4S_EINVAL, "kv_cache: required pointer is NULL");
   if (c->store != C4S_KV_BF16 && c->store != C4S_KV_Q8) return fail(ctx, C4S_EINVAL, "kv_cache: unknown store");
   if (c->store == C4S_KV_Q8 && (!c->k_scale || !c->v_scale)) return fail(ctx, C4S_EINVAL, "kv_cache: 8-bit codes need k_scale and v_scale");
