@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "c4s_join.hpp"
 #include "c4s_layers.hpp"
@@ -500,9 +501,319 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
   return full ? few<DH, false, true, BKEYS>(f, s) : few<DH, false, false, BKEYS>(f, s);
 }
 
+// ---- many rows ----------------------------------------------------------------------------
+//
+// Prompts: a workgroup has 64 NB rows of one sequence and key head, 16 NB a
+// wave, and goes through the positions in blocks of 64, which all four waves
+// share: a block's keys and values are loaded (codes converted, once for all
+// rows) into registers while the block before it is worked on, and written to
+// the other of two buffers in LDS, with one barrier a block. The rows of both
+// buffers are permuted in 16-byte pieces so that the fragment reads of sixteen
+// lanes that LDS serves together fall into different banks. Blocks behind a
+// wave's last row are skipped by it, masks are applied only where a block
+// holds the limit of some row, and the tiles with the most positions start
+// first.
+//
+// Weights enter the second product rounded to bf16 once: independent roundings
+// of 2^-9 at most, which add a quarter to the error of the output's own
+// rounding; as pairs, as with few rows, they would cost half as many matrix
+// instructions again. Their sum is taken before the rounding, in fp32.
+constexpr int kBlock = 64;         // positions
+constexpr int kSegment = 16384;    // positions whose pages LDS holds at a time
+
+struct ManyArgs {
+  AttnArgs a;
+  int tiles;
+};
+
+// Where row r of a block of keys (NP pieces a row) keeps piece p, and row r of
+// one of values (eight pieces). LDS serves lanes 0-3, 12-15, 20-23 and 24-27 (and
+// so on) together: those read rows 16 apart (keys) or next to each other
+// (values), and in two lane groups' pieces.
+template <int NP>
+__device__ __forceinline__ int key_piece(int r, int p) {
+  const int f = NP == 8 ? ((r >> 1) & 1) | ((r >> 4) & 3) << 1 : (r & 3) | ((r >> 4) & 3) << 2;
+  return (r * NP + (p ^ f)) * 16;
+}
+__device__ __forceinline__ int value_piece(int r, int p) {
+  return (r * 8 + (p ^ (((r >> 1) & 1) << 1 | ((r >> 2) & 1) | ((r >> 3) & 1) << 2))) * 16;
+}
+
+template <int DH, bool Q8, int NB>
+__global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(ManyArgs f) {
+  constexpr int kSteps = DH / 32, kTiles = DH / 16, kNP = DH / 8;   // kNP: pieces of a key
+  constexpr int kLoads = (Q8 ? DH / 64 : DH / 32);                  // a thread's, of the keys and of the values
+  constexpr int kBuf = 2 * kBlock * DH * 2;
+  __shared__ __align__(16) char lds[2][kBuf];
+  __shared__ __align__(16) float scales[2][Q8 ? 2 * kBlock : 4];    // [buffer][keys', values']
+  __shared__ int32_t pages[kSegment / 16];
+  const AttnArgs& a = f.a;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, c = lane % 16, g = lane / 16;
+  const int dim = a.c.dim, head = blockIdx.x % a.c.n_heads, tile = f.tiles - 1 - blockIdx.x / a.c.n_heads, seq = blockIdx.y;
+  const Seq sq(a, seq);
+  const int n_all = sq.n_new * a.shared, r0 = tile * 64 * NB;
+  if (r0 >= n_all) return;
+  const int fst = sq.fst, shift = a.c.page_shift, ps = 1 << shift;
+  // This wave's rows; a lane has row 16 b + c of each block b.
+  const int w0 = r0 + 16 * NB * wave;
+  const bool any_rows = w0 < n_all;
+  int lim[NB], least = 0, most = 0;   // least, most: of the wave's first and last row
+  const uint16_t* qp[NB];
+  uint16_t* op[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int r = min(w0 + 16 * b + c, n_all - 1), token = r / a.shared, qh = head * a.shared + r % a.shared;
+    lim[b] = min(sq.past + token + 1, sq.cap);
+    qp[b] = a.q + (int64_t)(sq.row0 + token) * a.ldq + qh * dim;
+    op[b] = a.out + (int64_t)(sq.row0 + token) * a.ld_out + qh * dim;
+  }
+  if (any_rows) {
+    least = min(sq.past + w0 / a.shared + 1, sq.cap);
+    most = min(sq.past + min(w0 + 16 * NB - 1, n_all - 1) / a.shared + 1, sq.cap);
+  }
+  const int kend = min(sq.past + min(r0 + 64 * NB - 1, n_all - 1) / a.shared + 1, sq.cap);   // the workgroup's last
+
+  uint4 q[NB][kSteps];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      q[b][s] = 32 * s + 8 * g < dim ? *reinterpret_cast<const uint4*>(qp[b] + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+
+  constexpr int kSize = Q8 ? 1 : 2;
+  const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;
+  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head;
+  const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head;
+  const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
+  const float c2 = a.scale * kLog2e;
+
+  float m[NB], l[NB];
+  f32x4 o[NB][kTiles] = {};
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    m[b] = -__builtin_inff();
+    l[b] = 0.0f;
+  }
+
+  for (int seg = fst & ~(kSegment - 1); seg < kend; seg += kSegment) {
+    const int begin = max(seg, fst & ~(kBlock - 1)), end = min(seg + kSegment, kend);
+    __syncthreads();
+    for (int i = tid; i < kSegment >> shift; i += kAttnThreads) {
+      const int at = (seg >> shift) + i;
+      const int p = at < a.c.max_pages ? table[at] : -1;
+      pages[i] = p < a.c.n_pages ? p : -1;
+    }
+    __syncthreads();
+    uint4 kst[kLoads], vst[kLoads];
+    float sst = 0.0f;
+    auto page_of = [&](int pos) { return (uint64_t)(uint32_t)max(pages[(pos - seg) >> shift], 0); };   // what has no page is dropped
+    // A thread's pieces: of the keys in order; of the values in the order in which a page has them.
+    const int row_shift = min(shift, 6) - (Q8 ? 4 : 3);   // log2 of the pieces a page's row has in a block
+    auto load = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = tid + kAttnThreads * i;
+        constexpr int kKP = Q8 ? DH / 16 : DH / 8;   // a key's pieces
+        const int key = t + at / kKP, d = at % kKP * (Q8 ? 16 : 8);
+        kst[i] = make_uint4(0, 0, 0, 0);
+        if (DH == 64 || DH == 256 || d < dim)
+          if (d < dim)
+            kst[i] = *reinterpret_cast<const uint4*>(kbase + page_of(key) * page_bytes + (uint32_t)((key & (ps - 1)) * dim + d) * kSize);
+        const int vd = (at >> row_shift) % DH, piece = (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
+        const int pos = t + piece * (Q8 ? 16 : 8);
+        vst[i] = *reinterpret_cast<const uint4*>(vbase + page_of(pos) * page_bytes + (uint32_t)((min(vd, dim - 1) << shift) + (pos & (ps - 1))) * kSize);
+      }
+      if constexpr (Q8) {
+        if (tid < 2 * kBlock) {
+          const int pos = t + tid % kBlock;
+          sst = (tid < kBlock ? a.c.k_scale : a.c.v_scale)[(page_of(pos) * a.c.n_heads + head << shift) + (pos & (ps - 1))];
+        }
+      }
+    };
+    auto stage = [&](int buf) {
+      char* kl = lds[buf];
+      char* vl = kl + kBlock * DH * 2;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = tid + kAttnThreads * i;
+        constexpr int kKP = Q8 ? DH / 16 : DH / 8;
+        const int vd = (at >> row_shift) % DH, piece = (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
+        if constexpr (Q8) {
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP * 2)) = codes(make_uint2(kst[i].x, kst[i].y));
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP * 2 + 1)) = codes(make_uint2(kst[i].z, kst[i].w));
+          *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece)) = codes(make_uint2(vst[i].x, vst[i].y));
+          *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece + 1)) = codes(make_uint2(vst[i].z, vst[i].w));
+        } else {
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP)) = kst[i];
+          *reinterpret_cast<uint4*>(vl + value_piece(vd, piece)) = vst[i];
+        }
+      }
+      if constexpr (Q8) {
+        if (tid < 2 * kBlock) scales[buf][tid] = sst;
+      }
+    };
+    load(begin);
+    stage(0);
+    if (begin + kBlock < end) load(begin + kBlock);
+    int buf = 0;
+    for (int t = begin; t < end; t += kBlock, buf ^= 1) {
+      __syncthreads();   // this block is there, and the other buffer has been read
+      if (t + kBlock < end) {
+        stage(buf ^ 1);
+        if (t + 2 * kBlock < end) load(t + 2 * kBlock);
+      }
+      if (t >= most) continue;   // no row of this wave sees it
+      const char* kl = lds[buf];
+      const char* vl = kl + kBlock * DH * 2;
+      f32x4 s[NB][4] = {};
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kl + key_piece<kNP>(16 * (c / 4) + 4 * tt + c % 4, 4 * st + g));
+#pragma unroll
+          for (int b = 0; b < NB; ++b) s[b][tt] = mfma(w, q[b][st], s[b][tt]);
+        }
+      const int vt = t + 16 * g;   // a lane's 16 positions
+      if constexpr (Q8) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[buf][16 * g + 4 * tt]) * c2;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) s[b][tt] *= ks;
+        }
+      } else {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) s[b][tt] *= c2;
+      }
+      const bool there = pages[(vt - seg) >> shift] >= 0;
+      const bool edge = t < fst || t + kBlock > least || __any(!there);
+      if (edge) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int from = max(fst - vt, 0), to = there ? lim[b] - vt : 0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = ((j >= from) & (j < to)) ? s[b][j / 4][j % 4] : -__builtin_inff();
+        }
+      }
+      uint32_t p[NB][8];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float top = s[b][0][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, s[b][j / 4][j % 4]);
+        top = fmaxf(max4(top), m[b]);
+        const float base = top == -__builtin_inff() ? 0.0f : top;   // nothing seen yet
+        if (__any(top > m[b])) {
+          const float old = __builtin_amdgcn_exp2f(m[b] - base);
+          l[b] *= old;
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d) o[b][d] *= old;
+          m[b] = top;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          float x = __builtin_amdgcn_exp2f(s[b][j / 4][j % 4] - base), y = __builtin_amdgcn_exp2f(s[b][j / 4][j % 4 + 1] - base);
+          sum += x + y;
+          if constexpr (Q8) {   // 0 for a masked position, whatever its scale
+            const f32x2 vs = *reinterpret_cast<const f32x2*>(&scales[buf][kBlock + 16 * g + j]);
+            x = x != 0.0f ? x * vs[0] : 0.0f;
+            y = y != 0.0f ? y * vs[1] : 0.0f;
+          }
+          p[b][j / 2] = pack(x, y);
+        }
+        l[b] += sum;
+      }
+      auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
+      if (!Q8 && edge) {
+        // As with few rows: what is not there or not for any row becomes zeros, and a value that is not
+        // finite where only some of the rows see it makes NaN of those.
+        const int from = there ? fst - vt : 16, to = there ? most - vt : 16;
+#pragma unroll 1
+        for (int d = 0; d < kTiles; ++d) {
+          if (16 * d >= dim) break;
+          uint4 v[2], ones[2];
+          int odd = 0;
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            v[st] = keep(*reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st)), 8 * st, from, to);
+            odd |= odd_exp(v[st].x) | odd_exp(v[st].y) | odd_exp(v[st].z) | odd_exp(v[st].w);
+          }
+          const bool apart = least != most && __any(odd);
+          if (apart) {
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              part_odd(v[st].x, ones[st].x);
+              part_odd(v[st].y, ones[st].y);
+              part_odd(v[st].z, ones[st].z);
+              part_odd(v[st].w, ones[st].w);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            f32x4 add = {};
+            if (apart) {
+#pragma unroll
+              for (int st = 0; st < 2; ++st) add = mfma(ones[st], quad(p[b] + 4 * st), add);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) add[i] = add[i] != 0.0f ? __builtin_nanf("") : 0.0f;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) add = mfma(v[st], quad(p[b] + 4 * st), add);
+#pragma unroll
+            for (int dd = 0; dd < kTiles; ++dd)   // (registers are not indexed)
+              if (dd == d) o[b][dd] += add;
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) {
+        if (DH != 64 && 16 * d >= dim) break;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st));
+#pragma unroll
+          for (int b = 0; b < NB; ++b) o[b][d] = mfma(v, quad(p[b] + 4 * st), o[b][d]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float sum = sum4(l[b]);
+    const int r = w0 + 16 * b + c;
+    if (r >= n_all) continue;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < kTiles; ++d) {
+      if (16 * d >= dim) break;
+      const f32x4 v = o[b][d] * inv;
+      *reinterpret_cast<uint2*>(op[b] + 16 * d + 4 * g) = make_uint2(pack(v[0], v[1]), pack(v[2], v[3]));
+    }
+    if (a.lse && g == 0)
+      a.lse[(int64_t)(sq.row0 + r / a.shared) * a.n_heads + head * a.shared + r % a.shared] = sum == 0.0f ? -__builtin_inff() : (m[b] + log2f(sum)) * kLn2;
+  }
+}
+
+template <int DH, int NB>
+hipError_t many(const AttnArgs& a, hipStream_t s) {
+  const ManyArgs f{a, (int)(((int64_t)a.max_new * a.shared + 64 * NB - 1) / (64 * NB))};
+  const dim3 grid((unsigned)((int64_t)f.tiles * a.c.n_heads), a.c.n_seqs);
+  if (a.c.store == C4S_KV_Q8) hipLaunchKernelGGL((k_attn_many<DH, true, NB>), grid, dim3(kAttnThreads), 0, s, f);
+  else hipLaunchKernelGGL((k_attn_many<DH, false, NB>), grid, dim3(kAttnThreads), 0, s, f);
+  return hipGetLastError();
+}
+
+bool many_pays(const AttnArgs& a) { return (int64_t)a.max_new * a.shared > (getenv("C4S_MANY") ? atoi(getenv("C4S_MANY")) : 32); }
+
 }  // namespace
 
 LayerSpace attn_space(const AttnArgs& a) {
+  if (many_pays(a)) return {};
   const FewArgs f = few_args(a);
   if (f.splits == 1) return {};
   const int64_t groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
@@ -510,6 +821,11 @@ LayerSpace attn_space(const AttnArgs& a) {
 }
 
 hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipStream_t s) {
+  if (many_pays(a)) {
+    if (a.c.dim <= 64) return many<64, 2>(a, s);
+    if (a.c.dim <= 128) return many<128, 2>(a, s);
+    return many<256, 1>(a, s);
+  }
   FewArgs f = few_args(a);
   f.arrived = counters;
   f.part = space;
