@@ -13,7 +13,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "c4s_join.hpp"
 #include "c4s_layers.hpp"
@@ -54,13 +53,20 @@ __device__ __forceinline__ uint4 codes(uint2 q) {
 __device__ __forceinline__ void here(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
 
 // Over the four lanes that share a row.
+// (v_permlane16_swap exchanges one operand's odd rows of 16 lanes with the
+// other's even ones, v_permlane32_swap the halves: of v with itself the two
+// results hold v and its partner.)
 __device__ __forceinline__ float max4(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum4(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 // Dwords of two bf16, of which those at index lo .. hi - 1 stay and the others become zero.
@@ -517,9 +523,11 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
 // Weights enter the second product rounded to bf16 once: independent roundings
 // of 2^-9 at most, which add a quarter to the error of the output's own
 // rounding; as pairs, as with few rows, they would cost half as many matrix
-// instructions again. Their sum is taken before the rounding, in fp32.
+// instructions again. Their sum is taken before the rounding, in fp32 (from the
+// matrix engine, of the rounded weights, it would be cheaper and lse off by 3e-4).
 constexpr int kBlock = 64;         // positions
 constexpr int kSegment = 16384;    // positions whose pages LDS holds at a time
+constexpr float kSlack = 8.0f;     // weights stay below 2^kSlack: rows are rescaled only when that would not hold
 
 struct ManyArgs {
   AttnArgs a;
@@ -539,19 +547,26 @@ __device__ __forceinline__ int value_piece(int r, int p) {
   return (r * 8 + (p ^ (((r >> 1) & 1) << 1 | ((r >> 2) & 1) | ((r >> 3) & 1) << 2))) * 16;
 }
 
-template <int DH, bool Q8, int NB>
-__global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(ManyArgs f) {
+template <int DH, bool Q8, int NB, int W, int OCC>
+__global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   constexpr int kSteps = DH / 32, kTiles = DH / 16, kNP = DH / 8;   // kNP: pieces of a key
-  constexpr int kLoads = (Q8 ? DH / 64 : DH / 32);                  // a thread's, of the keys and of the values
+  constexpr int kThreads = 64 * W, kPieces = kBlock * DH / (Q8 ? 16 : 8);      // of a block's keys, and of its values
+  constexpr int kLoads = kPieces < kThreads ? 1 : kPieces / kThreads;               // a thread's
+  constexpr int kStagers = kPieces < kThreads ? kPieces : kThreads;                 // threads that have some
   constexpr int kBuf = 2 * kBlock * DH * 2;
   __shared__ __align__(16) char lds[2][kBuf];
   __shared__ __align__(16) float scales[2][Q8 ? 2 * kBlock : 4];    // [buffer][keys', values']
   __shared__ int32_t pages[kSegment / 16];
+  // Values that are not finite where only some of a block's rows see them: by dim (codes: for all dims), the
+  // first position of one. They enter the products as zeros, and rows that end behind it become NaN. (What an
+  // earlier block left here did that already to the rows it is for.)
+  __shared__ int bad[Q8 ? 1 : DH];
+  __shared__ int odd[2][W];   // whether a wave staged such values
   const AttnArgs& a = f.a;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, c = lane % 16, g = lane / 16;
   const int dim = a.c.dim, head = blockIdx.x % a.c.n_heads, tile = f.tiles - 1 - blockIdx.x / a.c.n_heads, seq = blockIdx.y;
   const Seq sq(a, seq);
-  const int n_all = sq.n_new * a.shared, r0 = tile * 64 * NB;
+  const int n_all = sq.n_new * a.shared, r0 = tile * 16 * NB * W;
   if (r0 >= n_all) return;
   const int fst = sq.fst, shift = a.c.page_shift, ps = 1 << shift;
   // This wave's rows; a lane has row 16 b + c of each block b.
@@ -571,23 +586,30 @@ __global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(M
     least = min(sq.past + w0 / a.shared + 1, sq.cap);
     most = min(sq.past + min(w0 + 16 * NB - 1, n_all - 1) / a.shared + 1, sq.cap);
   }
-  const int kend = min(sq.past + min(r0 + 64 * NB - 1, n_all - 1) / a.shared + 1, sq.cap);   // the workgroup's last
+  const int kend = min(sq.past + min(r0 + 16 * NB * W - 1, n_all - 1) / a.shared + 1, sq.cap);   // the workgroup's last
 
+  const int first_lim = min(sq.past + r0 / a.shared + 1, sq.cap);                              // ... and its first
+
+  // Scores become powers of two's exponents by one multiplication with a positive factor: a negative scale
+  // turns q's signs, and none at all is so small that the weights are equal.
+  const uint32_t turn = a.scale < 0.0f ? 0x80008000u : 0u;
+  const float c2 = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-100f);
   uint4 q[NB][kSteps];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      q[b][s] = 32 * s + 8 * g < dim ? *reinterpret_cast<const uint4*>(qp[b] + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < kSteps; ++s) {
+      const uint4 w = 32 * s + 8 * g < dim ? *reinterpret_cast<const uint4*>(qp[b] + 32 * s + 8 * g) : make_uint4(0, 0, 0, 0);
+      q[b][s] = make_uint4(w.x ^ turn, w.y ^ turn, w.z ^ turn, w.w ^ turn);
+    }
 
   constexpr int kSize = Q8 ? 1 : 2;
   const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;
   const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head;
   const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
-  const float c2 = a.scale * kLog2e;
-
-  float m[NB], l[NB];
+  float m[NB];   // what the weights are relative to (as exponents of two), within kSlack of the maximum seen
+  float l[NB];   // a lane's part of the weights' sum
   f32x4 o[NB][kTiles] = {};
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -595,71 +617,110 @@ __global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(M
     l[b] = 0.0f;
   }
 
+  for (int i = tid; i < (Q8 ? 1 : DH); i += kThreads) bad[i] = INT32_MAX;
   for (int seg = fst & ~(kSegment - 1); seg < kend; seg += kSegment) {
     const int begin = max(seg, fst & ~(kBlock - 1)), end = min(seg + kSegment, kend);
     __syncthreads();
-    for (int i = tid; i < kSegment >> shift; i += kAttnThreads) {
+    for (int i = tid; i < kSegment >> shift; i += kThreads) {
       const int at = (seg >> shift) + i;
       const int p = at < a.c.max_pages ? table[at] : -1;
       pages[i] = p < a.c.n_pages ? p : -1;
     }
     __syncthreads();
+    bool missing = false;   // whether a page of the segment is not there
+    for (int i = tid; i < (end - seg + ps - 1) >> shift; i += kThreads) missing |= pages[i] < 0 && (i + 1) * ps + seg > fst;
+    missing = __syncthreads_or(missing);
     uint4 kst[kLoads], vst[kLoads];
     float sst = 0.0f;
-    auto page_of = [&](int pos) { return (uint64_t)(uint32_t)max(pages[(pos - seg) >> shift], 0); };   // what has no page is dropped
-    // A thread's pieces: of the keys in order; of the values in the order in which a page has them.
-    const int row_shift = min(shift, 6) - (Q8 ? 4 : 3);   // log2 of the pieces a page's row has in a block
+    // A thread's pieces of a block: of the keys in order; of the values in the order in which a page has them.
+    // A block begins at a multiple of 64, so that of a piece's place in its page and in the table only what
+    // the block adds changes.
+    constexpr int kKP = Q8 ? DH / 16 : DH / 8, kPer = Q8 ? 16 : 8;   // a key's pieces; dims or positions a piece
+    const int row_shift = min(shift, 6) - (Q8 ? 4 : 3);              // log2 of the pieces a page's row has in a block
+    auto key_of = [&](int i) { return (tid + kThreads * i) / kKP; };
+    auto dim_of = [&](int i) { return ((tid + kThreads * i) >> row_shift) % DH; };   // of a piece of values, and which of its row
+    auto piece_of = [&](int i) {
+      const int at = tid + kThreads * i;
+      return (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
+    };
+    auto page_at = [&](int t, int in) { return (uint64_t)(uint32_t)max(pages[((t - seg) >> shift) + (in >> shift)], 0); };   // what has no page is dropped
     auto load = [&](int t) {
+      const uint32_t key_add = (uint32_t)((t & (ps - 1)) * dim * kSize), value_add = (uint32_t)((t & (ps - 1)) * kSize);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int at = tid + kAttnThreads * i;
-        constexpr int kKP = Q8 ? DH / 16 : DH / 8;   // a key's pieces
-        const int key = t + at / kKP, d = at % kKP * (Q8 ? 16 : 8);
+        if (kStagers < kThreads && tid >= kStagers) break;
+        const int d = tid % kKP * kPer;   // the threads are a multiple of a key's pieces
         kst[i] = make_uint4(0, 0, 0, 0);
-        if (DH == 64 || DH == 256 || d < dim)
-          if (d < dim)
-            kst[i] = *reinterpret_cast<const uint4*>(kbase + page_of(key) * page_bytes + (uint32_t)((key & (ps - 1)) * dim + d) * kSize);
-        const int vd = (at >> row_shift) % DH, piece = (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
-        const int pos = t + piece * (Q8 ? 16 : 8);
-        vst[i] = *reinterpret_cast<const uint4*>(vbase + page_of(pos) * page_bytes + (uint32_t)((min(vd, dim - 1) << shift) + (pos & (ps - 1))) * kSize);
+        if (d < dim)
+          kst[i] = *reinterpret_cast<const uint4*>(kbase + key_add + page_at(t, key_of(i)) * page_bytes + (uint32_t)(((key_of(i) & (ps - 1)) * dim + d) * kSize));
+        const int pos = piece_of(i) * kPer;
+        vst[i] = *reinterpret_cast<const uint4*>(vbase + value_add + page_at(t, pos) * page_bytes + (uint32_t)(((min(dim_of(i), dim - 1) << shift) + (pos & (ps - 1))) * kSize));
       }
       if constexpr (Q8) {
         if (tid < 2 * kBlock) {
           const int pos = t + tid % kBlock;
-          sst = (tid < kBlock ? a.c.k_scale : a.c.v_scale)[(page_of(pos) * a.c.n_heads + head << shift) + (pos & (ps - 1))];
+          sst = (tid < kBlock ? a.c.k_scale : a.c.v_scale)[(page_at(t, tid % kBlock) * a.c.n_heads + head << shift) + (pos & (ps - 1))];
         }
       }
     };
-    auto stage = [&](int buf) {
+    auto stage = [&](int t, int buf) {
       char* kl = lds[buf];
       char* vl = kl + kBlock * DH * 2;
+      // What is not there or not for any row may hold anything: zeros (codes: their scales).
+      int strange = 0;
+      const bool edge = t < fst || t + kBlock > first_lim || missing;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int at = tid + kAttnThreads * i;
-        constexpr int kKP = Q8 ? DH / 16 : DH / 8;
-        const int vd = (at >> row_shift) % DH, piece = (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
+        if (kStagers < kThreads && tid >= kStagers) break;
+        const int vd = dim_of(i), piece = piece_of(i);
         if constexpr (Q8) {
-          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP * 2)) = codes(make_uint2(kst[i].x, kst[i].y));
-          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP * 2 + 1)) = codes(make_uint2(kst[i].z, kst[i].w));
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2)) = codes(make_uint2(kst[i].x, kst[i].y));
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2 + 1)) = codes(make_uint2(kst[i].z, kst[i].w));
           *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece)) = codes(make_uint2(vst[i].x, vst[i].y));
           *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece + 1)) = codes(make_uint2(vst[i].z, vst[i].w));
         } else {
-          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(at / kKP, at % kKP)) = kst[i];
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP)) = kst[i];
+          if (edge) {
+            const int pos = t + 8 * piece;
+            const bool there = pages[(pos - seg) >> shift] >= 0;
+            vst[i] = keep(vst[i], 0, fst - pos, there ? kend - pos : 0);
+            if (odd_exp(vst[i].x) | odd_exp(vst[i].y) | odd_exp(vst[i].z) | odd_exp(vst[i].w)) {
+              strange = 1;
+              uint32_t w[4] = {vst[i].x, vst[i].y, vst[i].z, vst[i].w}, was;
+#pragma unroll
+              for (int j = 3; j >= 0; --j) {
+                part_odd(w[j], was);
+                if (was) atomicMin(&bad[vd], pos + 2 * j + (was & 0xFFFFu ? 0 : 1));
+              }
+              vst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
           *reinterpret_cast<uint4*>(vl + value_piece(vd, piece)) = vst[i];
         }
       }
       if constexpr (Q8) {
-        if (tid < 2 * kBlock) scales[buf][tid] = sst;
+        if (tid < 2 * kBlock) {
+          const int pos = t + tid % kBlock;
+          if (edge && (pos < fst || pos >= kend || pages[(pos - seg) >> shift] < 0)) sst = 0.0f;
+          if (edge && tid >= kBlock && !(sst - sst == 0.0f)) {
+            strange = 1;
+            sst = 0.0f;
+            atomicMin(&bad[0], pos);
+          }
+          scales[buf][tid] = sst;
+        }
       }
+      const bool mark = __any(strange);
+      if (lane == 0) odd[buf][wave] = mark;
     };
     load(begin);
-    stage(0);
+    stage(begin, 0);
     if (begin + kBlock < end) load(begin + kBlock);
     int buf = 0;
     for (int t = begin; t < end; t += kBlock, buf ^= 1) {
       __syncthreads();   // this block is there, and the other buffer has been read
       if (t + kBlock < end) {
-        stage(buf ^ 1);
+        stage(t + kBlock, buf ^ 1);
         if (t + 2 * kBlock < end) load(t + 2 * kBlock);
       }
       if (t >= most) continue;   // no row of this wave sees it
@@ -678,98 +739,56 @@ __global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(M
       if constexpr (Q8) {
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[buf][16 * g + 4 * tt]) * c2;
+          const f32x4 ks = *reinterpret_cast<const f32x4*>(&scales[buf][16 * g + 4 * tt]);
 #pragma unroll
           for (int b = 0; b < NB; ++b) s[b][tt] *= ks;
         }
-      } else {
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-          for (int b = 0; b < NB; ++b) s[b][tt] *= c2;
       }
-      const bool there = pages[(vt - seg) >> shift] >= 0;
-      const bool edge = t < fst || t + kBlock > least || __any(!there);
-      if (edge) {
+      if (t + kBlock > least || missing) {
+        const bool there = pages[(vt - seg) >> shift] >= 0;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const int from = max(fst - vt, 0), to = there ? lim[b] - vt : 0;
+          const int to = there ? lim[b] - vt : 0;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = ((j >= from) & (j < to)) ? s[b][j / 4][j % 4] : -__builtin_inff();
+          for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = j < to ? s[b][j / 4][j % 4] : -__builtin_inff();
         }
+      }
+      if (t < fst) {
+        const int from = fst - vt;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = j < from ? -__builtin_inff() : s[b][j / 4][j % 4];
       }
       uint32_t p[NB][8];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float top = s[b][0][0];
+        float top = fmaxf(s[b][0][0], s[b][0][1]);
 #pragma unroll
-        for (int j = 1; j < 16; ++j) top = fmaxf(top, s[b][j / 4][j % 4]);
-        top = fmaxf(max4(top), m[b]);
-        const float base = top == -__builtin_inff() ? 0.0f : top;   // nothing seen yet
-        if (__any(top > m[b])) {
-          const float old = __builtin_amdgcn_exp2f(m[b] - base);
+        for (int j = 2; j < 16; ++j) top = fmaxf(top, s[b][j / 4][j % 4]);
+        if (__any(top * c2 > m[b] + kSlack)) {   // seldom, after a row's first block
+          top = fmaxf(max4(top) * c2, m[b]);
+          const float old = __builtin_amdgcn_exp2f(m[b] - (top == -__builtin_inff() ? 0.0f : top));
           l[b] *= old;
 #pragma unroll
           for (int d = 0; d < kTiles; ++d) o[b][d] *= old;
           m[b] = top;
         }
-        float sum = 0.0f;
+        const float base = m[b] == -__builtin_inff() ? 0.0f : m[b];   // nothing seen yet
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          float x = __builtin_amdgcn_exp2f(s[b][j / 4][j % 4] - base), y = __builtin_amdgcn_exp2f(s[b][j / 4][j % 4 + 1] - base);
-          sum += x + y;
-          if constexpr (Q8) {   // 0 for a masked position, whatever its scale
+          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j / 4][j % 4], c2, -base));
+          float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j / 4][j % 4 + 1], c2, -base));
+          l[b] += x + y;
+          if constexpr (Q8) {
             const f32x2 vs = *reinterpret_cast<const f32x2*>(&scales[buf][kBlock + 16 * g + j]);
-            x = x != 0.0f ? x * vs[0] : 0.0f;
-            y = y != 0.0f ? y * vs[1] : 0.0f;
+            x *= vs[0];
+            y *= vs[1];
           }
           p[b][j / 2] = pack(x, y);
         }
-        l[b] += sum;
       }
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
-      if (!Q8 && edge) {
-        // As with few rows: what is not there or not for any row becomes zeros, and a value that is not
-        // finite where only some of the rows see it makes NaN of those.
-        const int from = there ? fst - vt : 16, to = there ? most - vt : 16;
-#pragma unroll 1
-        for (int d = 0; d < kTiles; ++d) {
-          if (16 * d >= dim) break;
-          uint4 v[2], ones[2];
-          int odd = 0;
-#pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            v[st] = keep(*reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st)), 8 * st, from, to);
-            odd |= odd_exp(v[st].x) | odd_exp(v[st].y) | odd_exp(v[st].z) | odd_exp(v[st].w);
-          }
-          const bool apart = least != most && __any(odd);
-          if (apart) {
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-              part_odd(v[st].x, ones[st].x);
-              part_odd(v[st].y, ones[st].y);
-              part_odd(v[st].z, ones[st].z);
-              part_odd(v[st].w, ones[st].w);
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            f32x4 add = {};
-            if (apart) {
-#pragma unroll
-              for (int st = 0; st < 2; ++st) add = mfma(ones[st], quad(p[b] + 4 * st), add);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) add[i] = add[i] != 0.0f ? __builtin_nanf("") : 0.0f;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) add = mfma(v[st], quad(p[b] + 4 * st), add);
-#pragma unroll
-            for (int dd = 0; dd < kTiles; ++dd)   // (registers are not indexed)
-              if (dd == d) o[b][dd] += add;
-          }
-        }
-        continue;
-      }
 #pragma unroll
       for (int d = 0; d < kTiles; ++d) {
         if (DH != 64 && 16 * d >= dim) break;
@@ -779,6 +798,18 @@ __global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(M
 #pragma unroll
           for (int b = 0; b < NB; ++b) o[b][d] = mfma(v, quad(p[b] + 4 * st), o[b][d]);
         }
+      }
+      int strange = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) strange |= odd[buf][w];
+      if (strange) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (bad[Q8 ? 0 : 16 * d + 4 * g + i] < lim[b]) o[b][d][i] = __builtin_nanf("");
       }
     }
   }
@@ -799,16 +830,21 @@ __global__ __launch_bounds__(kAttnThreads, DH == 256 ? 1 : 2) void k_attn_many(M
   }
 }
 
-template <int DH, int NB>
+template <int DH, bool Q8, int NB, int W, int OCC>
 hipError_t many(const AttnArgs& a, hipStream_t s) {
-  const ManyArgs f{a, (int)(((int64_t)a.max_new * a.shared + 64 * NB - 1) / (64 * NB))};
-  const dim3 grid((unsigned)((int64_t)f.tiles * a.c.n_heads), a.c.n_seqs);
-  if (a.c.store == C4S_KV_Q8) hipLaunchKernelGGL((k_attn_many<DH, true, NB>), grid, dim3(kAttnThreads), 0, s, f);
-  else hipLaunchKernelGGL((k_attn_many<DH, false, NB>), grid, dim3(kAttnThreads), 0, s, f);
+  const ManyArgs f{a, (int)(((int64_t)a.max_new * a.shared + 16 * NB * W - 1) / (16 * NB * W))};
+  hipLaunchKernelGGL((k_attn_many<DH, Q8, NB, W, OCC>), dim3((unsigned)((int64_t)f.tiles * a.c.n_heads), a.c.n_seqs), dim3(64 * W), 0, s, f);
   return hipGetLastError();
 }
 
-bool many_pays(const AttnArgs& a) { return (int64_t)a.max_new * a.shared > (getenv("C4S_MANY") ? atoi(getenv("C4S_MANY")) : 32); }
+// Few rows' tiles re-read the positions but share them out over the chip: they win while they are few (many /
+// few rows' kernel, us: 4 rows of 128 over 4000, 20 heads of 64, 640 tiles: 78 / 70; 4 of 300 over 500, 1520
+// tiles: 22 / 31; 1 of 300, 8 key heads of 128 with 4 query heads each, 600 tiles: 21 / 14; 16 of 32, 1024
+// tiles: 11 / 13), and where a sequence has one tile, of which the other kernel would leave most rows empty.
+bool many_pays(const AttnArgs& a) {
+  const int64_t tiles = ((int64_t)a.max_new * a.shared + kRows - 1) / kRows;
+  return tiles > 1 && tiles * a.c.n_heads * a.c.n_seqs > 700;
+}
 
 }  // namespace
 
@@ -822,9 +858,9 @@ LayerSpace attn_space(const AttnArgs& a) {
 
 hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipStream_t s) {
   if (many_pays(a)) {
-    if (a.c.dim <= 64) return many<64, 2>(a, s);
-    if (a.c.dim <= 128) return many<128, 2>(a, s);
-    return many<256, 1>(a, s);
+    if (a.c.dim <= 64) return a.c.store == C4S_KV_Q8 ? many<64, true, 1, 8, 4>(a, s) : many<64, false, 1, 8, 4>(a, s);
+    if (a.c.dim <= 128) return a.c.store == C4S_KV_Q8 ? many<128, true, 2, 8, 2>(a, s) : many<128, false, 2, 8, 2>(a, s);
+    return a.c.store == C4S_KV_Q8 ? many<256, true, 1, 8, 2>(a, s) : many<256, false, 1, 8, 2>(a, s);
   }
   FewArgs f = few_args(a);
   f.arrived = counters;
