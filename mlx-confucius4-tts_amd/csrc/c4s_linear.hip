@@ -21,6 +21,7 @@ namespace c4s {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 Quad __attribute__((ext_vector_type(4)));   // rounds to nearest even
 
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -70,33 +71,23 @@ __device__ __forceinline__ uint4 centred(uint2 q) {
 __device__ __forceinline__ float sigmoid_of(float y, float z) {
   return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z));
 }
-__device__ __forceinline__ float activate(float y, int act) {
-  if (act == C4S_ACT_GELU)   // y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
-    return sigmoid_of(y, y * __builtin_fmaf(-0.10294324f, y * y, -2.3022082f));
-  if (act == C4S_ACT_SILU) return sigmoid_of(y, y * -1.4426950408889634f);
-  if (act == C4S_ACT_RELU) return y > 0.0f ? y : (y != y ? y : 0.0f);
-  return y;
+template <int N>
+__device__ __forceinline__ void activate(float (&y)[N], int act) {
+  if (act == C4S_ACT_GELU) {   // y / 2 (1 + tanh u) = y / (1 + exp(-2 u)), u = sqrt(2 / pi) (y + 0.044715 y^3)
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = sigmoid_of(y[i], y[i] * __builtin_fmaf(-0.10294324f, y[i] * y[i], -2.3022082f));
+  } else if (act == C4S_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = sigmoid_of(y[i], y[i] * -1.4426950408889634f);
+  } else if (act == C4S_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = y[i] > 0.0f ? y[i] : (y[i] != y[i] ? y[i] : 0.0f);
+  }
 }
 
-// Four consecutive outputs n .. n + 3 of row m: bias, activation, residual, store.
-// Few: n + 3 may lie behind the last output, or the tensors' rows off four elements' alignment.
-__device__ __forceinline__ void finish(const c4s_linear_desc& a, bool vec, int m, int n, f32x4 y) {
-  if (!vec) {
-#pragma unroll 1
-    for (int i = 0; i < 4 && n + i < a.N; ++i) {
-      float v = i < 2 ? (i ? y[1] : y[0]) : (i > 2 ? y[3] : y[2]);
-      v = activate(v + (a.bias ? a.bias[n + i] : 0.0f), a.act);
-      const int64_t r = (int64_t)m * a.ld_res + n + i, o = (int64_t)m * a.ld_out + n + i;
-      if (a.residual)
-        v += a.res_dtype == C4S_DTYPE_BF16 ? from_bf16(static_cast<const uint16_t*>(a.residual)[r]) : static_cast<const float*>(a.residual)[r];
-      if (a.out_dtype == C4S_DTYPE_BF16) static_cast<uint16_t*>(a.out)[o] = (uint16_t)to_bf16(v);
-      else static_cast<float*>(a.out)[o] = v;
-    }
-    return;
-  }
-  if (n >= a.N) return;
-  f32x4 b = {}, r = {};
-  if (a.bias) b = *reinterpret_cast<const f32x4*>(a.bias + n);
+// Activation, residual and store of four outputs n .. n + 3 of row m, with the bias in y.
+__device__ __forceinline__ void finish4(const c4s_linear_desc& a, int m, int n, f32x4 y) {
+  f32x4 r = {};
   const int64_t ro = (int64_t)m * a.ld_res + n, o = (int64_t)m * a.ld_out + n;
   if (a.residual) {
     if (a.res_dtype == C4S_DTYPE_BF16) {
@@ -106,13 +97,37 @@ __device__ __forceinline__ void finish(const c4s_linear_desc& a, bool vec, int m
       r = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + ro);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = activate(y[i] + b[i], a.act);
+  float v[4] = {y[0], y[1], y[2], y[3]};
+  activate(v, a.act);
+  y = f32x4{v[0], v[1], v[2], v[3]};
   if (a.residual) y += r;
   if (a.out_dtype == C4S_DTYPE_BF16)
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) = make_uint2(to_bf16(y[0]) | to_bf16(y[1]) << 16, to_bf16(y[2]) | to_bf16(y[3]) << 16);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) = __builtin_bit_cast(uint2, Quad{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]});
   else
     *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + o) = y;
+}
+
+// Four consecutive outputs n .. n + 3 of row m: bias, activation, residual, store.
+// Few: n + 3 may lie behind the last output, or the tensors' rows off four elements' alignment.
+__device__ __forceinline__ void finish(const c4s_linear_desc& a, bool vec, int m, int n, f32x4 y) {
+  if (!vec) {
+#pragma unroll 1
+    for (int i = 0; i < 4 && n + i < a.N; ++i) {
+      float u[1] = {(i < 2 ? (i ? y[1] : y[0]) : (i > 2 ? y[3] : y[2])) + (a.bias ? a.bias[n + i] : 0.0f)};
+      activate(u, a.act);
+      float v = u[0];
+      const int64_t r = (int64_t)m * a.ld_res + n + i, o = (int64_t)m * a.ld_out + n + i;
+      if (a.residual)
+        v += a.res_dtype == C4S_DTYPE_BF16 ? from_bf16(static_cast<const uint16_t*>(a.residual)[r]) : static_cast<const float*>(a.residual)[r];
+      if (a.out_dtype == C4S_DTYPE_BF16) static_cast<uint16_t*>(a.out)[o] = (uint16_t)to_bf16(v);
+      else static_cast<float*>(a.out)[o] = v;
+    }
+    return;
+  }
+  if (n >= a.N) return;
+  f32x4 b = {};
+  if (a.bias) b = *reinterpret_cast<const f32x4*>(a.bias + n);
+  finish4(a, m, n, y + b);
 }
 
 // Whether finish() may use vectors.
@@ -370,16 +385,29 @@ template <int NW, int MW>
 __device__ __forceinline__ void write_tile(const ManyArgs& f, char* lds, int wave, int m, int n, const f32x4 (&acc)[NW][MW]) {
   constexpr int kPitch = 16 * NW + 4, kQuads = 4 * NW;
   const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
+  static_assert(64 % kQuads == 0, "a lane keeps its outputs");
   float* red = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
+  const int at = 4 * (lane % kQuads);
+  f32x4 b = {};
+  if (f.vec && f.d.bias && n + at < f.d.N) b = *reinterpret_cast<const f32x4*>(f.d.bias + n + at);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < MW; ++j) {
 #pragma unroll
     for (int i = 0; i < NW; ++i) *reinterpret_cast<f32x4*>(red + c * kPitch + 16 * i + 4 * g) = acc[i][j];
+    if (f.vec) {
+      if (n + at >= f.d.N) continue;
+#pragma unroll
+      for (int q = lane; q < 16 * kQuads; q += 64) {
+        const int row = m + 16 * j + q / kQuads;
+        if (row < f.d.M) finish4(f.d, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at) + b);
+      }
+    } else {
 #pragma unroll 1
-    for (int q = lane; q < 16 * kQuads; q += 64) {
-      const int row = m + 16 * j + q / kQuads, at = 4 * (q % kQuads);
-      if (row < f.d.M) finish(f.d, f.vec, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at));
+      for (int q = lane; q < 16 * kQuads; q += 64) {
+        const int row = m + 16 * j + q / kQuads;
+        if (row < f.d.M) finish(f.d, false, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at));
+      }
     }
   }
 }
