@@ -85,7 +85,16 @@ __device__ __forceinline__ void activate(float (&y)[N], int act) {
   }
 }
 
-// Activation, residual and store of four outputs n .. n + 3 of row m, with the bias in y.
+template <bool PAST, class V>
+__device__ __forceinline__ void put(V* p, V v) {
+  if (PAST) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
+// Activation, residual and store of four outputs n .. n + 3 of row m, with the bias
+// in y. PAST: the store goes past the caches, which keeps the operands of many rows'
+// tiles in them (12345 x 5120 x 1280: 180 us, and 170 so).
+template <bool PAST = false>
 __device__ __forceinline__ void finish4(const c4s_linear_desc& a, int m, int n, f32x4 y) {
   f32x4 r = {};
   const int64_t ro = (int64_t)m * a.ld_res + n, o = (int64_t)m * a.ld_out + n;
@@ -102,9 +111,9 @@ __device__ __forceinline__ void finish4(const c4s_linear_desc& a, int m, int n, 
   y = f32x4{v[0], v[1], v[2], v[3]};
   if (a.residual) y += r;
   if (a.out_dtype == C4S_DTYPE_BF16)
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) = __builtin_bit_cast(uint2, Quad{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]});
+    put<PAST>(reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + o), __builtin_bit_cast(u32x2, Quad{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]}));
   else
-    *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + o) = y;
+    put<PAST>(reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + o), y);
 }
 
 // Four consecutive outputs n .. n + 3 of row m: bias, activation, residual, store.
@@ -400,7 +409,7 @@ __device__ __forceinline__ void write_tile(const ManyArgs& f, char* lds, int wav
 #pragma unroll
       for (int q = lane; q < 16 * kQuads; q += 64) {
         const int row = m + 16 * j + q / kQuads;
-        if (row < f.d.M) finish4(f.d, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at) + b);
+        if (row < f.d.M) finish4<true>(f.d, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at) + b);
       }
     } else {
 #pragma unroll 1
