@@ -15,7 +15,7 @@
  * Conventions are those of c4s_sampling.h: status codes, device pointers, work
  * queued on the given stream, text of the last failure from c4s_last_error. A
  * call that fails its checks queues nothing. A call with no rows queues nothing
- * and returns C4S_OK. All four may be captured into a graph (c4s_attn and
+ * and returns C4S_OK. All of them may be captured into a graph (c4s_attn and
  * c4s_linear with a workspace: after a call of that size outside a capture).
  *
  * Activations are bf16, the residual stream bf16 or fp32; sums, softmax
@@ -167,7 +167,10 @@ int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_kv_rows* rows
  *   out[r][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[r][h] . k_j),
  * with the keys and values of head h / (n_heads / n_kv_heads); a row that sees
  * nothing is zero. Values that are not finite matter only to rows that see them
- * (those read inf or NaN). */
+ * (those read inf or NaN).
+ * Refused (C4S_EINVAL): max_pages above 1024 together with more than 262144 of
+ * (sequence, key head, 16 of its new rows' query heads), where few rows a sequence
+ * have their positions' parts joined. */
 typedef struct c4s_attn_desc {
   const uint16_t* q;            /* [n_rows][ldq] bf16: row r's head h at q + r * ldq + h * head_dim; 16-byte aligned, ldq a multiple of 8 */
   int64_t ldq;

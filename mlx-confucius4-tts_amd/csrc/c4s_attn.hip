@@ -121,7 +121,7 @@ constexpr int kRows = 16;   // rows of a workgroup
 // own. Keys and values go from memory straight into the matrix engine's
 // registers; a block's keys are asked for as soon as the block before it has
 // given its scores, its values as soon as the values before them have been
-// used, and its pages one block earlier still, so that a wave always has about
+// used, and its pages are in LDS from the start, so that a wave always has about
 // a block in flight and never waits for a table. The waves' parts meet in LDS,
 // the chunks' in the workspace, where the last workgroup of a row joins them
 // (c4s_join.hpp), in the chunks' order.
@@ -132,7 +132,7 @@ constexpr int kRows = 16;   // rows of a workgroup
 constexpr int kWaves = 4;
 constexpr int kAttnThreads = 64 * kWaves;
 constexpr int kMaxParts = 128;       // chunks of a sequence
-constexpr int kMaxChunk = 16384;     // positions of a chunk: its pages fit the table in LDS
+constexpr int kMaxPages = 1024;      // a chunk's pages, in a table in LDS
 
 struct FewArgs {
   AttnArgs a;
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   const int seq = blockIdx.y;
   const int shift = a.c.page_shift, ps = 1 << shift;
   // The chunk's part of the table (-1: no page), asked for while the lengths are on their way.
-  __shared__ int32_t pages[kMaxChunk / 16 + 16];
+  __shared__ int32_t pages[kMaxPages + 16];
   const int base = split * f.chunk;
   auto fill = [&](int from) {
     const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
@@ -489,7 +489,7 @@ FewArgs few_args(const AttnArgs& a) {
   const int64_t coarse = std::max<int64_t>(512 / groups, 1), fine = std::max<int64_t>(2048 / groups, 1);
   int64_t chunk = std::min(cap / coarse, std::max<int64_t>(1280, cap / fine)) + 255;
   chunk = std::max(chunk, (cap + kMaxParts - 1) / kMaxParts + 255) / 256 * 256;
-  f.chunk = (int)std::min<int64_t>(std::max<int64_t>(chunk, 256), kMaxChunk);
+  f.chunk = (int)std::min<int64_t>(std::max<int64_t>(chunk, 256), (int64_t)kMaxPages << a.c.page_shift);
   f.splits = (int)std::max<int64_t>((cap + f.chunk - 1) / f.chunk, 1);
   return f;
 }
@@ -509,8 +509,8 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
 
 // ---- many rows ----------------------------------------------------------------------------
 //
-// Prompts: a workgroup has 64 NB rows of one sequence and key head, 16 NB a
-// wave, and goes through the positions in blocks of 64, which all four waves
+// Prompts: a workgroup has 16 NB W rows of one sequence and key head, 16 NB a
+// wave, and goes through the positions in blocks of 64, which all W waves
 // share: a block's keys and values are loaded (codes converted, once for all
 // rows) into registers while the block before it is worked on, and written to
 // the other of two buffers in LDS, with one barrier a block. The rows of both

@@ -136,7 +136,7 @@ constexpr size_t kNoAllocBytes = (size_t)8 << 20;
 hipError_t noalloc_scratch(void** ptr);
 
 // Bytes at the start of a decoder layer's workspace that are zero between calls.
-constexpr size_t kLayerZeroed = (size_t)1 << 18;
+constexpr size_t kLayerZeroed = (size_t)1 << 20;
 // Zeroes `bytes` (a multiple of 4) from p on.
 hipError_t launch_zero(void* p, size_t bytes, hipStream_t s);
 

@@ -110,6 +110,19 @@ class Cache:
         x = x.to(torch.float64)
         return x * self.t[name + "_scale"][pg, :, at, None].to(torch.float64) if self.q8 else x
 
+    def rows(self, name, b, n):
+        """(values [n][heads][dim] of sequence b's first n positions in float64, which of them have a page [n])."""
+        pos = torch.arange(n)
+        i = pos // self.page
+        pg = torch.where(i < self.table.shape[1], self.table[b, i.clamp(max=self.table.shape[1] - 1)].long(), torch.tensor(-1))
+        there = (pg >= 0) & (pg < self.n_pages)
+        pg, at = torch.where(there, pg, torch.tensor(0)), pos % self.page
+        x = self.t[name][pg, :, at] if name == "k" else self.t[name][pg, :, :, at]
+        x = x.to(torch.float64)
+        if self.q8:
+            x = x * self.t[name + "_scale"][pg, :, at, None].to(torch.float64)
+        return x, there
+
 
 def quantise(x):
     """8-bit codes and scales of rows of the last dimension, in the float32 steps of the definition."""
@@ -145,3 +158,19 @@ def attn(cache, q, n_new, heads, scale, first=None):
                     sq[r] = (w * v).square().sum(0).sqrt()
             r += 1
     return out, lse, mag, sq
+
+
+def attn_row(cache, b, pos, q, scale, first=0):
+    """One row of attn(): q [heads][dim] of sequence b's position pos."""
+    heads, shared = q.shape[0], q.shape[0] // cache.heads
+    k, there = cache.rows("k", b, pos + 1)
+    v, _ = cache.rows("v", b, pos + 1)
+    there[:max(0, min(first, pos + 1))] = False
+    if not there.any():
+        zero = torch.zeros(heads, cache.dim, dtype=torch.float64)
+        return zero, torch.full((heads,), -np.inf, dtype=torch.float64), zero, zero
+    k, v = (x[there].repeat_interleave(shared, 1) for x in (k, v))
+    z = (k * f64(q)[None]).sum(-1) * scale
+    lse = torch.logsumexp(z, 0)
+    w = torch.exp(z - lse)[..., None]
+    return (w * v).sum(0), lse, (w * v.abs()).sum(0), (w * v).square().sum(0).sqrt()
