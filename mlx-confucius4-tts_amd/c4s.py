@@ -11,6 +11,7 @@ import atexit
 import ctypes as C
 import os
 import re
+import struct
 import weakref
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -157,11 +158,10 @@ def lib() -> C.CDLL:
     L.c4s_head_weights_load.argtypes = [C.c_char_p, C.c_int32, C.c_int32, C.POINTER(HeadWeights)]
     L.c4s_head_weights_free.argtypes = [C.POINTER(HeadWeights)]
     L.c4s_weights_last_error.restype = C.c_char_p
-    L.c4s_block_norm.argtypes = [_vp, C.POINTER(Norm), _vp]
-    L.c4s_linear.argtypes = [_vp, C.POINTER(Linear), _vp]
-    L.c4s_kv_append.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(KvRows), _vp]
-    L.c4s_kv_read.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(KvRows), _vp]
-    L.c4s_attn.argtypes = [_vp, C.POINTER(KvCacheDesc), C.POINTER(Attn), _vp]
+    for f in (L.c4s_block_norm, L.c4s_linear):   # descriptors as bytes (_packer)
+        f.argtypes = [_vp, C.c_char_p, _vp]
+    for f in (L.c4s_kv_append, L.c4s_kv_read, L.c4s_attn):
+        f.argtypes = [_vp, C.c_char_p, C.c_char_p, _vp]
     _lib = L
     return L
 
@@ -237,63 +237,77 @@ def free_head_weights(hw: HeadWeights) -> None:
     lib().c4s_head_weights_free(C.byref(hw))
 
 
-# The layer calls come once a layer and AR step, so what they check is checked
-# in few Python operations: messages are constants, nothing is formatted.
+# The layer calls come once a layer and AR step, so their host time counts: what
+# they check is checked in few Python operations (an attribute of a tensor costs
+# about 0.1 us), messages are constants, and descriptors are packed as bytes,
+# which takes half the time of filling a ctypes structure.
+
+def _packer(cls):
+    """pack(*fields) -> the bytes of a ctypes structure; pointers as integers (0: NULL)."""
+    s = struct.Struct("@" + "".join({C.c_int32: "i", C.c_float: "f", C.c_int64: "q", _vp: "P"}[t]
+                                    for _, t in cls._fields_) + "0P")
+    assert s.size == C.sizeof(cls)
+    return s.pack
+
+
+_pack_norm, _pack_linear, _pack_rows, _pack_attn = (_packer(c) for c in (Norm, Linear, KvRows, Attn))
+
+
+class _Torch:
+    """torch's dtypes and its current stream, from the first context on."""
+    kinds, bf16, f32, i32, u8, raw_stream = {}, None, None, None, None, None
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.kinds = {torch.float32: F32, torch.bfloat16: BF16}
+        cls.bf16, cls.f32, cls.i32, cls.u8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+        cls.raw_stream = torch._C._cuda_getCurrentRawStream
+
 
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
 
 
-def _dtype(t, what) -> int:
-    """C4S_DTYPE_* of a tensor that is bfloat16 or float32."""
-    import torch
-    d = t.dtype
-    if d is torch.bfloat16:
-        return BF16
-    if d is torch.float32:
-        return F32
-    raise ValueError(what)
-
-
 def _vector(t, n, what):
-    """The address of a contiguous float32 vector of n values, or None."""
-    import torch
+    """The address of a contiguous float32 vector of n values; 0 of None."""
     if t is None:
-        return None
-    if t.dtype is torch.float32 and t.shape == (n,) and t.is_contiguous():
+        return 0
+    if t.dtype is _Torch.f32 and t.numel() == n and t.is_contiguous():
         return t.data_ptr()
     raise ValueError(what)
 
 
 def _i32(t, n, what):
-    """The address of a contiguous int32 vector of n values, or None."""
-    import torch
+    """The address of a contiguous int32 vector of n values; 0 of None."""
     if t is None:
-        return None
-    if t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous():
+        return 0
+    if t.dtype is _Torch.i32 and t.numel() == n and t.is_contiguous():
         return t.data_ptr()
     raise ValueError(what)
 
 
 def _rows(t, shape, what):
-    """(address, row stride) of a [rows][width] tensor of this shape whose rows are
-    contiguous; (None, 0) of None."""
+    """(address, row stride, C4S_DTYPE_*) of a [rows][width] tensor of this shape, bfloat16 or
+    float32, whose rows are contiguous; (0, 0, F32) of None."""
     if t is None:
-        return None, 0
-    if t.shape == shape:
+        return 0, 0, F32
+    kind = _Torch.kinds.get(t.dtype)
+    if kind is not None and t.shape == shape:
         ld, one = t.stride()
         if one == 1 or shape[1] <= 1:
-            return t.data_ptr(), (ld if shape[0] > 1 else shape[1])
+            return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), kind
     raise ValueError(what)
 
 
 def _heads(t, shape, what):
-    """(address, row stride) of a [rows][heads][dim] tensor of this shape whose rows are contiguous."""
-    if t.shape == shape:
+    """As _rows, of a [rows][heads][dim] tensor."""
+    kind = _Torch.kinds.get(t.dtype)
+    if kind is not None and t.shape == shape:
         ld, dim, one = t.stride()
         if one == 1 and (dim == shape[2] or shape[1] == 1):
-            return t.data_ptr(), (ld if shape[0] > 1 else shape[1] * shape[2])
+            return t.data_ptr(), (ld if shape[0] > 1 else shape[1] * shape[2]), kind
     raise ValueError(what)
 
 
@@ -327,7 +341,7 @@ class KvCache:
         self.desc = KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), _p(block_table),
                                 block_table.stride(0) if n_seqs > 1 else max_pages, n_seqs, max_pages, pages, size,
                                 heads, dim, KV_Q8 if q8 else KV_BF16)
-        self.ref = C.byref(self.desc)
+        self.packed = bytes(self.desc)
 
     @classmethod
     def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, q8=False):
@@ -345,6 +359,7 @@ class Context:
 
     def __init__(self, device: int = 0):
         self._h = _vp()
+        _Torch.load()
         rc = lib().c4s_create(device, C.byref(self._h))
         if rc != OK:
             raise C4SError(f"c4s_create(device={device}) failed with code {rc} "
@@ -486,10 +501,7 @@ class Context:
     # ---- the decoder layer's operators (include/c4s_layers.h) ---------------------------
     def _queue(self, stream):
         """The HIP stream of a call: the given one, or this device's current one."""
-        if stream is None:
-            import torch
-            return torch._C._cuda_getCurrentRawStream(self.device)
-        return _stream_handle(stream)
+        return _Torch.raw_stream(self.device) if stream is None else _stream_handle(stream)
 
     def block_norm(self, x, gamma, beta, out, y=None, x_out=None, post=False, post_gamma=None, post_beta=None,
                    gate=None, gate_rows=1, scale=1.0, eps=1e-5, rms=False, stream=None):
@@ -498,26 +510,26 @@ class Context:
         float32 [ceil(rows / gate_rows)][D]; without y, r = x."""
         shape = x.shape
         M, D = shape
-        xt = _dtype(x, "block_norm: x must be bfloat16 or float32")
-        yt = F32 if y is None else _dtype(y, "block_norm: y must be bfloat16 or float32")
-        ot = F32 if out is None else _dtype(out, "block_norm: out must be bfloat16 or float32")
-        if x_out is not None and x_out.dtype is not x.dtype:
-            raise ValueError("block_norm: x_out must have x's dtype")
-        g, ldg = None, 0
+        xp, ldx, xt = _rows(x, shape, "block_norm: x must be bfloat16 or float32, its rows contiguous")
+        yp, ldy, yt = _rows(y, shape, "block_norm: y must be bfloat16 or float32 of x's shape, its rows contiguous")
+        op, ldo, ot = _rows(out, shape, "block_norm: out must be bfloat16 or float32 of x's shape, its rows contiguous")
+        xo = ldxo = g = ldg = 0
+        if x_out is not None:
+            xo, ldxo, t = _rows(x_out, shape, "block_norm: x_out must have x's shape and dtype, its rows contiguous")
+            _need(t == xt, "block_norm: x_out must have x's dtype")
         if gate is not None:
-            if not (gate_rows >= 1 and gate.shape[0] * gate_rows >= M and _dtype(gate, "block_norm: gate must be float32") == F32):
-                raise ValueError("block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
-            g, ldg = _rows(gate, (gate.shape[0], D), "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
-        xp, ldx = _rows(x, shape, "block_norm: rows of x must be contiguous")
-        yp, ldy = _rows(y, shape, "block_norm: y must have x's shape, its rows contiguous")
-        xo, ldxo = _rows(x_out, shape, "block_norm: x_out must have x's shape, its rows contiguous")
-        op, ldo = _rows(out, shape, "block_norm: out must have x's shape, its rows contiguous")
-        d = Norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, xt, yt, yp, ldy, 1 if post else 0, gate_rows,
-                 _vector(post_gamma, D, "block_norm: post_gamma must be a float32 vector of D"),
-                 _vector(post_beta, D, "block_norm: post_beta must be a float32 vector of D"), g, ldg, scale, ot,
-                 _vector(gamma, D, "block_norm: gamma must be a float32 vector of D"),
-                 _vector(beta, D, "block_norm: beta must be a float32 vector of D"), xo, ldxo, op, ldo)
-        rc = lib().c4s_block_norm(self._h, C.byref(d), self._queue(stream))
+            g, ldg, t = _rows(gate, (gate.shape[0], D), "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+            _need(t == F32 and gate_rows >= 1 and gate.shape[0] * gate_rows >= M,
+                  "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+        if post_gamma is not None or post_beta is not None:
+            post_gamma = _vector(post_gamma, D, "block_norm: post_gamma must be a float32 vector of D")
+            post_beta = _vector(post_beta, D, "block_norm: post_beta must be a float32 vector of D")
+        rc = _lib.c4s_block_norm(
+            self._h, _pack_norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, xt, yt, yp, ldy, 1 if post else 0,
+                                gate_rows, post_gamma or 0, post_beta or 0, g, ldg, scale, ot,
+                                _vector(gamma, D, "block_norm: gamma must be a float32 vector of D"),
+                                _vector(beta, D, "block_norm: beta must be a float32 vector of D"), xo, ldxo, op, ldo),
+            _Torch.raw_stream(self.device) if stream is None else _stream_handle(stream))
         if rc:
             self._check(rc, "block_norm")
 
@@ -525,60 +537,59 @@ class Context:
         """out = residual + act(x @ weight^T + bias). x: bfloat16 [M][K]; weight:
         [N][K], bfloat16, or uint8 codes with quant=(scales, offsets, group);
         residual, out: [M][N], bfloat16 or float32; act: none, gelu, silu, relu."""
-        import torch
-        M, K = x.shape
-        N = weight.shape[0]
-        if not (x.dtype is torch.bfloat16 and weight.shape == (N, K) and weight.is_contiguous()):
+        xs, ws = x.shape, weight.shape
+        M, K = xs
+        N = ws[0]
+        xp, ldx, t = _rows(x, xs, "linear: x must be bfloat16 [M][K], its rows contiguous")
+        if not (t == BF16 and ws == (N, K) and weight.is_contiguous()):
             raise ValueError("linear: x must be bfloat16 [M][K], weight contiguous [N][K]")
-        ws = wb = None
-        wt, group = W_BF16, 0
+        sp = bp = group = 0
+        wt = W_BF16
         if quant is not None:
-            ws, wb, group = quant
+            scales, offsets, group = quant
             wt = W_Q8
-            if not (group > 0 and ws.dtype is torch.float32 and wb.dtype is torch.float32 and
-                    ws.shape == wb.shape == (N, K // group) and ws.is_contiguous() and wb.is_contiguous()):
+            if not (group > 0 and scales.shape == offsets.shape == (N, K // group)):
                 raise ValueError("linear: scales and offsets must be contiguous float32 [N][K / group]")
-            ws, wb = ws.data_ptr(), wb.data_ptr()
-        if weight.dtype is not (torch.bfloat16 if quant is None else torch.uint8):
+            sp = _vector(scales, N * (K // group), "linear: scales must be contiguous float32 [N][K / group]")
+            bp = _vector(offsets, N * (K // group), "linear: offsets must be contiguous float32 [N][K / group]")
+        if weight.dtype is not (_Torch.bf16 if quant is None else _Torch.u8):
             raise ValueError("linear: weights are bfloat16, or uint8 with quant=(scales, offsets, group)")
-        if act not in ACTS:
+        kind = ACTS.get(act)
+        if kind is None:
             raise ValueError("linear: act must be none, gelu, silu or relu")
-        xp, ldx = _rows(x, (M, K), "linear: rows of x must be contiguous")
-        op, ldo = _rows(out, (M, N), "linear: out must be [M][N], its rows contiguous")
-        rp, ldr = _rows(residual, (M, N), "linear: residual must be [M][N], its rows contiguous")
-        d = Linear(M, N, K, ACTS[act], xp, ldx, weight.data_ptr(), wt, group, ws, wb,
-                   _vector(bias, N, "linear: bias must be a float32 vector of N"), rp, ldr,
-                   F32 if residual is None else _dtype(residual, "linear: residual must be bfloat16 or float32"),
-                   _dtype(out, "linear: out must be bfloat16 or float32"), op, ldo)
-        rc = lib().c4s_linear(self._h, C.byref(d), self._queue(stream))
+        shape = (M, N)
+        op, ldo, ot = _rows(out, shape, "linear: out must be bfloat16 or float32 [M][N], its rows contiguous")
+        rp, ldr, rt = _rows(residual, shape, "linear: residual must be bfloat16 or float32 [M][N], its rows contiguous")
+        rc = _lib.c4s_linear(
+            self._h, _pack_linear(M, N, K, kind, xp, ldx, weight.data_ptr(), wt, group, sp, bp,
+                                  _vector(bias, N, "linear: bias must be a float32 vector of N"), rp, ldr, rt, ot, op, ldo),
+            _Torch.raw_stream(self.device) if stream is None else _stream_handle(stream))
         if rc:
             self._check(rc, "linear")
 
     @staticmethod
     def _kv_rows(cache, k, v, lens, rows_off):
-        shape = (k.shape[0], cache.n_kv_heads, cache.head_dim)
-        kp, ldk = _heads(k, shape, "kv rows: k must be [rows][n_kv_heads][head_dim], a row contiguous")
-        vp, ldv = _heads(v, shape, "kv rows: v must be [rows][n_kv_heads][head_dim], a row contiguous")
-        t = _dtype(k, "kv rows: k and v must be bfloat16 or float32")
-        if v.dtype is not k.dtype:
-            raise ValueError("kv rows: k and v must have one dtype")
-        return KvRows(kp, vp, ldk, ldv, _i32(lens, cache.n_seqs, "kv rows: lens must be an int32 vector of n_seqs"),
-                      _i32(rows_off, cache.n_seqs + 1, "kv rows: rows_off must be an int32 vector of n_seqs + 1"),
-                      shape[0], t)
+        shape = k.shape
+        rows, heads, dim = shape
+        _need(heads == cache.n_kv_heads and dim == cache.head_dim, "kv rows: k must be [rows][n_kv_heads][head_dim]")
+        kp, ldk, t = _heads(k, shape, "kv rows: k must be bfloat16 or float32, a row contiguous")
+        vp, ldv, vt = _heads(v, shape, "kv rows: v must have k's shape and dtype, a row contiguous")
+        _need(vt == t, "kv rows: k and v must have one dtype")
+        n = cache.n_seqs
+        return _pack_rows(kp, vp, ldk, ldv, _i32(lens, n, "kv rows: lens must be an int32 vector of n_seqs"),
+                          _i32(rows_off, n + 1, "kv rows: rows_off must be an int32 vector of n_seqs + 1"), rows, t)
 
     def kv_append(self, cache, k, v, lens, rows_off=None, stream=None):
         """The rows k, v (bfloat16 [rows][n_kv_heads][head_dim]) into the cache, as
         the last positions of lens[b]; rows_off as in include/c4s_layers.h."""
-        r = self._kv_rows(cache, k, v, lens, rows_off)
-        rc = lib().c4s_kv_append(self._h, cache.ref, C.byref(r), self._queue(stream))
+        rc = _lib.c4s_kv_append(self._h, cache.packed, self._kv_rows(cache, k, v, lens, rows_off), self._queue(stream))
         if rc:
             self._check(rc, "kv_append")
 
     def kv_read(self, cache, k, v, lens, rows_off=None, stream=None):
         """The cache's values at the last positions of lens[b] into the rows k, v
         (bfloat16 or float32)."""
-        r = self._kv_rows(cache, k, v, lens, rows_off)
-        rc = lib().c4s_kv_read(self._h, cache.ref, C.byref(r), self._queue(stream))
+        rc = _lib.c4s_kv_read(self._h, cache.packed, self._kv_rows(cache, k, v, lens, rows_off), self._queue(stream))
         if rc:
             self._check(rc, "kv_read")
 
@@ -586,23 +597,22 @@ class Context:
         """Attention of the rows q (bfloat16 [rows][n_heads][head_dim], the last
         positions of lens[b]) over the cache, into out. max_new: the most rows a
         sequence has (default: all rows); scale: 1 / sqrt(head_dim) by default."""
-        import torch
         shape = q.shape
         rows, heads, dim = shape
-        if not (q.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and dim == cache.head_dim):
-            raise ValueError("attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's")
-        if lse is not None and not (lse.dtype is torch.float32 and lse.shape == (rows, heads) and lse.is_contiguous()):
-            raise ValueError("attn: lse must be contiguous float32 [rows][n_heads]")
-        qp, ldq = _heads(q, shape, "attn: rows of q must be contiguous")
-        op, ldo = _heads(out, shape, "attn: out must have q's shape, its rows contiguous")
+        qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous")
+        op, ldo, ot = _heads(out, shape, "attn: out must be bfloat16 of q's shape, a row contiguous")
+        _need(qt == BF16 and ot == BF16 and dim == cache.head_dim,
+              "attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's")
         n = cache.n_seqs
-        d = Attn(qp, ldq, op, ldo, None if lse is None else lse.data_ptr(),
-                 _i32(lens, n, "attn: lens must be an int32 vector of n_seqs"),
-                 _i32(rows_off, n + 1, "attn: rows_off must be an int32 vector of n_seqs + 1"),
-                 _i32(first, n, "attn: first must be an int32 vector of n_seqs"), rows,
-                 rows if max_new is None or max_new > rows else max_new, heads,
-                 dim ** -0.5 if scale is None else scale)
-        rc = lib().c4s_attn(self._h, cache.ref, C.byref(d), self._queue(stream))
+        rc = _lib.c4s_attn(
+            self._h, cache.packed,
+            _pack_attn(qp, ldq, op, ldo, _vector(lse, rows * heads, "attn: lse must be contiguous float32 [rows][n_heads]"),
+                       _i32(lens, n, "attn: lens must be an int32 vector of n_seqs"),
+                       _i32(rows_off, n + 1, "attn: rows_off must be an int32 vector of n_seqs + 1"),
+                       _i32(first, n, "attn: first must be an int32 vector of n_seqs"), rows,
+                       rows if max_new is None or max_new > rows else max_new, heads,
+                       dim ** -0.5 if scale is None else scale),
+            self._queue(stream))
         if rc:
             self._check(rc, "attn")
 
