@@ -563,6 +563,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   // earlier block left here did that already to the rows it is for.)
   __shared__ int bad[Q8 ? 1 : DH];
   __shared__ int odd[2][W];   // whether a wave staged such values
+  __shared__ int gaps[W];     // whether a wave found a page of the segment missing
   const AttnArgs& a = f.a;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, c = lane % 16, g = lane / 16;
   const int dim = a.c.dim, pairs = a.c.n_heads * f.together, tile = f.tiles - 1 - blockIdx.x / pairs;
@@ -621,18 +622,22 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   }
 
   for (int i = tid; i < (Q8 ? 1 : DH); i += kThreads) bad[i] = INT32_MAX;
-  for (int seg = fst & ~(kSegment - 1); seg < kend; seg += kSegment) {
+  // (From fst < kend on, a segment's first block begins before its end: its table holds every block's pages.)
+  for (int seg = fst & ~(kSegment - 1); fst < kend && seg < kend; seg += kSegment) {
     const int begin = max(seg, fst & ~(kBlock - 1)), end = min(seg + kSegment, kend);
-    __syncthreads();
-    for (int i = tid; i < kSegment >> shift; i += kThreads) {
+    if (seg > fst) __syncthreads();   // the segment before has been read
+    bool missing = false;             // whether a page of the segment is not there
+    for (int i = tid; i < (((end - seg + kBlock - 1) & ~(kBlock - 1)) + ps - 1) >> shift; i += kThreads) {   // through the last block
       const int at = (seg >> shift) + i;
       const int p = at < a.c.max_pages ? table[at] : -1;
       pages[i] = p < a.c.n_pages ? p : -1;
+      missing |= (p < 0 || p >= a.c.n_pages) && (i + 1) * ps + seg > fst && i * ps + seg < end;
     }
+    missing = __any(missing);
+    if (lane == 0) gaps[wave] = missing;
     __syncthreads();
-    bool missing = false;   // whether a page of the segment is not there
-    for (int i = tid; i < (end - seg + ps - 1) >> shift; i += kThreads) missing |= pages[i] < 0 && (i + 1) * ps + seg > fst;
-    missing = __syncthreads_or(missing);
+#pragma unroll
+    for (int w = 0; w < W; ++w) missing |= gaps[w] != 0;
     uint4 kst[kLoads], vst[kLoads];
     float sst = 0.0f;
     // A thread's pieces of a block: of the keys in order; of the values in the order in which a page has them.
@@ -666,12 +671,13 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
         }
       }
     };
+    auto edge_of = [&](int t) { return t < fst || t + kBlock > first_lim || missing; };
     auto stage = [&](int t, int buf) {
       char* kl = lds[buf];
       char* vl = kl + kBlock * DH * 2;
       // What is not there or not for any row may hold anything: zeros (codes: their scales).
       int strange = 0;
-      const bool edge = t < fst || t + kBlock > first_lim || missing;
+      const bool edge = edge_of(t);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         if (kStagers < kThreads && tid >= kStagers) break;
@@ -763,6 +769,14 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = j < from ? -__builtin_inff() : s[b][j / 4][j % 4];
       }
+      auto value = [&](int d, int st) { return *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st)); };
+      constexpr bool kAhead = DH == 64;   // two dim tiles' values asked for before the weights, the others' before the products
+      uint4 va[kAhead ? 4 : 1];
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) va[i] = value(i / 2, i % 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       uint32_t p[NB][8];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -792,19 +806,42 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
         }
       }
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
+      if constexpr (kAhead) {
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) {
-        if (DH != 64 && 16 * d >= dim) break;
+        for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(l[b]));   // summed here: the weights' registers are free for values
+        uint4 vb[4];
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st));
+        for (int i = 0; i < 4; ++i) vb[i] = value(2 + i / 2, i % 2);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int b = 0; b < NB; ++b) o[b][d] = mfma(v, quad(p[b] + 4 * st), o[b][d]);
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b][d] = mfma(va[2 * d + st], quad(p[b] + 4 * st), o[b][d]);
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b][2 + d] = mfma(vb[2 * d + st], quad(p[b] + 4 * st), o[b][2 + d]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          if (16 * d >= dim) break;
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st));
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b][d] = mfma(v, quad(p[b] + 4 * st), o[b][d]);
+          }
         }
       }
       int strange = 0;
+      if (!kAhead || edge_of(t)) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) strange |= odd[buf][w];
+        for (int w = 0; w < W; ++w) strange |= odd[buf][w];
+      }
       if (strange) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
