@@ -573,6 +573,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   const int n_all = sq.n_new * a.shared, r0 = tile * 16 * NB * W;
   if (r0 >= n_all) return;
   const int fst = sq.fst, shift = a.c.page_shift, ps = 1 << shift;
+  auto token_of = [&](int r) { return a.shared == 1 ? r : r / a.shared; };
   // This wave's rows; a lane has row 16 b + c of each block b.
   const int w0 = r0 + 16 * NB * wave;
   const bool any_rows = w0 < n_all;
@@ -581,18 +582,18 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   uint16_t* op[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int r = min(w0 + 16 * b + c, n_all - 1), token = r / a.shared, qh = head * a.shared + r % a.shared;
+    const int r = min(w0 + 16 * b + c, n_all - 1), token = token_of(r), qh = head * a.shared + r - token * a.shared;
     lim[b] = min(sq.past + token + 1, sq.cap);
     qp[b] = a.q + (int64_t)(sq.row0 + token) * a.ldq + qh * dim;
     op[b] = a.out + (int64_t)(sq.row0 + token) * a.ld_out + qh * dim;
   }
   if (any_rows) {
-    least = min(sq.past + w0 / a.shared + 1, sq.cap);
-    most = min(sq.past + min(w0 + 16 * NB - 1, n_all - 1) / a.shared + 1, sq.cap);
+    least = min(sq.past + token_of(w0) + 1, sq.cap);
+    most = min(sq.past + token_of(min(w0 + 16 * NB - 1, n_all - 1)) + 1, sq.cap);
   }
-  const int kend = min(sq.past + min(r0 + 16 * NB * W - 1, n_all - 1) / a.shared + 1, sq.cap);   // the workgroup's last
+  const int kend = min(sq.past + token_of(min(r0 + 16 * NB * W - 1, n_all - 1)) + 1, sq.cap);   // the workgroup's last
 
-  const int first_lim = min(sq.past + r0 / a.shared + 1, sq.cap);                              // ... and its first
+  const int first_lim = min(sq.past + token_of(r0) + 1, sq.cap);                              // ... and its first
 
   // Scores become powers of two's exponents by one multiplication with a positive factor: a negative scale
   // turns q's signs, and none at all is so small that the weights are equal.
@@ -866,7 +867,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
       *reinterpret_cast<uint2*>(op[b] + 16 * d + 4 * g) = make_uint2(pack(v[0], v[1]), pack(v[2], v[3]));
     }
     if (a.lse && g == 0)
-      a.lse[(int64_t)(sq.row0 + r / a.shared) * a.n_heads + head * a.shared + r % a.shared] = sum == 0.0f ? -__builtin_inff() : (m[b] + log2f(sum)) * kLn2;
+      a.lse[(int64_t)(sq.row0 + token_of(r)) * a.n_heads + head * a.shared + r - token_of(r) * a.shared] = sum == 0.0f ? -__builtin_inff() : (m[b] + log2f(sum)) * kLn2;
   }
 }
 
