@@ -172,10 +172,11 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   if (r0 >= n_all) return;
   const int valid = min(kRows, n_all - r0);
   const int r = r0 + min(c, valid - 1);
-  const int token = r / a.shared, qh = head * a.shared + r % a.shared;
+  auto token_of = [&](int r) { return a.shared == 1 ? r : r / a.shared; };
+  const int token = token_of(r), qh = head * a.shared + r - token * a.shared;
   const int lim = min(sq.past + token + 1, sq.cap);                            // this row sees positions before it
-  const int least = min(sq.past + r0 / a.shared + 1, sq.cap);                  // ... the tile's first row
-  const int kend = min(sq.past + (r0 + valid - 1) / a.shared + 1, sq.cap);     // ... its last
+  const int least = min(sq.past + token_of(r0) + 1, sq.cap);                  // ... the tile's first row
+  const int kend = min(sq.past + token_of(r0 + valid - 1) + 1, sq.cap);     // ... its last
   const int fst = sq.fst;
   const int first_chunk = fst / f.chunk, parts = kend > fst ? (kend - 1) / f.chunk + 1 - first_chunk : 1;
   if (split >= parts) return;
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   float* mine = f.part + (group * f.splits + split) * words * 4;
   auto finish = [&](int row, int i, f32x4 v, float top, float sum) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int rr = r0 + row, tok = sq.row0 + rr / a.shared, hh = head * a.shared + rr % a.shared;
+    const int rr = r0 + row, tk = token_of(rr), tok = sq.row0 + tk, hh = head * a.shared + rr - tk * a.shared;
     *reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.ld_out + hh * dim + 4 * i) = make_uint2(pack(v[0] * inv, v[1] * inv), pack(v[2] * inv, v[3] * inv));
     if (a.lse && i == 0) a.lse[(int64_t)tok * a.n_heads + hh] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * kLn2;
   };
