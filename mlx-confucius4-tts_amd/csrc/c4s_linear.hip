@@ -604,13 +604,20 @@ int64_t tiles_of(const c4s_linear_desc& a, int m, int n) {
 }
 
 // Which kernel. Few rows' tiles (32 outputs by 64 rows) cost about alike, and
-// from 1280 of them on the others win (us, bf16, K = 1280, N = 5120: 512 rows 21
-// and 25, 1024 rows 36 and 27; K = 5120, N = 1280: 2000 rows 61 and 62; 8-bit,
-// N = 5120: 512 rows 29 and 42, 800 rows 44 and 46). 256 x 256 wins where
-// 128 x 128 takes more than one round of two a CU (2048 rows of 5120 x 1280, 640
-// tiles: 45 and 48 us; 1024 rows, 320 tiles: 44 and 27).
+// from 1280 of them on the others win (us, bf16, K = 1280, N = 5120: 512 rows 19
+// and 21, 640 rows 23 and 21, 1024 rows 31 and 24; K = 5120, N = 1280: 2000 rows 59
+// and 59; 8-bit, N = 5120: 512 rows 31 and 39, 800 rows 46 and 45).
 bool few_pays(const c4s_linear_desc& a) {
   return tiles_of(a, kFewM, kFewN) <= (a.wdtype == C4S_W_Q8 ? 1600 : 1280);
+}
+
+// 128 x 128, two workgroups a CU, or 256 x 256: a round of the chip with the former
+// takes 9/16 of one with the latter, which does twice the work (128 / 256, us: 1600 x
+// 5120 x 1280, 2 and 1 rounds, 43 / 40; 4096, 3 and 2, 67 / 78; 5000, 4 and 2, 88 / 78;
+// 7000, 5 and 3, 111 / 117; 12345, 8 and 4, 188 / 160; 4000 x 1280 x 1280, one, 24 / 39).
+bool small_tiles_pay(const c4s_linear_desc& a) {
+  const int64_t small = (tiles_of(a, 128, 128) + 511) / 512, large = (tiles_of(a, 256, 256) + 255) / 256;
+  return 9 * small <= 16 * large;
 }
 
 }  // namespace
@@ -633,7 +640,7 @@ hipError_t launch_linear(const c4s_linear_desc& a, uint32_t* counters, float* sp
   if (a.wdtype == C4S_W_Q8) {
     const ManyArgs f = many_args<4, 4, 2, 2>(a);
     hipLaunchKernelGGL(k_linear_many_q8, many_grid(f), dim3(256), 0, s, f);
-  } else if (tiles_of(a, 128, 128) <= 512) {
+  } else if (small_tiles_pay(a)) {
     const ManyArgs f = many_args<4, 4, 2, 2>(a);
     hipLaunchKernelGGL((k_linear_many<4, 4, 2, 2>), many_grid(f), dim3(256), 0, s, f);
   } else {
