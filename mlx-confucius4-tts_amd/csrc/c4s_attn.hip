@@ -23,6 +23,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -80,8 +81,10 @@ __device__ __forceinline__ uint4 keep(uint4 w, int at, int lo, int hi) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ int odd_exp(uint32_t w) {   // either half inf or NaN
-  return (int)((w & 0x7F80u) == 0x7F80u) | (int)((w & 0x7F800000u) == 0x7F800000u);
+__device__ __forceinline__ bool any_odd(uint4 w) {   // one of eight inf or NaN: the largest exponent there is
+  auto e = [](uint32_t v) { return __builtin_bit_cast(u16x2, v & 0x7F807F80u); };
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(e(w.x), e(w.y)), __builtin_elementwise_max(e(w.z), e(w.w)));
+  return max(m[0], m[1]) == 0x7F80u;
 }
 
 // The finite halves of w, and ones where the others were.
@@ -335,7 +338,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
 #pragma unroll
           for (int i = 0; i < kVLoads; ++i) {
             vr[i] = keep(vr[i], 8 * (i % (KEYS / 32)), from, to);
-            odd |= odd_exp(vr[i].x) | odd_exp(vr[i].y) | odd_exp(vr[i].z) | odd_exp(vr[i].w);
+            odd |= any_odd(vr[i]);
           }
           if (least != kend && __any(odd)) {
 #pragma unroll
@@ -693,9 +696,9 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
           *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP)) = kst[i];
           if (edge) {
             const int pos = t + 8 * piece;
-            const bool there = pages[(pos - seg) >> shift] >= 0;
-            vst[i] = keep(vst[i], 0, fst - pos, there ? kend - pos : 0);
-            if (odd_exp(vst[i].x) | odd_exp(vst[i].y) | odd_exp(vst[i].z) | odd_exp(vst[i].w)) {
+            if (t < fst || t + kBlock > kend || missing)
+              vst[i] = keep(vst[i], 0, fst - pos, pages[(pos - seg) >> shift] >= 0 ? kend - pos : 0);
+            if (any_odd(vst[i])) {
               strange = 1;
               uint32_t w[4] = {vst[i].x, vst[i].y, vst[i].z, vst[i].w}, was;
 #pragma unroll
