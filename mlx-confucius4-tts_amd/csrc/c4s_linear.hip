@@ -21,7 +21,9 @@ namespace c4s {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 Quad __attribute__((ext_vector_type(4)));   // rounds to nearest even
+typedef __bf16 Quad __attribute__((ext_vector_type(4)));   // these round to nearest even
+typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+typedef uint32_t Eight __attribute__((ext_vector_type(4), aligned(8)));   // eight bf16
 
 __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -85,35 +87,11 @@ __device__ __forceinline__ void activate(float (&y)[N], int act) {
   }
 }
 
-template <bool PAST, class V>
-__device__ __forceinline__ void put(V* p, V v) {
-  if (PAST) __builtin_nontemporal_store(v, p);
-  else *p = v;
-}
-
-// Activation, residual and store of four outputs n .. n + 3 of row m, with the bias
-// in y. PAST: the store goes past the caches, which keeps the operands of many rows'
-// tiles in them (12345 x 5120 x 1280: 180 us, and 170 so).
-template <bool PAST = false>
-__device__ __forceinline__ void finish4(const c4s_linear_desc& a, int m, int n, f32x4 y) {
-  f32x4 r = {};
-  const int64_t ro = (int64_t)m * a.ld_res + n, o = (int64_t)m * a.ld_out + n;
-  if (a.residual) {
-    if (a.res_dtype == C4S_DTYPE_BF16) {
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.residual) + ro);
-      r = f32x4{from_bf16(w.x & 0xFFFFu), from_bf16(w.x >> 16), from_bf16(w.y & 0xFFFFu), from_bf16(w.y >> 16)};
-    } else {
-      r = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + ro);
-    }
-  }
-  float v[4] = {y[0], y[1], y[2], y[3]};
-  activate(v, a.act);
-  y = f32x4{v[0], v[1], v[2], v[3]};
-  if (a.residual) y += r;
-  if (a.out_dtype == C4S_DTYPE_BF16)
-    put<PAST>(reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + o), __builtin_bit_cast(u32x2, Quad{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]}));
-  else
-    put<PAST>(reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + o), y);
+// Four values of the residual, from element o on.
+__device__ __forceinline__ f32x4 residual4(const c4s_linear_desc& a, int64_t o) {
+  if (a.res_dtype != C4S_DTYPE_BF16) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.residual) + o);
+  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.residual) + o);
+  return f32x4{from_bf16(w.x & 0xFFFFu), from_bf16(w.x >> 16), from_bf16(w.y & 0xFFFFu), from_bf16(w.y >> 16)};
 }
 
 // Four consecutive outputs n .. n + 3 of row m: bias, activation, residual, store.
@@ -136,7 +114,15 @@ __device__ __forceinline__ void finish(const c4s_linear_desc& a, bool vec, int m
   if (n >= a.N) return;
   f32x4 b = {};
   if (a.bias) b = *reinterpret_cast<const f32x4*>(a.bias + n);
-  finish4(a, m, n, y + b);
+  float v[4] = {y[0] + b[0], y[1] + b[1], y[2] + b[2], y[3] + b[3]};
+  activate(v, a.act);
+  y = f32x4{v[0], v[1], v[2], v[3]};
+  if (a.residual) y += residual4(a, (int64_t)m * a.ld_res + n);
+  const int64_t o = (int64_t)m * a.ld_out + n;
+  if (a.out_dtype == C4S_DTYPE_BF16)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) = __builtin_bit_cast(uint2, Quad{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]});
+  else
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + o) = y;
 }
 
 // Whether finish() may use vectors.
@@ -387,36 +373,92 @@ __device__ __forceinline__ bool tile_of(const ManyArgs& f, int& n, int& m) {
   return true;
 }
 
-// A wave's NW x MW fragments from (m, n) on, sixteen rows at a time through its
-// own part of LDS (16 (16 NW + 4) floats), so that rows are loaded and stored in
-// runs of 16 NW outputs. Every wave is done with LDS.
-template <int NW, int MW>
-__device__ __forceinline__ void write_tile(const ManyArgs& f, char* lds, int wave, int m, int n, const f32x4 (&acc)[NW][MW]) {
-  constexpr int kPitch = 16 * NW + 4, kQuads = 4 * NW;
+// Quad i of lane group g becomes quad g of lane group i (of the four groups of 16
+// lanes; T two or four dwords a quad).
+template <int T>
+__device__ __forceinline__ void swap_groups(uint32_t (&q)[4][T]) {
+#pragma unroll
+  for (int e = 0; e < T; ++e) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto r = __builtin_amdgcn_permlane32_swap(q[i][e], q[i + 2][e], false, false);
+      q[i][e] = r[0];
+      q[i + 2][e] = r[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const auto r = __builtin_amdgcn_permlane16_swap(q[i][e], q[i + 1][e], false, false);
+      q[i][e] = r[0];
+      q[i + 1][e] = r[1];
+    }
+  }
+}
+
+// A wave's 4 x MW fragments from (m, n) on: lane (g, c) has outputs n + 16 i + 4 g ..
+// + 3 of rows m + 16 j + c. Bias, activation and residual are applied as they lie;
+// results in bf16 change lanes so that each stores 16 outputs next to each other.
+// Stores go past the caches, which keeps the operands of the tiles in them (12345 x
+// 5120 x 1280: 180 us, and 170 so).
+template <int MW>
+__device__ __forceinline__ void write_tile(const ManyArgs& f, int m, int n, const f32x4 (&acc)[4][MW]) {
+  const c4s_linear_desc& a = f.d;
   const int lane = threadIdx.x % 64, c = lane % 16, g = lane / 16;
-  static_assert(64 % kQuads == 0, "a lane keeps its outputs");
-  float* red = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
-  const int at = 4 * (lane % kQuads);
-  f32x4 b = {};
-  if (f.vec && f.d.bias && n + at < f.d.N) b = *reinterpret_cast<const f32x4*>(f.d.bias + n + at);
-  __syncthreads();
+  if (!f.vec) {
+#pragma unroll
+    for (int j = 0; j < MW; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (m + 16 * j + c < a.M) finish(a, false, m + 16 * j + c, n + 16 * i + 4 * g, acc[i][j]);
+    return;
+  }
+  f32x4 b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = n + 16 * i + 4 * g;
+    b[i] = a.bias && at < a.N ? *reinterpret_cast<const f32x4*>(a.bias + at) : f32x4{};
+  }
 #pragma unroll
   for (int j = 0; j < MW; ++j) {
+    const int row = m + 16 * j + c;
+    const bool in = row < a.M;
+    f32x4 r[4] = {};
+    if (a.residual && in) {
+      const int64_t o = (int64_t)row * a.ld_res + n + 4 * g;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) *reinterpret_cast<f32x4*>(red + c * kPitch + 16 * i + 4 * g) = acc[i][j];
-    if (f.vec) {
-      if (n + at >= f.d.N) continue;
+      for (int i = 0; i < 4; ++i)
+        if (n + 16 * i + 4 * g < a.N) r[i] = residual4(a, o + 16 * i);
+    }
+    float y[16];
 #pragma unroll
-      for (int q = lane; q < 16 * kQuads; q += 64) {
-        const int row = m + 16 * j + q / kQuads;
-        if (row < f.d.M) finish4<true>(f.d, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at) + b);
+    for (int i = 0; i < 16; ++i) y[i] = acc[i / 4][j][i % 4] + b[i / 4][i % 4];
+    activate(y, a.act);
+    if (a.residual) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] += r[i / 4][i % 4];
+    }
+    if (a.out_dtype == C4S_DTYPE_BF16) {
+      uint32_t q[4][2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i / 2][i % 2] = __builtin_bit_cast(uint32_t, Pair{(__bf16)y[2 * i], (__bf16)y[2 * i + 1]});
+      swap_groups(q);
+      uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)row * a.ld_out + n + 16 * g;
+      if (in) {
+        if (n + 16 * g + 16 <= a.N) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            __builtin_nontemporal_store(Eight{q[2 * i][0], q[2 * i][1], q[2 * i + 1][0], q[2 * i + 1][1]}, reinterpret_cast<Eight*>(o + 8 * i));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + 16 * g + 4 * i < a.N) __builtin_nontemporal_store(u32x2{q[i][0], q[i][1]}, reinterpret_cast<u32x2*>(o + 4 * i));
+        }
       }
-    } else {
-#pragma unroll 1
-      for (int q = lane; q < 16 * kQuads; q += 64) {
-        const int row = m + 16 * j + q / kQuads;
-        if (row < f.d.M) finish(f.d, false, row, n + at, *reinterpret_cast<const f32x4*>(red + q / kQuads * kPitch + at));
-      }
+    } else if (in) {
+      float* o = static_cast<float*>(a.out) + (int64_t)row * a.ld_out + n + 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + 16 * i + 4 * g < a.N)
+          __builtin_nontemporal_store(f32x4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]}, reinterpret_cast<f32x4*>(o + 16 * i));
     }
   }
 }
@@ -433,7 +475,6 @@ template <int NW, int MW, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM, WN * WM == 8 ? 1 : 2) void k_linear_many(ManyArgs f) {
   constexpr int kN = 16 * NW * WN, kM = 16 * MW * WM, kWaves = WN * WM, kStage = (kN + kM) * 128;
   constexpr int kLoads = (kN + kM) / 8 / kWaves;   // a wave's of a stage
-  static_assert(2 * kStage >= kWaves * 16 * (16 * NW + 4) * 4, "the waves' rows in LDS");
   __shared__ __align__(128) char lds[2 * kStage];
   const c4s_linear_desc& a = f.d;
   const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64), c = lane % 16, g = lane / 16;
@@ -494,7 +535,7 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM == 8 ? 1 : 2) void k_linear_m
     mul(fb);
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing on its way into LDS any more
-  write_tile<NW, MW>(f, lds, wave, m0 + wm, n0 + wn, acc);
+  write_tile(f, m0 + wm, n0 + wn, acc);
 }
 
 // 8-bit codes: 128 x 128, four waves, two workgroups a CU. The codes pass through
@@ -589,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void k_linear_many_q8(ManyArgs f) {
       for (int j = 0; j < MW; ++j) sum[j] = f32x4{};
     }
   }
-  write_tile<NW, MW>(f, xs, wave, m0 + wm, n0 + wn, acc);
+  write_tile(f, m0 + wm, n0 + wn, acc);
 }
 
 template <int NW, int MW, int WN, int WM>
