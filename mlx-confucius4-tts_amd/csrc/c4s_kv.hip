@@ -84,27 +84,21 @@ struct Tile {
   int n_lead, n_single;
 
   __device__ __forceinline__ void find(const KvArgs& c, const KvRowsArgs& rows) {
-    if (threadIdx.x < TILE) at[threadIdx.x] = place_of(c, rows.lens, rows.off, rows.n_rows, blockIdx.x / c.n_heads * TILE + threadIdx.x);
-    __syncthreads();
     if (threadIdx.x < 64) {   // one wave: a lane a row
       const int r = threadIdx.x;
-      const bool row = r < TILE && at[r].page >= 0;
-      auto leads = [&](int g) {
-        if (g < 0 || g + 4 > TILE || at[g].page < 0 || (at[g].at & 3)) return false;
-        bool all = true;
-#pragma unroll
-        for (int j = 1; j < 4; ++j) all = all && at[g + j].page == at[g].page && at[g + j].at == at[g].at + j;
-        return all;
-      };
-      const bool is_lead = row && leads(r);
-      bool in_group = false;
-      if (row) {
-        const int g = r - (at[r].at & 3);
-        in_group = leads(g) && at[g].page == at[r].page && at[g].at == (at[r].at & ~3);
+      Place p{-1, 0};
+      if (r < TILE) {
+        p = place_of(c, rows.lens, rows.off, rows.n_rows, blockIdx.x / c.n_heads * TILE + r);
+        at[r] = p;
       }
-      const uint64_t lm = __ballot(is_lead), sm = __ballot(row && !in_group), below = (1ull << r) - 1;
-      if (is_lead) lead[__popcll(lm & below)] = (uint8_t)r;
-      if (row && !in_group) single[__popcll(sm & below)] = (uint8_t)r;
+      const int page = (int)p.page;
+      const bool row = page >= 0;
+      // rows whose next one follows them in their page; four in line from a multiple of four on go together
+      const uint64_t next = __ballot(row & (__shfl_down(page, 1) == page) & (__shfl_down(p.at, 1) == p.at + 1));
+      const uint64_t lm = __ballot(row & !(p.at & 3)) & next & next >> 1 & next >> 2;
+      const uint64_t sm = __ballot(row) & ~(lm | lm << 1 | lm << 2 | lm << 3), below = (1ull << r) - 1;
+      if (lm >> r & 1) lead[__popcll(lm & below)] = (uint8_t)r;
+      if (sm >> r & 1) single[__popcll(sm & below)] = (uint8_t)r;
       if (r == 0) {
         n_lead = __popcll(lm);
         n_single = __popcll(sm);
