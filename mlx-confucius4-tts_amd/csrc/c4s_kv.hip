@@ -136,7 +136,7 @@ struct Values {
   // To (TO_PAGES) or from the pages' rows of positions; v0: where a place's position
   // of dim 0 lies. Then words of four dims (Q8) or two for four positions at once.
   template <bool TO_PAGES, class V0>
-  __device__ __forceinline__ void move(const Tile<TILE>& tile, int dim, int ps, V0 v0) {
+  __device__ __forceinline__ void move(const Tile<TILE>& tile, int dim, int shift, V0 v0) {
     if ((int)threadIdx.x % kGroups < tile.n_lead) {
       const int g = tile.lead[threadIdx.x % kGroups];
       uint8_t* at = v0(tile.at[g]);
@@ -148,19 +148,19 @@ struct Values {
           for (int j = 0; j < 4; ++j) x[j] = words[g + j][w];
         }
         if (Q8) {
-          uint8_t* p = at + (int64_t)(4 * w) * ps;
+          uint8_t* p = at + ((uint32_t)(4 * w) << shift);
           if (!TO_PAGES) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint32_t*>(p + (int64_t)j * ps);
+            for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint32_t*>(p + ((uint32_t)j << shift));
           }
           transpose_bytes(x);
           if (TO_PAGES) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(p + (int64_t)j * ps) = x[j];
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(p + ((uint32_t)j << shift)) = x[j];
           }
         } else {
-          uint2* p0 = reinterpret_cast<uint2*>(at + (int64_t)(2 * w) * ps * 2);
-          uint2* p1 = reinterpret_cast<uint2*>(at + (int64_t)(2 * w + 1) * ps * 2);
+          uint2* p0 = reinterpret_cast<uint2*>(at + ((uint32_t)(4 * w) << shift));
+          uint2* p1 = reinterpret_cast<uint2*>(at + ((uint32_t)(4 * w + 2) << shift));
           if (TO_PAGES) {
             swap_halves(x[0], x[1]);
             swap_halves(x[2], x[3]);
@@ -186,8 +186,8 @@ struct Values {
       T* mine = reinterpret_cast<T*>(words[g]);
 #pragma unroll 4
       for (int d = threadIdx.x / TILE; d < dim; d += kThreads / TILE) {
-        if (TO_PAGES) at[(int64_t)d * ps] = mine[d];
-        else mine[d] = at[(int64_t)d * ps];
+        if (TO_PAGES) at[(uint32_t)d << shift] = mine[d];
+        else mine[d] = at[(uint32_t)d << shift];
       }
     }
   }
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs 
     }
   }
   __syncthreads();
-  values.template move<true>(tile, dim, ps, [&](const Place& q) {
+  values.template move<true>(tile, dim, c.page_shift, [&](const Place& q) {
     return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * dim + q.at) * (Q8 ? 1 : 2);
   });
 }
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
       raw[0][i] = *reinterpret_cast<const Piece*>(static_cast<const uint16_t*>(c.k) + slot * dim + d);
     }
   }
-  values.template move<false>(tile, dim, ps, [&](const Place& q) {
+  values.template move<false>(tile, dim, c.page_shift, [&](const Place& q) {
     return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * dim + q.at) * (Q8 ? 1 : 2);
   });
   // a row between two sequences' rows, or behind the last, is not the call's to write
