@@ -523,7 +523,7 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
 // wave's last row are skipped by it, masks are applied only where a block
 // holds the limit of some row, and the tiles with the most positions start
 // first, those of up to 64 sequences together (of one after the other: 8 of 2048,
-// 20 heads of 64, 184 us for 171; 4 of 2000, 5 heads of 256 222 for 197).
+// 20 heads of 64, 169 us for 152; 4 of 2000, 5 heads of 256 195 for 172).
 //
 // Weights enter the second product rounded to bf16 once: independent roundings
 // of 2^-9 at most, which add a quarter to the error of the output's own

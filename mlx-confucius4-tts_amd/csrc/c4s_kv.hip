@@ -11,7 +11,7 @@
 // are then read and written next to each other in time.
 //
 // Memory bounds both for prompts, reads nearly (24 prompts of 70 to 1500 tokens, 20
-// heads of 64, 8-bit: 224 MB out in 42 us, 5.4 TB/s), writes less so (151 MB in 54 us:
+// heads of 64, 8-bit: 224 MB in 41 us, 5.5 TB/s), writes less so (151 MB in 52 us:
 // the pages' rows that a tile's ends leave half full, and about half the time in
 // which the codes are computed, add to it).
 
@@ -198,8 +198,8 @@ struct Values {
 // A code is value / scale to nearest even. One correction of the product with the
 // rounded reciprocal gives the rounded quotient (Markstein 1990) where nothing
 // leaves the range; adding 1.5 * 2^23 then leaves the integer to nearest even in
-// the sum's low bits. (With divisions the prompts above take 59 us for 54, a
-// step's 64 rows 5.1 for 4.4.)
+// the sum's low bits. (With divisions the prompts above take 58 us for 52, a
+// step's 64 rows 4.8 for 4.1.)
 template <bool Q8, int PIECES, int TILE>
 __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs rows) {
   __shared__ Tile<TILE> tile;
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
       for (int j = 0; j < 8; ++j)
         v[j] = Q8 ? (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale[which]
                   : __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-      // past the caches, which keeps the pages in them (42 us for 52)
+      // past the caches, which keeps the pages in them (41 us for 52)
       if (rows.f32) {
         typedef float Quad __attribute__((ext_vector_type(4)));
         Quad* q = reinterpret_cast<Quad*>(static_cast<float*>(out) + o + d);
@@ -348,8 +348,8 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
 }
 
 // Tiles of 64 rows once there is one for every compute unit (24 prompts as above:
-// written in 54 us, in tiles of 16 in 59), else of 16 (64 single tokens: written in
-// 4.4 us, in tiles of 64 in 6.7). `launch` gets the store, the pieces of a lane and the tile's rows.
+// written in 52 us, in tiles of 16 in 57), else of 16 (64 single tokens: written in
+// 4.1 us, in tiles of 64 in 6.5). `launch` gets the store, the pieces of a lane and the tile's rows.
 template <class Launch>
 hipError_t by_kind(const KvArgs& c, const KvRowsArgs& r, Launch launch) {
   auto tile = [&](auto q8, auto pieces) {

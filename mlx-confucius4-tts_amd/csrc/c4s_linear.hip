@@ -398,7 +398,7 @@ __device__ __forceinline__ void swap_groups(uint32_t (&q)[4][T]) {
 // + 3 of rows m + 16 j + c. Bias, activation and residual are applied as they lie;
 // results in bf16 change lanes so that each stores 16 outputs next to each other.
 // Stores go past the caches, which keeps the operands of the tiles in them (12345 x
-// 5120 x 1280: 180 us, and 170 so).
+// 5120 x 1280, gelu: 170 us, and 166 so; through LDS, a quad a lane: 170).
 template <int MW>
 __device__ __forceinline__ void write_tile(const ManyArgs& f, int m, int n, const f32x4 (&acc)[4][MW]) {
   const c4s_linear_desc& a = f.d;
