@@ -373,30 +373,24 @@ __device__ __forceinline__ bool tile_of(const ManyArgs& f, int& n, int& m) {
   return true;
 }
 
-// Quad i of lane group g becomes quad g of lane group i (of the four groups of 16
-// lanes; T two or four dwords a quad).
-template <int T>
-__device__ __forceinline__ void swap_groups(uint32_t (&q)[4][T]) {
+// Of the quads that lane group g (of the four of 16 lanes) has, q[i] number 4 i + g
+// of a row, to q[2 s + e] number 8 s + 2 g + e: two pairs of quads next to each other.
+__device__ __forceinline__ void swap_groups(uint32_t (&q)[4][2]) {
 #pragma unroll
-  for (int e = 0; e < T; ++e) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const auto r = __builtin_amdgcn_permlane32_swap(q[i][e], q[i + 2][e], false, false);
-      q[i][e] = r[0];
-      q[i + 2][e] = r[1];
-    }
+  for (int e = 0; e < 2; ++e)
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      const auto r = __builtin_amdgcn_permlane16_swap(q[i][e], q[i + 1][e], false, false);
-      q[i][e] = r[0];
-      q[i + 1][e] = r[1];
+      const auto r = __builtin_amdgcn_permlane32_swap(q[i][e], q[i + 1][e], false, false);
+      const auto t = __builtin_amdgcn_permlane16_swap(r[0], r[1], false, false);
+      q[i][e] = t[0];
+      q[i + 1][e] = t[1];
     }
-  }
 }
 
 // A wave's 4 x MW fragments from (m, n) on: lane (g, c) has outputs n + 16 i + 4 g ..
 // + 3 of rows m + 16 j + c. Bias, activation and residual are applied as they lie;
-// results in bf16 change lanes so that each stores 16 outputs next to each other.
+// results in bf16 change lanes so that a store is of 32 outputs of a row next to each
+// other.
 // Stores go past the caches, which keeps the operands of the tiles in them (12345 x
 // 5120 x 1280, gelu: 170 us, and 166 so; through LDS, a quad a lane: 170).
 template <int MW>
@@ -441,17 +435,12 @@ __device__ __forceinline__ void write_tile(const ManyArgs& f, int m, int n, cons
 #pragma unroll
       for (int i = 0; i < 8; ++i) q[i / 2][i % 2] = __builtin_bit_cast(uint32_t, Pair{(__bf16)y[2 * i], (__bf16)y[2 * i + 1]});
       swap_groups(q);
-      uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)row * a.ld_out + n + 16 * g;
-      if (in) {
-        if (n + 16 * g + 16 <= a.N) {
+      uint16_t* o = static_cast<uint16_t*>(a.out) + (int64_t)row * a.ld_out + n + 8 * g;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            __builtin_nontemporal_store(Eight{q[2 * i][0], q[2 * i][1], q[2 * i + 1][0], q[2 * i + 1][1]}, reinterpret_cast<Eight*>(o + 8 * i));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + 16 * g + 4 * i < a.N) __builtin_nontemporal_store(u32x2{q[i][0], q[i][1]}, reinterpret_cast<u32x2*>(o + 4 * i));
-        }
+      for (int i = 0; i < 4; i += 2, o += 32) {
+        const int at = n + 16 * i + 8 * g;
+        if (in && at + 8 <= a.N) __builtin_nontemporal_store(Eight{q[i][0], q[i][1], q[i + 1][0], q[i + 1][1]}, reinterpret_cast<Eight*>(o));
+        else if (in && at < a.N) __builtin_nontemporal_store(u32x2{q[i][0], q[i][1]}, reinterpret_cast<u32x2*>(o));
       }
     } else if (in) {
       float* o = static_cast<float*>(a.out) + (int64_t)row * a.ld_out + n + 4 * g;
