@@ -151,7 +151,7 @@ typedef struct c4s_kv_rows {
   int64_t ldk, ldv;
   const int32_t* lens;          /* [n_seqs] */
   const int32_t* rows_off;      /* [n_seqs + 1] or NULL */
-  int32_t n_rows;
+  int32_t n_rows;               /* n_rows * n_kv_heads up to 536870912 */
   int32_t dtype;                /* c4s_kv_append: C4S_DTYPE_BF16; c4s_kv_read: or C4S_DTYPE_F32 */
 } c4s_kv_rows;
 
@@ -181,7 +181,7 @@ typedef struct c4s_attn_desc {
   const int32_t* rows_off;      /* [n_seqs + 1] or NULL (one row a sequence) */
   const int32_t* first;         /* [n_seqs] or NULL (= 0): the positions before it are padding */
   int32_t n_rows;
-  int32_t max_new;              /* rows a sequence has at most; what is beyond is not computed */
+  int32_t max_new;              /* rows a sequence has at most; what is beyond is not computed; max_new * n_heads up to 536870912 */
   int32_t n_heads;              /* a multiple of the cache's n_kv_heads */
   float scale;
 } c4s_attn_desc;

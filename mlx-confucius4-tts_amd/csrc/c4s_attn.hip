@@ -877,8 +877,11 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
 
 template <int DH, bool Q8, int NB, int W, int OCC>
 hipError_t many(const AttnArgs& a, hipStream_t s) {
-  const int together = std::min(a.c.n_seqs, 64);
-  const ManyArgs f{a, (int)(((int64_t)a.max_new * a.shared + 16 * NB * W - 1) / (16 * NB * W)), together};
+  const int tiles = (int)(((int64_t)a.max_new * a.shared + 16 * NB * W - 1) / (16 * NB * W));
+  // 64 sequences, or what the grid has room for (2^32 threads in a dimension)
+  const int64_t room = (int64_t)(UINT32_MAX / (64 * W)) / ((int64_t)tiles * a.c.n_heads);
+  const int together = (int)std::min<int64_t>(std::min(a.c.n_seqs, 64), std::max<int64_t>(room, 1));
+  const ManyArgs f{a, tiles, together};
   hipLaunchKernelGGL((k_attn_many<DH, Q8, NB, W, OCC>), dim3((unsigned)((int64_t)f.tiles * a.c.n_heads * together), (a.c.n_seqs + together - 1) / together),
                      dim3(64 * W), 0, s, f);
   return hipGetLastError();

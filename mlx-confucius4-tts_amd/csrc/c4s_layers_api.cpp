@@ -135,6 +135,7 @@ int check_rows(c4s_ctx* ctx, const c4s_kv_cache* c, const c4s_kv_rows* r, bool r
   const uintptr_t mask = r->dtype == C4S_DTYPE_F32 ? 15u : 7u;
   if (((bits(r->k) | bits(r->v)) & mask) || ((r->ldk | r->ldv) & 3))
     return fail(ctx, C4S_EINVAL, "kv_rows: rows must start on 8 bytes (f32: 16)");
+  if ((int64_t)r->n_rows * c->n_kv_heads > 1 << 29) return fail(ctx, C4S_EINVAL, "kv_rows: n_rows * n_kv_heads above 536870912");
   if (!r->rows_off && r->n_rows > c->n_seqs) return fail(ctx, C4S_EINVAL, "kv_rows: more rows than sequences without rows_off");
   return C4S_OK;
 }
@@ -156,8 +157,8 @@ int check_attn(c4s_ctx* ctx, const c4s_kv_cache* c, const c4s_attn_desc* a) {
     return fail(ctx, C4S_EINVAL, "attn: rows of q must start on 16 bytes, rows of out on 8");
   if (!a->rows_off && a->n_rows > c->n_seqs) return fail(ctx, C4S_EINVAL, "attn: more rows than sequences without rows_off");
   if (!(a->scale - a->scale == 0.0f)) return fail(ctx, C4S_EINVAL, "attn: scale is not finite");
-  if (a->max_new > a->n_rows || (int64_t)a->max_new * a->n_heads > INT32_MAX - 1024)
-    return fail(ctx, C4S_EINVAL, "attn: max_new out of range");
+  if (a->max_new > a->n_rows || (int64_t)a->max_new * a->n_heads > 1 << 29)
+    return fail(ctx, C4S_EINVAL, "attn: max_new above n_rows, or max_new * n_heads above 536870912");
   return C4S_OK;
 }
 

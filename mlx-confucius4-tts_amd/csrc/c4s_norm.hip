@@ -164,8 +164,9 @@ template <int T, int E, bool TAIL, bool X, bool Y>
 __global__ __launch_bounds__(T > kNormThreads ? T : kNormThreads) void k_block_norm(c4s_norm a) {
   constexpr int kRows = T < kNormThreads ? kNormThreads / T : 1;
   __shared__ float part[4 * (T / 64)];
-  const int m = blockIdx.x * kRows + (kRows > 1 ? (int)threadIdx.x / T : 0);
-  if (m >= a.M) return;   // whole waves: with T > 64 a workgroup is one row
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kRows + (kRows > 1 ? (int)threadIdx.x / T : 0);
+  if (row >= a.M) return;   // whole waves: with T > 64 a workgroup is one row
+  const int m = (int)row;
   Row<T, E, TAIL> r;
   r.D = a.D;
   r.t = threadIdx.x % T;
@@ -204,7 +205,9 @@ template <int T, int E, bool TAIL>
 hipError_t launch(const c4s_norm& a, hipStream_t s) {
   constexpr int kRows = T < kNormThreads ? kNormThreads / T : 1;
   const bool x = a.x_dtype == C4S_DTYPE_BF16, y = a.y && a.y_dtype == C4S_DTYPE_BF16;
-  const dim3 grid((a.M + kRows - 1) / kRows), block(std::max(T, kNormThreads));
+  // a grid has up to 2^32 threads in a dimension
+  const uint32_t groups = ((uint32_t)a.M + kRows - 1) / kRows, wide = std::min(groups, 1u << 20);
+  const dim3 grid(wide, (groups + wide - 1) / wide), block(std::max(T, kNormThreads));
   if (x && y) hipLaunchKernelGGL((k_block_norm<T, E, TAIL, true, true>), grid, block, 0, s, a);
   else if (x) hipLaunchKernelGGL((k_block_norm<T, E, TAIL, true, false>), grid, block, 0, s, a);
   else if (y) hipLaunchKernelGGL((k_block_norm<T, E, TAIL, false, true>), grid, block, 0, s, a);

@@ -363,3 +363,33 @@ def test_split_calls_on_two_streams_at_once(gpu_ctx):
     torch.cuda.synchronize()
     for s, w in ((a, wa), (b, wb)):
         assert torch.equal(s["a"], w[0]) and torch.equal(s["o"], w[1])
+
+
+# ---- sizes ----------------------------------------------------------------------------------------
+
+def test_norm_of_many_short_rows(gpu_ctx):
+    """More rows than a grid's first dimension holds workgroups for (2^20 of four rows)."""
+    M, D = (1 << 22) + 5, 3
+    x = torch.randn((M, D), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = torch.empty((M, D), device="cuda")
+    gpu_ctx.block_norm(x.cuda(), None, None, out)
+    want = L.norm(L.f64(x), False, 1e-5, None, None)
+    # deviations of three values: the mean's three roundings, twice an ulp of its products and the root
+    err = 16 * L.U * (want.abs() + (L.f64(x).abs().amax(1) / (L.f64(x).var(1, unbiased=False) + 1e-5).sqrt())[:, None])
+    assert ((L.f64(out) - want).abs() <= err).all()
+
+
+def test_sizes_past_the_grid_are_refused(gpu_ctx):
+    """Nothing is queued: the addresses are of small tensors."""
+    z = lambda *s, t=torch.bfloat16: torch.zeros(s, dtype=t, device="cuda")  # noqa: E731
+    kc = c4s.KvCache(z(3, 2, 16, 64), z(3, 2, 64, 16), z(2, 3, t=torch.int32))
+    p, lens, off = z(16, 2, 64).data_ptr(), z(2, t=torch.int32).data_ptr(), z(3, t=torch.int32).data_ptr()
+    rows = c4s._pack_rows(p, p, 128, 128, lens, off, (1 << 28) + 1, c4s.BF16)
+    for call in (c4s.lib().c4s_kv_append, c4s.lib().c4s_kv_read):
+        assert call(gpu_ctx._h, kc.packed, rows, None) == c4s.EINVAL
+        assert b"536870912" in c4s.lib().c4s_last_error(gpu_ctx._h)
+    n = (1 << 28) + 1
+    attn = c4s._pack_attn(p, 128, p, 128, 0, lens, off, 0, n, n, 2, 0.125)
+    assert c4s.lib().c4s_attn(gpu_ctx._h, kc.packed, attn, None) == c4s.EINVAL
+    assert b"536870912" in c4s.lib().c4s_last_error(gpu_ctx._h)
+    torch.cuda.synchronize()
