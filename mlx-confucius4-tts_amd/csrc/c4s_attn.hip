@@ -525,11 +525,14 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
 // first, those of up to 64 sequences together (of one after the other: 8 of 2048,
 // 20 heads of 64, 169 us for 152; 4 of 2000, 5 heads of 256 195 for 172).
 //
-// Weights enter the second product rounded to bf16 once: independent roundings
-// of 2^-9 at most, which add a quarter to the error of the output's own
-// rounding; as pairs, as with few rows, they would cost half as many matrix
-// instructions again. Their sum is taken before the rounding, in fp32 (from the
-// matrix engine, of the rounded weights, it would be cheaper and lse off by 3e-4).
+// Weights for bf16 values enter the second product rounded to bf16 once:
+// independent roundings of 2^-9 at most, which leave 1.15 to 1.4 times the error of
+// the output's own rounding (the largest weight is often 1, which has none); as
+// pairs, as with few rows, they would cost half as many matrix instructions again.
+// Weights for codes have the values' scales in them, none is exact, and the error
+// would come to 1.5 times: those enter as pairs (8 prompts of 2048, 20 heads of 64:
+// 224 us for 185, 1.0 times). The weights' sum is taken before the rounding, in fp32
+// (from the matrix engine, of the rounded weights, it would be cheaper and lse off by 3e-4).
 constexpr int kBlock = 64;         // positions
 constexpr int kSegment = 16384;    // positions whose pages LDS holds at a time
 constexpr float kSlack = 8.0f;     // weights stay below 2^kSlack: rows are rescaled only when that would not hold
@@ -782,7 +785,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
         for (int i = 0; i < 4; ++i) va[i] = value(i / 2, i % 2);
         __builtin_amdgcn_sched_barrier(0);
       }
-      uint32_t p[NB][8];
+      uint32_t p[NB][8], rest[NB][Q8 ? 8 : 1];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         float top = fmaxf(s[b][0][0], s[b][0][1]);
@@ -808,9 +811,14 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
             y *= vs[1];
           }
           p[b][j / 2] = pack(x, y);
+          if constexpr (Q8) rest[b][j / 2] = pack(x - low(p[b][j / 2]), y - high(p[b][j / 2]));
         }
       }
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
+      auto add = [&](f32x4& to, uint4 v, int b, int st) {
+        to = mfma(v, quad(p[b] + 4 * st), to);
+        if constexpr (Q8) to = mfma(v, quad(rest[b] + 4 * st), to);
+      };
       if constexpr (kAhead) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(l[b]));   // summed here: the weights' registers are free for values
@@ -823,13 +831,13 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
 #pragma unroll
           for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b][d] = mfma(va[2 * d + st], quad(p[b] + 4 * st), o[b][d]);
+            for (int b = 0; b < NB; ++b) add(o[b][d], va[2 * d + st], b, st);
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
           for (int d = 0; d < 2; ++d)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b][2 + d] = mfma(vb[2 * d + st], quad(p[b] + 4 * st), o[b][2 + d]);
+            for (int b = 0; b < NB; ++b) add(o[b][2 + d], vb[2 * d + st], b, st);
       } else {
 #pragma unroll
         for (int d = 0; d < kTiles; ++d) {
@@ -838,7 +846,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
           for (int st = 0; st < 2; ++st) {
             const uint4 v = *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st));
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b][d] = mfma(v, quad(p[b] + 4 * st), o[b][d]);
+            for (int b = 0; b < NB; ++b) add(o[b][d], v, b, st);
           }
         }
       }
