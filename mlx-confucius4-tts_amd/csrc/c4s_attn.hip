@@ -895,13 +895,18 @@ hipError_t many(const AttnArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Few rows' tiles re-read the positions but share them out over the chip: they win while they are few (many /
-// few rows' kernel, us: 4 rows of 128 over 4000, 20 heads of 64, 640 tiles: 78 / 70; 4 of 300 over 500, 1520
-// tiles: 22 / 31; 1 of 300, 8 key heads of 128 with 4 query heads each, 600 tiles: 21 / 14; 16 of 32, 1024
-// tiles: 11 / 13), and where a sequence has one tile, of which the other kernel would leave most rows empty.
+// Few rows' tiles re-read the positions but share them out over the chip: they win while they are few, and where
+// the other kernel would leave most rows of a workgroup empty. Few / many rows' kernel, us, by tiles: bf16, 20 heads
+// of 64: 1 of 500 rows, 640, 9.2 / 11.8; 4 of 128 over 4000, 640, 72 / 66; 2 of 300, 760, 8.1 / 8.2; 4 of 300 over 500,
+// 1520, 31 / 18; 8 key heads of 128 with 4 query heads each: 1 of 300, 600, 15.5 / 18.9; 2 of 200 over 1000, 800, 70 /
+// 50. 8-bit codes are converted for each block of the many rows' kernel by all its waves: 20 heads of 64: 4 of 128 over
+// 1000, 640, 21 / 30; 2 of 600, 1520, 17.9 / 18.9; 4 of 300 over 500, 1520, 27 / 24; 64 of 48 and of 64 over 300,
+// three and four tiles a sequence, 35 / 39 and 45 / 42; 8 heads of 128: 2 of 200 over 1000, 800, 43 / 65; 2 of 400 over 400, 1600, 48 / 48; 5 heads of 256: 4
+// of 200 over 200, 500, 30 / 29; 4 of 500 over 500, 1260, 107 / 59.
 bool many_pays(const AttnArgs& a) {
-  const int64_t tiles = ((int64_t)a.max_new * a.shared + kRows - 1) / kRows;
-  return tiles > 1 && tiles * a.c.n_heads * a.c.n_seqs > 700;
+  const int64_t tiles = ((int64_t)a.max_new * a.shared + kRows - 1) / kRows, all = tiles * a.c.n_heads * a.c.n_seqs;
+  if (a.c.store == C4S_KV_Q8 && a.c.dim <= 128) return tiles > 3 && all > 1500;
+  return tiles > 1 && all > 700;
 }
 
 }  // namespace

@@ -13,9 +13,12 @@ from test_gpu_layers import _check_attn, _close, _packed, _run_attn
 pytestmark = pytest.mark.gpu
 
 
-def _fills(new, heads, kv_heads, seqs):
-    """Tiles of 16 (row, query head) pairs of a key head: more than 700, and more than one a sequence."""
+def _fills(new, heads, kv_heads, seqs, q8=False, dim=64):
+    """Tiles of 16 (row, query head) pairs of a key head: more than 700, and more than one a sequence
+    (8-bit heads of up to 128: 1500, three)."""
     tiles = -(-max(new) * (heads // kv_heads) // 16)
+    if q8 and dim <= 128:
+        return tiles > 3 and tiles * kv_heads * seqs > 1500
     return tiles > 1 and tiles * kv_heads * seqs > 700
 
 
@@ -23,15 +26,17 @@ def _fills(new, heads, kv_heads, seqs):
 
 PROMPTS = [  # new, past, heads, kv_heads, dim, page, q8
     ([210, 1, 64, 0, 129], [0, 50, 17, 3, 64], 20, 20, 64, 16, False),
-    ([210, 1, 64, 0, 129], [7, 150, 17, 3, 63], 20, 20, 64, 32, True),
+    ([210, 1, 64, 0, 129], [7, 150, 17, 3, 63], 24, 24, 64, 32, True),
     ([190, 257], [300, 0], 32, 8, 48, 64, False),
     ([100, 31, 97], [29, 0, 200], 60, 20, 80, 128, False),
-    ([150, 65], [3, 300], 40, 10, 128, 64, True),
+    ([150, 65], [3, 300], 80, 20, 128, 64, True),
+    ([210, 1, 64, 70, 129], [7, 150, 17, 3, 63], 24, 24, 80, 16, True),
+    ([400, 65], [3, 300], 32, 32, 48, 256, True),
     ([150, 65], [3, 300], 40, 10, 128, 16, False),
     ([70, 140], [7, 120], 40, 40, 256, 16, True),
     ([70, 140], [7, 120], 40, 40, 256, 256, False),
     ([61, 17, 40], [64, 1000, 0], 64, 16, 192, 32, False),
-    ([260, 3], [5, 90], 32, 2, 112, 64, True),
+    ([260, 3, 50], [5, 90, 0], 32, 2, 112, 64, True),
     ([700], [1], 20, 20, 16, 16, False),
 ]
 
@@ -40,7 +45,7 @@ PROMPTS = [  # new, past, heads, kv_heads, dim, page, q8
 def test_prompts(gpu_ctx, new, past, heads, kv_heads, dim, page, q8):
     """Unused places of the pages hold NaN."""
     print(f"attn prompts new={new} past={past} heads={heads}/{kv_heads} dim={dim} page={page} q8={q8}", flush=True)
-    assert _fills(new, heads, kv_heads, len(new))
+    assert _fills(new, heads, kv_heads, len(new), q8, dim)
     cache = L.Cache([n + p for n, p in zip(new, past)], kv_heads, dim, page, q8, seed=dim + page, junk=float("nan"))
     q, out, lse = _run_attn(gpu_ctx, cache, new, heads)
     _check_attn(cache, q, out, lse, new, heads, prompts=True)
@@ -51,9 +56,9 @@ def test_prompts(gpu_ctx, new, past, heads, kv_heads, dim, page, q8):
 def test_prompts_first(gpu_ctx, dim, q8):
     """Padding in front, in the middle of a block, past whole blocks, past every key of some rows or of all:
     zeros and an lse of -inf there. What is masked is not finite."""
-    new, past, first, heads = [130, 100, 70, 20], [5, 130, 90, 0], [10, 131, 165, 2 ** 31 - 1], 32
+    new, past, first, heads = [130, 100, 70, 20], [5, 130, 90, 0], [10, 131, 165, 2 ** 31 - 1], 48 if q8 else 32
     print(f"attn prompts first={first} dim={dim} q8={q8}", flush=True)
-    assert _fills(new, heads, heads, 4)
+    assert _fills(new, heads, heads, 4, q8, dim)
     cache = L.Cache([n + p for n, p in zip(new, past)], heads, dim, 32, q8, seed=5, junk=float("inf"))
     for b, f in enumerate(first):
         for p in range(min(f, cache.lens[b])):
@@ -74,8 +79,8 @@ def test_prompts_first(gpu_ctx, dim, q8):
 @pytest.mark.parametrize("q8", [False, True])
 def test_prompts_missing_pages(gpu_ctx, q8):
     """Pages that are not there, one or several blocks of them, and a sequence of none; one longer than its table."""
-    new, heads = [200, 30, 150, 90], 16
-    assert _fills(new, heads, heads, 4)
+    new, heads = [200, 30, 150, 90], 32 if q8 else 16
+    assert _fills(new, heads, heads, 4, q8)
     cache = L.Cache([300, 30, 150, 100], heads, 64, 16, q8, seed=8)
     cache.table[0, 3:11] = -1
     cache.table[0, 14] = cache.n_pages + 5
@@ -91,8 +96,8 @@ def test_prompts_missing_pages(gpu_ctx, q8):
 @pytest.mark.parametrize("n,p", [(700, 3), (640, 200)])
 def test_prompts_later_rows_do_not_reach_earlier_ones(gpu_ctx, n, p, q8):
     """Keys and values that are not finite in later positions, up to two in a block of them."""
-    heads = 20
-    assert _fills([n], heads, heads, 1)
+    heads = 40 if q8 else 20
+    assert _fills([n], heads, heads, 1, q8)
     make = lambda: L.Cache([n + p], heads, 64, 16, q8, seed=6)  # noqa: E731
     cache, clean = make(), make()
     for bad in (p + n // 2, p + n // 2 + 2, p + n // 2 + 200):
@@ -147,20 +152,21 @@ def _sampled(cache, q, out, lse, first_row, n, b, heads, rows, single):
 @pytest.mark.parametrize("q8", [False, True])
 def test_prompts_behind_long_prefixes(gpu_ctx, q8):
     """Prefixes of more pages than a workgroup looks up at a time (16384 positions), begun with the prefix or in it."""
-    new, heads = [50, 3, 64], 64
-    assert _fills(new, heads, 16, 3)
-    cache = L.Cache([33000, 40, 16384 + 30], 16, 64, 16, q8, seed=3)
+    new, kv_heads = [50, 3, 64], 34 if q8 else 16
+    heads = 4 * kv_heads
+    assert _fills(new, heads, kv_heads, 3, q8)
+    cache = L.Cache([33000, 40, 16384 + 30], kv_heads, 64, 16, q8, seed=3)
     q, out, lse = _run_attn(gpu_ctx, cache, new, heads, one=False)
     _sampled(cache, q, out, lse, 0, 50, 0, heads, [0, 17, 49], True)
     _sampled(cache, q, out, lse, 53, 64, 2, heads, [0, 33, 34, 63], True)
-    cache = L.Cache([16384 + 60, 200], 90, 32, 16, q8, seed=4)
-    new = [64, 64]
-    assert _fills(new, 90, 90, 2)
-    q, out, lse = _run_attn(gpu_ctx, cache, new, 90, one=False)
-    _sampled(cache, q, out, lse, 0, 64, 0, 90, [0, 3, 4, 5, 63], True)
-    _sampled(cache, q, out, lse, 64, 64, 1, 90, [0, 63], True)
+    new, heads = [64, 64], 190 if q8 else 90
+    assert _fills(new, heads, heads, 2, q8)
+    cache = L.Cache([16384 + 60, 200], heads, 32, 16, q8, seed=4)
+    q, out, lse = _run_attn(gpu_ctx, cache, new, heads, one=False)
+    _sampled(cache, q, out, lse, 0, 64, 0, heads, [0, 3, 4, 5, 63], True)
+    _sampled(cache, q, out, lse, 64, 64, 1, heads, [0, 63], True)
     first = [16384 + 2, 0]
-    q, out, lse = _run_attn(gpu_ctx, cache, new, 90, one=False, first=first)
+    q, out, lse = _run_attn(gpu_ctx, cache, new, heads, one=False, first=first)
     for i in (0, 1, 2, 5, 6, 63):
         want, wlse, mag, sq = L.attn_row(cache, 0, 16384 + 60 - 64 + i, q[i], 32 ** -0.5, first[0])
         _close(out[i], want, 1e-4 * mag + 6 * 2.0 ** -9 * sq)
