@@ -270,45 +270,51 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _vector(t, n, what):
-    """The address of a contiguous float32 vector of n values; 0 of None."""
+def _refuse(t, what, device):
+    """Raises what is wrong with tensor t. (A kernel that is given an address of the host's, or of another GPU,
+    faults and takes the process with it, so every helper below looks where its tensor lives.)"""
+    raise ValueError(what if t.get_device() == device else f"{what}; it must be on the context's device, cuda:{device}")
+
+
+def _vector(t, n, what, device):
+    """The address of a contiguous float32 vector of n values on this device; 0 of None."""
     if t is None:
         return 0
-    if t.dtype is _Torch.f32 and t.numel() == n and t.is_contiguous():
+    if t.dtype is _Torch.f32 and t.numel() == n and t.is_contiguous() and t.get_device() == device:
         return t.data_ptr()
-    raise ValueError(what)
+    _refuse(t, what, device)
 
 
-def _i32(t, n, what):
-    """The address of a contiguous int32 vector of n values; 0 of None."""
+def _i32(t, n, what, device):
+    """The address of a contiguous int32 vector of n values on this device; 0 of None."""
     if t is None:
         return 0
-    if t.dtype is _Torch.i32 and t.numel() == n and t.is_contiguous():
+    if t.dtype is _Torch.i32 and t.numel() == n and t.is_contiguous() and t.get_device() == device:
         return t.data_ptr()
-    raise ValueError(what)
+    _refuse(t, what, device)
 
 
-def _rows(t, shape, what):
-    """(address, row stride, C4S_DTYPE_*) of a [rows][width] tensor of this shape, bfloat16 or
-    float32, whose rows are contiguous; (0, 0, F32) of None."""
+def _rows(t, shape, what, device):
+    """(address, row stride, C4S_DTYPE_*) of a [rows][width] tensor of this shape on this device,
+    bfloat16 or float32, whose rows are contiguous; (0, 0, F32) of None."""
     if t is None:
         return 0, 0, F32
     kind = _Torch.kinds.get(t.dtype)
-    if kind is not None and t.shape == shape:
+    if kind is not None and t.shape == shape and t.get_device() == device:
         ld, one = t.stride()
         if one == 1 or shape[1] <= 1:
             return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), kind
-    raise ValueError(what)
+    _refuse(t, what, device)
 
 
-def _heads(t, shape, what):
+def _heads(t, shape, what, device):
     """As _rows, of a [rows][heads][dim] tensor."""
     kind = _Torch.kinds.get(t.dtype)
-    if kind is not None and t.shape == shape:
+    if kind is not None and t.shape == shape and t.get_device() == device:
         ld, dim, one = t.stride()
         if one == 1 and (dim == shape[2] or shape[1] == 1):
             return t.data_ptr(), (ld if shape[0] > 1 else shape[1] * shape[2]), kind
-    raise ValueError(what)
+    _refuse(t, what, device)
 
 
 class KvCache:
@@ -335,6 +341,9 @@ class KvCache:
                   "KvCache: scales must be contiguous float32 [n_pages][n_kv_heads][page_size]")
         _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and
               (block_table.shape[1] <= 1 or block_table.stride(1) == 1), "KvCache: block_table must be int32 rows")
+        self.device = k.get_device()
+        _need(self.device >= 0 and all(t is None or t.get_device() == self.device for t in (v, block_table, k_scale, v_scale)),
+              "KvCache: all tensors must be on one GPU")
         n_seqs, max_pages = block_table.shape
         self.k, self.v, self.k_scale, self.v_scale, self.block_table = k, v, k_scale, v_scale, block_table
         self.n_seqs, self.n_kv_heads, self.head_dim, self.page_size = n_seqs, heads, dim, size
@@ -508,27 +517,27 @@ class Context:
         """r = x + scale * gate (.) u with u = y, or norm(y) when post; x_out = r;
         out = norm(r). x, y, x_out, out: [rows][D], bfloat16 or float32; gate:
         float32 [ceil(rows / gate_rows)][D]; without y, r = x."""
-        shape = x.shape
+        shape, dev = x.shape, self.device
         M, D = shape
-        xp, ldx, xt = _rows(x, shape, "block_norm: x must be bfloat16 or float32, its rows contiguous")
-        yp, ldy, yt = _rows(y, shape, "block_norm: y must be bfloat16 or float32 of x's shape, its rows contiguous")
-        op, ldo, ot = _rows(out, shape, "block_norm: out must be bfloat16 or float32 of x's shape, its rows contiguous")
+        xp, ldx, xt = _rows(x, shape, "block_norm: x must be bfloat16 or float32, its rows contiguous", dev)
+        yp, ldy, yt = _rows(y, shape, "block_norm: y must be bfloat16 or float32 of x's shape, its rows contiguous", dev)
+        op, ldo, ot = _rows(out, shape, "block_norm: out must be bfloat16 or float32 of x's shape, its rows contiguous", dev)
         xo = ldxo = g = ldg = 0
         if x_out is not None:
-            xo, ldxo, t = _rows(x_out, shape, "block_norm: x_out must have x's shape and dtype, its rows contiguous")
+            xo, ldxo, t = _rows(x_out, shape, "block_norm: x_out must have x's shape and dtype, its rows contiguous", dev)
             _need(t == xt, "block_norm: x_out must have x's dtype")
         if gate is not None:
-            g, ldg, t = _rows(gate, (gate.shape[0], D), "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
+            g, ldg, t = _rows(gate, (gate.shape[0], D), "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]", dev)
             _need(t == F32 and gate_rows >= 1 and gate.shape[0] * gate_rows >= M,
                   "block_norm: gate must be float32 [ceil(rows / gate_rows)][D]")
         if post_gamma is not None or post_beta is not None:
-            post_gamma = _vector(post_gamma, D, "block_norm: post_gamma must be a float32 vector of D")
-            post_beta = _vector(post_beta, D, "block_norm: post_beta must be a float32 vector of D")
+            post_gamma = _vector(post_gamma, D, "block_norm: post_gamma must be a float32 vector of D", dev)
+            post_beta = _vector(post_beta, D, "block_norm: post_beta must be a float32 vector of D", dev)
         rc = _lib.c4s_block_norm(
             self._h, _pack_norm(M, D, NORM_RMS if rms else NORM_LAYER, eps, xp, ldx, xt, yt, yp, ldy, 1 if post else 0,
                                 gate_rows, post_gamma or 0, post_beta or 0, g, ldg, scale, ot,
-                                _vector(gamma, D, "block_norm: gamma must be a float32 vector of D"),
-                                _vector(beta, D, "block_norm: beta must be a float32 vector of D"), xo, ldxo, op, ldo),
+                                _vector(gamma, D, "block_norm: gamma must be a float32 vector of D", dev),
+                                _vector(beta, D, "block_norm: beta must be a float32 vector of D", dev), xo, ldxo, op, ldo),
             _Torch.raw_stream(self.device) if stream is None else _stream_handle(stream))
         if rc:
             self._check(rc, "block_norm")
@@ -537,12 +546,12 @@ class Context:
         """out = residual + act(x @ weight^T + bias). x: bfloat16 [M][K]; weight:
         [N][K], bfloat16, or uint8 codes with quant=(scales, offsets, group);
         residual, out: [M][N], bfloat16 or float32; act: none, gelu, silu, relu."""
-        xs, ws = x.shape, weight.shape
+        xs, ws, dev = x.shape, weight.shape, self.device
         M, K = xs
         N = ws[0]
-        xp, ldx, t = _rows(x, xs, "linear: x must be bfloat16 [M][K], its rows contiguous")
-        if not (t == BF16 and ws == (N, K) and weight.is_contiguous()):
-            raise ValueError("linear: x must be bfloat16 [M][K], weight contiguous [N][K]")
+        xp, ldx, t = _rows(x, xs, "linear: x must be bfloat16 [M][K], its rows contiguous", dev)
+        if not (t == BF16 and ws == (N, K) and weight.is_contiguous() and weight.get_device() == dev):
+            _refuse(weight, "linear: x must be bfloat16 [M][K], weight contiguous [N][K]", dev)
         sp = bp = group = 0
         wt = W_BF16
         if quant is not None:
@@ -550,34 +559,34 @@ class Context:
             wt = W_Q8
             if not (group > 0 and scales.shape == offsets.shape == (N, K // group)):
                 raise ValueError("linear: scales and offsets must be contiguous float32 [N][K / group]")
-            sp = _vector(scales, N * (K // group), "linear: scales must be contiguous float32 [N][K / group]")
-            bp = _vector(offsets, N * (K // group), "linear: offsets must be contiguous float32 [N][K / group]")
+            sp = _vector(scales, N * (K // group), "linear: scales must be contiguous float32 [N][K / group]", dev)
+            bp = _vector(offsets, N * (K // group), "linear: offsets must be contiguous float32 [N][K / group]", dev)
         if weight.dtype is not (_Torch.bf16 if quant is None else _Torch.u8):
             raise ValueError("linear: weights are bfloat16, or uint8 with quant=(scales, offsets, group)")
         kind = ACTS.get(act)
         if kind is None:
             raise ValueError("linear: act must be none, gelu, silu or relu")
         shape = (M, N)
-        op, ldo, ot = _rows(out, shape, "linear: out must be bfloat16 or float32 [M][N], its rows contiguous")
-        rp, ldr, rt = _rows(residual, shape, "linear: residual must be bfloat16 or float32 [M][N], its rows contiguous")
+        op, ldo, ot = _rows(out, shape, "linear: out must be bfloat16 or float32 [M][N], its rows contiguous", dev)
+        rp, ldr, rt = _rows(residual, shape, "linear: residual must be bfloat16 or float32 [M][N], its rows contiguous", dev)
         rc = _lib.c4s_linear(
             self._h, _pack_linear(M, N, K, kind, xp, ldx, weight.data_ptr(), wt, group, sp, bp,
-                                  _vector(bias, N, "linear: bias must be a float32 vector of N"), rp, ldr, rt, ot, op, ldo),
+                                  _vector(bias, N, "linear: bias must be a float32 vector of N", dev), rp, ldr, rt, ot, op, ldo),
             _Torch.raw_stream(self.device) if stream is None else _stream_handle(stream))
         if rc:
             self._check(rc, "linear")
 
-    @staticmethod
-    def _kv_rows(cache, k, v, lens, rows_off):
-        shape = k.shape
+    def _kv_rows(self, cache, k, v, lens, rows_off):
+        shape, dev = k.shape, self.device
         rows, heads, dim = shape
+        _need(cache.device == dev, "kv rows: the cache is not on the context's device")
         _need(heads == cache.n_kv_heads and dim == cache.head_dim, "kv rows: k must be [rows][n_kv_heads][head_dim]")
-        kp, ldk, t = _heads(k, shape, "kv rows: k must be bfloat16 or float32, a row contiguous")
-        vp, ldv, vt = _heads(v, shape, "kv rows: v must have k's shape and dtype, a row contiguous")
+        kp, ldk, t = _heads(k, shape, "kv rows: k must be bfloat16 or float32, a row contiguous", dev)
+        vp, ldv, vt = _heads(v, shape, "kv rows: v must have k's shape and dtype, a row contiguous", dev)
         _need(vt == t, "kv rows: k and v must have one dtype")
         n = cache.n_seqs
-        return _pack_rows(kp, vp, ldk, ldv, _i32(lens, n, "kv rows: lens must be an int32 vector of n_seqs"),
-                          _i32(rows_off, n + 1, "kv rows: rows_off must be an int32 vector of n_seqs + 1"), rows, t)
+        return _pack_rows(kp, vp, ldk, ldv, _i32(lens, n, "kv rows: lens must be an int32 vector of n_seqs", dev),
+                          _i32(rows_off, n + 1, "kv rows: rows_off must be an int32 vector of n_seqs + 1", dev), rows, t)
 
     def kv_append(self, cache, k, v, lens, rows_off=None, stream=None):
         """The rows k, v (bfloat16 [rows][n_kv_heads][head_dim]) into the cache, as
@@ -597,19 +606,20 @@ class Context:
         """Attention of the rows q (bfloat16 [rows][n_heads][head_dim], the last
         positions of lens[b]) over the cache, into out. max_new: the most rows a
         sequence has (default: all rows); scale: 1 / sqrt(head_dim) by default."""
-        shape = q.shape
+        shape, dev = q.shape, self.device
         rows, heads, dim = shape
-        qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous")
-        op, ldo, ot = _heads(out, shape, "attn: out must be bfloat16 of q's shape, a row contiguous")
+        qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous", dev)
+        op, ldo, ot = _heads(out, shape, "attn: out must be bfloat16 of q's shape, a row contiguous", dev)
+        _need(cache.device == dev, "attn: the cache is not on the context's device")
         _need(qt == BF16 and ot == BF16 and dim == cache.head_dim,
               "attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's")
         n = cache.n_seqs
         rc = _lib.c4s_attn(
             self._h, cache.packed,
-            _pack_attn(qp, ldq, op, ldo, _vector(lse, rows * heads, "attn: lse must be contiguous float32 [rows][n_heads]"),
-                       _i32(lens, n, "attn: lens must be an int32 vector of n_seqs"),
-                       _i32(rows_off, n + 1, "attn: rows_off must be an int32 vector of n_seqs + 1"),
-                       _i32(first, n, "attn: first must be an int32 vector of n_seqs"), rows,
+            _pack_attn(qp, ldq, op, ldo, _vector(lse, rows * heads, "attn: lse must be contiguous float32 [rows][n_heads]", dev),
+                       _i32(lens, n, "attn: lens must be an int32 vector of n_seqs", dev),
+                       _i32(rows_off, n + 1, "attn: rows_off must be an int32 vector of n_seqs + 1", dev),
+                       _i32(first, n, "attn: first must be an int32 vector of n_seqs", dev), rows,
                        rows if max_new is None or max_new > rows else max_new, heads,
                        dim ** -0.5 if scale is None else scale),
             self._queue(stream))
