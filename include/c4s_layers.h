@@ -84,7 +84,7 @@ int c4s_block_norm(c4s_ctx* ctx, const c4s_norm* norm, void* stream);
 enum { C4S_ACT_NONE = 0, C4S_ACT_GELU = 1, C4S_ACT_SILU = 2, C4S_ACT_RELU = 3 };
 
 typedef struct c4s_linear_desc {
-  int32_t M, N, K;          /* N and K up to 4194304 */
+  int32_t M, N, K;          /* M up to 1073741824, N and K up to 4194304; ceil(M / 128) * ceil(N / 128) up to 16777208 */
   int32_t act;              /* C4S_ACT_* */
   const uint16_t* x;        /* [M][ldx] bf16 */
   int64_t ldx;              /* up to 4194304 */

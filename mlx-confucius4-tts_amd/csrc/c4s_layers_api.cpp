@@ -78,6 +78,10 @@ int check_norm(c4s_ctx* ctx, const c4s_norm* a) {
 int check_linear(c4s_ctx* ctx, const c4s_linear_desc* a) {
   if (a->M < 0 || a->N < 1 || a->K < 8 || a->K % 8) return fail(ctx, C4S_EINVAL, "linear: needs M >= 0, N >= 1, K a positive multiple of 8");
   if (a->N > 1 << 22 || a->K > 1 << 22) return fail(ctx, C4S_EINVAL, "linear: N or K above 4194304");
+  // rows are counted in 32 bits, up to a tile past the last; a grid has up to 2^32 threads, 256 a tile
+  if (a->M > 1 << 30) return fail(ctx, C4S_EINVAL, "linear: M above 1073741824");
+  if (((int64_t)a->M + 127) / 128 * ((a->N + 127) / 128) > (1 << 24) - 8)
+    return fail(ctx, C4S_EINVAL, "linear: more than 16777208 tiles of 128 x 128 outputs");
   if (a->M == 0) return C4S_OK;
   if (!a->x || !a->weight || !a->out) return fail(ctx, C4S_EINVAL, "linear: required pointer is NULL");
   if (a->act < C4S_ACT_NONE || a->act > C4S_ACT_RELU) return fail(ctx, C4S_EINVAL, "linear: unknown activation");

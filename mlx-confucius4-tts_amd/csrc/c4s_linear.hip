@@ -661,7 +661,6 @@ LayerSpace linear_space(const c4s_linear_desc& a) {
 }
 
 hipError_t launch_linear(const c4s_linear_desc& a, uint32_t* counters, float* space, hipStream_t s) {
-  if (tiles_of(a, 128, 128) > INT32_MAX - 8) return hipErrorInvalidValue;
   if (few_pays(a)) {
     const int64_t tiles = tiles_of(a, kFewM, kFewN);
     const FewArgs f{a, vectors(a), few_splits(a, tiles), (a.N + kFewN - 1) / kFewN, counters, space};

@@ -42,3 +42,30 @@ def test_host_tensors(gpu_ctx):
                                          first=z(2, t=I32), lse=z(2, 2, t=F32)), "cuda:0")
     _each_on_the_host(c4s.KvCache, dict(k=z(3, 2, 16, 64, t=I8), v=z(3, 2, 64, 16, t=I8), block_table=z(2, 3, t=I32),
                                         k_scale=z(3, 2, 16, t=F32), v_scale=z(3, 2, 16, t=F32)), "GPU")
+
+
+@pytest.mark.parametrize("M,N,what", [(2 ** 31 - 1, 4, b"1073741824"), (2 ** 31 - 200, 4, b"1073741824"),
+                                      (2 ** 30 + 1, 4, b"1073741824"), (2 ** 30, 129, b"16777208"),
+                                      (128 * 32768 + 1, 65536, b"16777208"), (2 ** 23, 2 ** 22, b"16777208")])
+def test_linear_past_a_grid(gpu_ctx, M, N, what):
+    """Within 255 of 2^31 rows a count of tiles in 32 bits turns negative; from 2^24 tiles on the grid has 2^32
+    threads. Nothing is queued: the addresses are of small tensors."""
+    x, w, out = z(16, 64), z(16, 64), z(16, 64)
+    desc = c4s._pack_linear(M, N, 64, 0, x.data_ptr(), 64, w.data_ptr(), c4s.W_BF16, 0, 0, 0, 0, 0, 0, c4s.F32, c4s.BF16,
+                            out.data_ptr(), N)
+    assert c4s.lib().c4s_linear(gpu_ctx._h, desc, None) == c4s.EINVAL
+    assert what in c4s.lib().c4s_last_error(gpu_ctx._h)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
+def test_linear_of_many_short_rows(gpu_ctx):
+    """2^28 + 3 rows of 8 inputs, past 2^32 bytes, and one output each."""
+    M = (1 << 28) + 3
+    g = torch.Generator().manual_seed(3)
+    small = torch.randint(-4, 5, (4099, 8), generator=g).to(BF).cuda()     # exact in every order
+    w = torch.randint(-4, 5, (1, 8), generator=g).to(BF).cuda()
+    x = small.repeat(-(-M // 4099), 1)[:M]
+    out = torch.empty((M, 1), device="cuda")
+    gpu_ctx.linear(x, w, out)
+    assert torch.equal(out[:, 0], (small.float() * w.float()).sum(1).repeat(-(-M // 4099))[:M])
