@@ -170,7 +170,8 @@ int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_kv_rows* rows
  * (those read inf or NaN).
  * Refused (C4S_EINVAL): max_pages above 1024 together with more than 262144 of
  * (sequence, key head, 16 of its new rows' query heads), where few rows a sequence
- * have their positions' parts joined. */
+ * have their positions' parts joined, or with more than 16777215 of (such a one of
+ * a single sequence, part of its positions), of which there are up to 128 parts. */
 typedef struct c4s_attn_desc {
   const uint16_t* q;            /* [n_rows][ldq] bf16: row r's head h at q + r * ldq + h * head_dim; 16-byte aligned, ldq a multiple of 8 */
   int64_t ldq;

@@ -915,6 +915,8 @@ LayerSpace attn_space(const AttnArgs& a) {
   if (many_pays(a)) return {};
   const FewArgs f = few_args(a);
   if (f.splits == 1) return {};
+  // more threads than a grid has room for in its first dimension: more counters than there are, which the caller refuses
+  if ((int64_t)f.tiles * f.splits * a.c.n_heads > (int64_t)(UINT32_MAX / kAttnThreads)) return {INT64_MAX / 4, 1};
   const int64_t groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
   return {groups, groups * f.splits * kRows * (a.c.dim + 4)};
 }

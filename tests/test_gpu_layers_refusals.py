@@ -69,3 +69,17 @@ def test_linear_of_many_short_rows(gpu_ctx):
     out = torch.empty((M, 1), device="cuda")
     gpu_ctx.linear(x, w, out)
     assert torch.equal(out[:, 0], (small.float() * w.float()).sum(1).repeat(-(-M // 4099))[:M])
+
+
+def test_attn_past_a_grid(gpu_ctx):
+    """65535 key heads, three tiles of query heads each, 128 parts of 2^21 positions: 2^32 threads and more. Refused
+    before any workspace is made; nothing is queued: the addresses are of small tensors."""
+    p, s, i = z(16, 64).data_ptr(), z(16, 64, t=F32).data_ptr(), z(64, t=I32).data_ptr()
+    heads, pages, shared = 65535, 131072, 48
+    cache = bytes(c4s.KvCacheDesc(p, p, s, s, i, pages, 1, pages, 1, 16, heads, 16, c4s.KV_Q8))
+    attn = c4s._pack_attn(p, heads * shared * 16, p, heads * shared * 16, 0, i, 0, 0, 1, 1, heads * shared, 0.25)
+    free = torch.cuda.mem_get_info()[0]
+    assert c4s.lib().c4s_attn(gpu_ctx._h, cache, attn, None) == c4s.EINVAL
+    assert b"too many parts" in c4s.lib().c4s_last_error(gpu_ctx._h)
+    assert free - torch.cuda.mem_get_info()[0] < 1 << 30
+    torch.cuda.synchronize()
