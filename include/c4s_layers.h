@@ -182,7 +182,8 @@ typedef struct c4s_attn_desc {
   const int32_t* rows_off;      /* [n_seqs + 1] or NULL (one row a sequence) */
   const int32_t* first;         /* [n_seqs] or NULL (= 0): the positions before it are padding */
   int32_t n_rows;
-  int32_t max_new;              /* rows a sequence has at most; what is beyond is not computed; max_new * n_heads up to 536870912 */
+  int32_t max_new;              /* with rows_off: rows a sequence has at most; what is beyond is not computed. Without it not
+                                   looked at (a sequence has one row). min(max_new, n_rows) * n_heads up to 536870912 */
   int32_t n_heads;              /* a multiple of the cache's n_kv_heads */
   float scale;
 } c4s_attn_desc;

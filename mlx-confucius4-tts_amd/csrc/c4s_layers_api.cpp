@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <new>
 
 #include "../../include/c4s_layers.h"
@@ -148,10 +149,13 @@ c4s::KvRowsArgs to_args(const c4s_kv_rows* r) {
   return c4s::KvRowsArgs{r->k, r->v, r->ldk, r->ldv, r->lens, r->rows_off, r->n_rows, r->dtype == C4S_DTYPE_F32};
 }
 
+// Rows a sequence has at most: one without rows_off, whatever max_new says, and never more than there are.
+int32_t new_rows(const c4s_attn_desc* a) { return a->rows_off ? std::min(a->max_new, a->n_rows) : 1; }
+
 int check_attn(c4s_ctx* ctx, const c4s_kv_cache* c, const c4s_attn_desc* a) {
   int rc = check_cache(ctx, c);
   if (rc) return rc;
-  if (a->n_rows < 0 || a->max_new < 0) return fail(ctx, C4S_EINVAL, "attn: n_rows or max_new < 0");
+  if (a->n_rows < 0 || (a->rows_off && a->max_new < 0)) return fail(ctx, C4S_EINVAL, "attn: n_rows or max_new < 0");
   if (a->n_heads < 1 || a->n_heads % c->n_kv_heads) return fail(ctx, C4S_EINVAL, "attn: n_heads must be a multiple of n_kv_heads");
   if (a->n_rows == 0) return C4S_OK;
   if (!a->q || !a->out || !a->lens) return fail(ctx, C4S_EINVAL, "attn: required pointer is NULL");
@@ -161,8 +165,7 @@ int check_attn(c4s_ctx* ctx, const c4s_kv_cache* c, const c4s_attn_desc* a) {
     return fail(ctx, C4S_EINVAL, "attn: rows of q must start on 16 bytes, rows of out on 8");
   if (!a->rows_off && a->n_rows > c->n_seqs) return fail(ctx, C4S_EINVAL, "attn: more rows than sequences without rows_off");
   if (!(a->scale - a->scale == 0.0f)) return fail(ctx, C4S_EINVAL, "attn: scale is not finite");
-  if (a->max_new > a->n_rows || (int64_t)a->max_new * a->n_heads > 1 << 29)
-    return fail(ctx, C4S_EINVAL, "attn: max_new above n_rows, or max_new * n_heads above 536870912");
+  if ((int64_t)new_rows(a) * a->n_heads > 1 << 29) return fail(ctx, C4S_EINVAL, "attn: max_new * n_heads above 536870912");
   return C4S_OK;
 }
 
@@ -211,7 +214,7 @@ int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_kv_rows* rows
 int c4s_attn(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_attn_desc* attn, void* stream) {
   return entry(ctx, cache && attn ? cache : nullptr, "attn", [&] {
     const int rc = check_attn(ctx, cache, attn);
-    if (rc || attn->n_rows == 0 || attn->max_new == 0 || cache->n_seqs == 0) return rc;
+    if (rc || attn->n_rows == 0 || new_rows(attn) == 0 || cache->n_seqs == 0) return rc;
     c4s::AttnArgs a{};
     a.c = to_args(cache);
     a.q = attn->q;
@@ -223,7 +226,7 @@ int c4s_attn(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_attn_desc* attn,
     a.off = attn->rows_off;
     a.first = attn->first;
     a.n_rows = attn->n_rows;
-    a.max_new = attn->rows_off ? attn->max_new : 1;
+    a.max_new = new_rows(attn);
     a.n_heads = attn->n_heads;
     a.shared = attn->n_heads / cache->n_kv_heads;
     a.scale = attn->scale;

@@ -1,0 +1,45 @@
+"""Calls of the decoder layer's operators that once gave something else than their contract (include/c4s_layers.h)."""
+import pytest
+import torch
+
+import c4s
+import layers_util as L
+
+pytestmark = pytest.mark.gpu
+
+
+def _attn_raw(ctx, cache, lens, q, out, lse, off, n_rows, max_new, scale=0.125):
+    """c4s_attn with every field as given."""
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    heads, dim = q.shape[1:]
+    desc = c4s._pack_attn(p(q), heads * dim, p(out), heads * dim, p(lse), p(lens), p(off), 0, n_rows, max_new, heads, scale)
+    return c4s.lib().c4s_attn(ctx._h, cache.packed, desc, torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("max_new", [0, -1, 1, 9, 2 ** 31 - 1])
+def test_attn_without_offsets_has_one_row_a_sequence(gpu_ctx, max_new):
+    """max_new means nothing without rows_off: a descriptor that leaves it zero computes all its rows."""
+    cache = L.Cache([70, 3, 200], 2, 64, 16, False, seed=1)
+    kc, lens = cache.cuda(), torch.tensor(cache.lens, dtype=torch.int32).cuda()
+    q = L.bf16((3, 4, 64), torch.Generator().manual_seed(2)).cuda()
+    out, lse = torch.full_like(q, 7.0), torch.full((3, 4), 7.0, device="cuda")
+    assert _attn_raw(gpu_ctx, kc, lens, q, out, lse, None, 3, max_new) == c4s.OK
+    want, wlse = torch.empty_like(q), torch.empty_like(lse)
+    gpu_ctx.attn(q, kc, lens, want, max_new=1, lse=wlse)
+    assert torch.equal(out, want) and torch.equal(lse, wlse) and (out != 7).any()
+
+
+def test_attn_with_offsets_and_a_generous_max_new(gpu_ctx):
+    """max_new above the rows there are says no more than their number."""
+    cache = L.Cache([70, 40], 2, 64, 16, False, seed=1)
+    kc, lens = cache.cuda(), torch.tensor(cache.lens, dtype=torch.int32).cuda()
+    off = torch.tensor([0, 2, 5], dtype=torch.int32).cuda()
+    q = L.bf16((5, 4, 64), torch.Generator().manual_seed(2)).cuda()
+    want, got = torch.empty_like(q), torch.full_like(q, 7.0)
+    gpu_ctx.attn(q, kc, lens, want, rows_off=off, max_new=5)
+    for max_new in (6, 64, 2 ** 31 - 1):
+        assert _attn_raw(gpu_ctx, kc, lens, q, got, None, off, 5, max_new) == c4s.OK
+        assert torch.equal(got, want)
+    assert _attn_raw(gpu_ctx, kc, lens, q, got.fill_(7.0), None, off, 5, 0) == c4s.OK
+    assert (got == 7).all()   # nothing is to be computed
+    assert _attn_raw(gpu_ctx, kc, lens, q, got, None, off, 5, -1) == c4s.EINVAL
