@@ -41,7 +41,7 @@ class Decoder:
     """One batch of sequences: begin(prompts), then step() for each further token.
 
     Sequences get their pages from one pool of `n_pages` when the batch begins,
-    for as many tokens as it may come to hold."""
+    for as many tokens as it may come to hold: `room` further steps are left."""
 
     def __init__(self, ctx: c4s.Context, weights: dict, heads: int, kv_heads: int, n_pages: int, page_size: int = 16,
                  q8_cache: bool = False):
@@ -51,6 +51,7 @@ class Decoder:
         table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
         self.caches = [c4s.KvCache.empty(n_pages, kv_heads, page_size, self.hd, table, q8=q8_cache)
                        for _ in weights["layers"]]
+        self.room = 0
 
     def _buffers(self, rows: int) -> dict:
         e = lambda *s: torch.empty(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
@@ -71,11 +72,18 @@ class Decoder:
             ctx.linear(b["m"], w["down"], b["x"], bias=w["down_bias"], residual=b["x"])
 
     def begin(self, prompts: list, max_new: int) -> torch.Tensor:
-        """Prompts (lists of ids) into the caches; the last hidden row of each, bf16 [sequences][dim]."""
+        """Prompts (lists of ids) into the caches, with room for max_new further tokens each; the last hidden row of
+        each, bf16 [sequences][dim]."""
+        self.room = 0
         n = [len(p) for p in prompts]
+        if not n or max_new < 0:
+            raise ValueError("no prompts, or max_new below 0")
         need = [-(-(k + max_new) // self.page_size) for k in n]
         if min(n) < 1 or sum(need) > self.n_pages or max(n) + max_new > self.w["positions"].shape[0]:
             raise ValueError("empty prompt, or more tokens than pages or positions")
+        ids = torch.cat([torch.as_tensor(p) for p in prompts])
+        if int(ids.min()) < 0 or int(ids.max()) >= self.vocab:   # on the device an index out of range ends the process
+            raise ValueError("a prompt's id is outside the vocabulary")
         table = torch.full((len(n), max(need)), -1, dtype=torch.int32)
         at = 0
         for row, k in zip(table, need):
@@ -84,7 +92,7 @@ class Decoder:
         table = table.cuda()
         self.caches = [c4s.KvCache(c.k, c.v, table, c.k_scale, c.v_scale) for c in self.caches]
         self.lens = torch.tensor(n, dtype=torch.int32, device="cuda")
-        ids = torch.cat([torch.as_tensor(p) for p in prompts]).cuda()
+        ids = ids.cuda()
         pos = torch.cat([torch.arange(k) for k in n]).cuda()
         off = torch.zeros(len(n) + 1, dtype=torch.int32)
         off[1:] = torch.tensor(n).cumsum(0)
@@ -92,10 +100,15 @@ class Decoder:
         torch.add(self.w["tokens"][ids].float(), self.w["positions"][pos].float(), out=b["x"])
         self._layers(b, off.cuda(), max(n))
         self.one = self._buffers(len(n))   # a step's
+        self.room = max_new
         return b["x"][(off[1:] - 1).cuda().long()].bfloat16()
 
     def step(self, tokens) -> torch.Tensor:
-        """One more token a sequence (int32 or int64 [sequences]); its hidden row, bf16. May be captured into a graph."""
+        """One more token a sequence (int32 or int64 [sequences], ids of the vocabulary); its hidden row, bf16. May be
+        captured into a graph, whose replays are the caller's to count."""
+        if self.room < 1:
+            raise ValueError("no room for a further token: begin() gives as many steps as its max_new")
+        self.room -= 1
         b = self.one
         torch.add(self.w["tokens"][tokens].float(), self.w["positions"][self.lens].float(), out=b["x"])
         self.lens.add_(1)
@@ -105,6 +118,8 @@ class Decoder:
     def generate(self, prompts: list, max_new: int, temp, top_k, top_p, pen, rng, graph: bool = True) -> torch.Tensor:
         """max_new sampled tokens of each prompt, int32 [sequences][max_new]; rng (int64 [sequences]) is advanced.
         temp, top_k, top_p, pen: one value a sequence, on the device. graph: steps as replays of one graph."""
+        if max_new < 1:
+            raise ValueError("max_new below 1")
         R, w = len(prompts), self.w
         bits = torch.zeros((R, (self.vocab + 31) // 32), dtype=torch.int32, device="cuda")
         token = torch.empty(R, dtype=torch.int32, device="cuda")

@@ -43,3 +43,33 @@ def test_attn_with_offsets_and_a_generous_max_new(gpu_ctx):
     assert _attn_raw(gpu_ctx, kc, lens, q, got.fill_(7.0), None, off, 5, 0) == c4s.OK
     assert (got == 7).all()   # nothing is to be computed
     assert _attn_raw(gpu_ctx, kc, lens, q, got, None, off, 5, -1) == c4s.EINVAL
+
+
+def test_decoder_counts_its_room(gpu_ctx):
+    """A step past the pages and positions that begin() gave is refused on the host (its position would be an index
+    past the table of positions, which ends the process), and so is an id that is no token."""
+    import c4s_decode as D
+
+    w = D.random_weights(1, 128, 2, 1, 99, 20, seed=1)
+    d = D.Decoder(gpu_ctx, w, 2, 1, 8)
+    tokens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="room"):
+        d.step(tokens)
+    d.begin([[1, 2, 3], [4] * 18], 2)
+    for _ in range(2):
+        assert torch.isfinite(d.step(tokens)).all()
+    with pytest.raises(ValueError, match="room"):
+        d.step(tokens)
+    assert d.lens.tolist() == [5, 20]
+    for prompts, new in (([[1, 99]], 1), ([[-1, 3]], 1), ([], 1), ([[1]], -1)):
+        with pytest.raises(ValueError):
+            d.begin(prompts, new)
+        with pytest.raises(ValueError, match="room"):   # what began before is over
+            d.step(tokens)
+    one = lambda v, t: torch.full((1,), v, dtype=t, device="cuda")  # noqa: E731
+    par = (one(0.9, torch.float32), one(5, torch.int32), one(0.9, torch.float32), one(1.0, torch.float32))
+    with pytest.raises(ValueError):
+        d.generate([[1, 2]], 0, *par, one(1, torch.int64))
+    for n in (1, 2, 3, 18):   # up to the last position
+        out = d.generate([[1, 2]], n, *par, one(7, torch.int64))
+        assert out.shape == (1, n) and ((out >= 0) & (out < 99)).all()
