@@ -77,7 +77,8 @@ int c4s_block_norm(c4s_ctx* ctx, const c4s_norm* norm, void* stream);
  *
  * weight is stored (out, in) as nn.cpp:11-16 has it: bf16, or 8-bit codes with
  * w[n][k] = wscale[n][k / group] q[n][k] + wbias[n][k / group] (C4S_W_Q8, as in
- * c4s_head). C4S_ACT_GELU is the tanh form, y/2 (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))). out may
+ * c4s_head; a row of x with an infinite value gives NaN there, since codes and
+ * offsets are summed apart). C4S_ACT_GELU is the tanh form, y/2 (1 + tanh(sqrt(2/pi) (y + 0.044715 y^3))). out may
  * be residual itself when both have one type and stride.
  * K must be a multiple of 8, and of group for 8-bit codes; x, weight and ldx
  * such that every row starts on 16 bytes (8-bit codes: 8); else C4S_EINVAL. */

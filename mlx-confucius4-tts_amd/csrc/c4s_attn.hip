@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   const float c2 = a.scale * kLog2e;
   constexpr int kSize = Q8 ? 1 : 2;
   const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;   // below 2^31
-  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head + (Q8 ? 16 : 16) * g + (c % 4) * dim * kSize;
+  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head + 16 * g + (c % 4) * dim * kSize;
   const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head + (uint64_t)(uint32_t)((c * kSize) << shift);
   const uint32_t scale_bytes = 4u * (uint32_t)a.c.n_heads << shift;
   const uint32_t tile_bytes = (16u * kSize) << shift;
@@ -291,10 +291,11 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       for (int j = 0; j < kOwn; ++j) p[j] = s[j / 4][j % 4] * (Q8 ? c2 * ks[j] : c2);
       const bool there = now.v >= 0;
       const bool edge = t < fst || t + KEYS > min(least, end) || __any(!there);
+      const int from = max(fst - vt, 0), to = there ? min(lim, end) - vt : 0;
+      auto sees = [&](int j) { return (j >= from) & (j < to); };   // whether this row sees position vt + j
       if (edge) {
-        const int from = max(fst - vt, 0), to = there ? min(lim, end) - vt : 0;
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) p[j] = ((j >= from) & (j < to)) ? p[j] : -__builtin_inff();
+        for (int j = 0; j < kOwn; ++j) p[j] = sees(j) ? p[j] : -__builtin_inff();
       }
       __builtin_amdgcn_sched_barrier(0);
       // The next block's loads; behind the last block that one's again, whose lines are near (a branch around
@@ -314,14 +315,20 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       l *= old;
 #pragma unroll
       for (int d = 0; d < kTiles; ++d) o[d] *= old;
+      if constexpr (Q8) {
+        if (edge) {   // what is masked may have any scale; what is seen has its own, also at a weight of 0
+#pragma unroll
+          for (int j = 0; j < kOwn; ++j) vs[j] = sees(j) ? vs[j] : 0.0f;
+        }
+      }
       uint32_t hi[kOwn / 2], lo[kOwn / 2];
 #pragma unroll
       for (int j = 0; j < kOwn; j += 2) {
         float x = __builtin_amdgcn_exp2f(p[j] - base), y = __builtin_amdgcn_exp2f(p[j + 1] - base);
         l += x + y;
-        if constexpr (Q8) {   // 0 for a masked position, whatever its scale
-          x = x != 0.0f ? x * vs[j] : 0.0f;
-          y = y != 0.0f ? y * vs[j + 1] : 0.0f;
+        if constexpr (Q8) {
+          x *= vs[j];
+          y *= vs[j + 1];
         }
         hi[j / 2] = pack(x, y);
         lo[j / 2] = pack(x - low(hi[j / 2]), y - high(hi[j / 2]));
@@ -332,15 +339,18 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
         if (edge) {
           // What is not there or not for any row may hold anything: zeros. Where some of the rows see a
           // position and others do not, 0 times a value that is not finite would reach those: such
-          // values are taken out, and the rows that see them become NaN.
-          const int from = there ? fst - vt : kOwn, to = there ? min(kend, end) - vt : kOwn;
+          // values are taken out, and the rows that see them, at whatever weight, become NaN.
+          const int any_to = there ? min(kend, end) - vt : 0;
           int odd = 0;
 #pragma unroll
           for (int i = 0; i < kVLoads; ++i) {
-            vr[i] = keep(vr[i], 8 * (i % (KEYS / 32)), from, to);
+            vr[i] = keep(vr[i], 8 * (i % (KEYS / 32)), from, any_to);
             odd |= any_odd(vr[i]);
           }
           if (least != kend && __any(odd)) {
+            uint32_t mine[kOwn / 2];   // ones where this row sees
+#pragma unroll
+            for (int j = 0; j < kOwn; j += 2) mine[j / 2] = (sees(j) ? 0x3F80u : 0u) | (sees(j + 1) ? 0x3F800000u : 0u);
 #pragma unroll
             for (int d = 0; d < kTiles; ++d) {
               f32x4 seen = {};
@@ -352,7 +362,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
                 part_odd(v.y, ones.y);
                 part_odd(v.z, ones.z);
                 part_odd(v.w, ones.w);
-                seen = mfma(ones, quad(hi + 4 * st), seen);
+                seen = mfma(ones, quad(mine + 4 * st), seen);
               }
 #pragma unroll
               for (int i = 0; i < 4; ++i)

@@ -73,3 +73,40 @@ def test_decoder_counts_its_room(gpu_ctx):
     for n in (1, 2, 3, 18):   # up to the last position
         out = d.generate([[1, 2]], n, *par, one(7, torch.int64))
         assert out.shape == (1, n) and ((out >= 0) & (out < 99)).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("new,length,at", [
+    (1, 300, 70), (1, 300, 290), (1, 33, 32), (1, 300, 0),     # single tokens: inside, in the last block, alone in it
+    (5, 300, 70), (5, 300, 297), (5, 300, 295), (16, 300, 290),  # seen by some of the rows only, or by all
+    (100, 300, 250), (1500, 1600, 800)])                       # prompts in either kernel
+def test_values_that_are_not_finite_at_a_weight_of_zero(gpu_ctx, new, length, at, q8):
+    """A seen position whose weight underflows still has a value: one that is not finite makes the rows that see it
+    inf or NaN (0 times such a value), the other rows stay as they are."""
+    heads, dim, page = 20 if new > 1000 else 2, 64, 16
+    caches = [L.Cache([length], heads, dim, page, q8, seed=9) for _ in range(2)]
+    for cache, bad in zip(caches, (True, False)):
+        pg, place = int(cache.table[0, at // page]), at % page
+        for name in cache.t:   # scores of every other position 0, of this one -512
+            if name.startswith("k"):
+                cache.t[name] = torch.zeros_like(cache.t[name])
+        cache.t["k"][pg, :, place] = -127 if q8 else -8
+        if q8:
+            cache.t["k_scale"][pg, :, place] = 8 / 127
+            if bad:
+                cache.t["v_scale"][pg, :, place] = float("nan")
+        elif bad:
+            cache.t["v"][pg, :, 5, place] = float("inf")
+            cache.t["v"][pg, :, 40, place] = float("nan")
+    lens, off = torch.tensor([length], dtype=torch.int32).cuda(), torch.tensor([0, new], dtype=torch.int32).cuda()
+    q = torch.ones((new, heads, dim), dtype=torch.bfloat16, device="cuda")
+    got, want = torch.empty_like(q), torch.empty_like(q)
+    for cache, out in zip(caches, (got, want)):
+        gpu_ctx.attn(q, cache.cuda(), lens, out, rows_off=off, max_new=new, scale=1.0)
+    assert torch.isfinite(want).all()
+    sees = torch.arange(length - new, length, device="cuda") >= at
+    odd = torch.ones(dim, dtype=torch.bool, device="cuda") if q8 else torch.zeros(dim, dtype=torch.bool, device="cuda")
+    odd[5] = odd[40] = True
+    assert not torch.isfinite(got[sees][:, :, odd]).any()
+    assert torch.equal(got[sees][:, :, ~odd], want[sees][:, :, ~odd])
+    assert torch.equal(got[~sees], want[~sees])
