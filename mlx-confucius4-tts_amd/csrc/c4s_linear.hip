@@ -637,8 +637,15 @@ int64_t tiles_of(const c4s_linear_desc& a, int m, int n) {
 // from 1280 of them on the others win (us, bf16, K = 1280, N = 5120: 512 rows 19
 // and 21, 640 rows 23 and 21, 1024 rows 31 and 24; K = 5120, N = 1280: 2000 rows 59
 // and 59; 8-bit, N = 5120: 512 rows 31 and 39, 800 rows 46 and 45).
+// With outputs so many that a single tile of rows exceeds that, the others' tiles are mostly rows
+// that are not there. 8-bit codes cost them their conversion all the same, so up to 64 rows stay here (N = 151936,
+// few / many, us: K = 1280: 1 row 58 / 110, 16 68 / 111, 64 107 / 116; K = 4096: 221 / 341, 247 / 344, 324 / 352). With
+// bf16, weights are all that counts: here as far as x is small beside them, and while rows are not 8 KB apart
+// or more, which whole stages take better (1 row: N = 151936, K = 1280 64 / 82, 3200 168 / 188, 4096 234 / 235; N =
+// 70000, K = 2560 61 / 95; 16 rows: 76 / 84, 183 / 189, 255 / 238; 71 / 97; 48 rows: 97 / 95, 231 / 196).
 bool few_pays(const c4s_linear_desc& a) {
-  return tiles_of(a, kFewM, kFewN) <= (a.wdtype == C4S_W_Q8 ? 1600 : 1280);
+  if (a.wdtype == C4S_W_Q8) return a.M <= kFewM || tiles_of(a, kFewM, kFewN) <= 1600;
+  return (a.M <= 16 && a.K < 4096) || tiles_of(a, kFewM, kFewN) <= 1280;
 }
 
 // 128 x 128, two workgroups a CU, or 256 x 256: a round of the chip with the former

@@ -110,3 +110,28 @@ def test_values_that_are_not_finite_at_a_weight_of_zero(gpu_ctx, new, length, at
     assert not torch.isfinite(got[sees][:, :, odd]).any()
     assert torch.equal(got[sees][:, :, ~odd], want[sees][:, :, ~odd])
     assert torch.equal(got[~sees], want[~sees])
+
+
+@pytest.mark.parametrize("M,N,K,group", [
+    # few rows by outputs just above what the few rows' kernel took before by its count of tiles, and at it
+    (1, 40960, 64, 0), (1, 40961, 64, 0), (16, 41000, 136, 0), (17, 41000, 136, 0), (64, 41003, 64, 0),
+    (1, 41000, 4096, 0), (16, 41000, 4104, 0),
+    (1, 51200, 64, 32), (1, 51201, 64, 64), (64, 51300, 128, 128), (65, 51300, 64, 32), (33, 60001, 96, 32)])
+def test_linear_of_few_rows_and_many_outputs(gpu_ctx, M, N, K, group):
+    print(f"linear {M}x{N}x{K} group={group}", flush=True)
+    g = torch.Generator().manual_seed(M + N)
+    x = L.bf16((M, K), g)
+    quant = None
+    if group:
+        w = torch.randint(0, 256, (N, K), generator=g, dtype=torch.uint8)
+        quant = (torch.rand((N, K // group), generator=g) * 0.02, torch.randn((N, K // group), generator=g), group)
+    else:
+        w = L.bf16((N, K), g)
+    bias = torch.randn(N, generator=g)
+    res = torch.randn((M, N), generator=g)
+    want, err = L.linear(x, w, quant, bias, "silu", res)
+    out = torch.empty((M, N), device="cuda")
+    gpu_ctx.linear(x.cuda(), w.cuda(), out, bias=bias.cuda(), residual=res.cuda(), act="silu",
+                   quant=None if quant is None else (quant[0].cuda(), quant[1].cuda(), group))
+    bad = ~((L.f64(out) - want).abs() <= err)
+    assert not bad.any(), f"{int(bad.sum())} off, first at {bad.nonzero()[0].tolist()}"
