@@ -277,10 +277,19 @@ __global__ __launch_bounds__(64 * W, W == 4 ? 2 : 1) void k_linear_few(FewArgs f
   FewChunk<Q8, MB> r;
   int ch = c0 + wave;
   if (ch < c1) load(r, ch);
+  // Lanes of the wave read what others wrote: order that the compiler keeps (it costs no instruction; LDS serves a
+  // wave's accesses in order).
+  auto wave_order = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
   for (; ch < c1; ch += W) {
     stage(r, ch);
+    wave_order();
     if (ch + W < c1) load(r, ch + W);
     compute();
+    wave_order();
   }
 
   // the waves' sums
