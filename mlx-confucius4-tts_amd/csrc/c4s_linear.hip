@@ -496,8 +496,10 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM == 8 ? 1 : 2) void k_linear_m
       const uint32_t at = 16 * ((lane % 8) ^ (((r + lane / 8) >> 1) & 7));
       const bool in = (uint32_t)(st * 128) + at < wp;   // behind the last input: past the buffers' ends, where loads give zeros
       const uint32_t v = (isx ? (r + lane / 8) * xp : (r - kM + lane / 8) * wp) + at;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(dst + 1024u * j), "v"(in ? v + 128u * st : 0x80000000u), "s"(isx ? xt.d : wt.d) : "memory");
+      // (m0, which says where in LDS, is the compiler's and cannot be named as clobbered: it is left as it was)
+      uint32_t m0_was;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                   : "=&s"(m0_was) : "s"(dst + 1024u * j), "v"(in ? v + 128u * st : 0x80000000u), "s"(isx ? xt.d : wt.d) : "memory");
     }
   };
   const int wn = wave % WN * 16 * NW, wm = wave / WN * 16 * MW;
