@@ -17,6 +17,9 @@
  * call that fails its checks queues nothing. A call with no rows queues nothing
  * and returns C4S_OK. All of them may be captured into a graph (c4s_attn and
  * c4s_linear with a workspace: after a call of that size outside a capture).
+ * Graphs captured on one stream share those calls' workspace, so their replays
+ * must not overlap, as c4s_sampling.h says of its own; here an overlap also
+ * leaves counters in the workspace off zero, and later replays are wrong too.
  *
  * Activations are bf16, the residual stream bf16 or fp32; sums, softmax
  * statistics and norms are fp32. Row strides are in elements.

@@ -604,8 +604,9 @@ class Context:
 
     def attn(self, q, cache, lens, out, rows_off=None, max_new=None, scale=None, first=None, lse=None, stream=None):
         """Attention of the rows q (bfloat16 [rows][n_heads][head_dim], the last
-        positions of lens[b]) over the cache, into out. max_new: the most rows a
-        sequence has (default: all rows); scale: 1 / sqrt(head_dim) by default."""
+        positions of lens[b]) over the cache, into out. max_new: with rows_off the most
+        rows a sequence has, by which the kernel is chosen (default: all rows); scale:
+        1 / sqrt(head_dim) by default."""
         shape, dev = q.shape, self.device
         rows, heads, dim = shape
         qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous", dev)
