@@ -533,12 +533,21 @@ hipError_t few(const FewArgs& f, hipStream_t s) {
 // wave's last row are skipped by it, masks are applied only where a block
 // holds the limit of some row, and the tiles with the most positions start
 // first, those of up to 64 sequences together (of one after the other: 8 of 2048,
-// 20 heads of 64, 169 us for 152; 4 of 2000, 5 heads of 256 195 for 172).
+// 20 heads of 64, 169 us for 152; 4 of 2000, 10 query heads on 5 of 256, 195 for 172).
+//
+// What bounds it (20 heads of 64, 12 prompts of 500 to 2100): the VALU, 63 % busy;
+// the matrix engine is 22 %, LDS 35 % (a tenth of it bank conflicts). Heads of 256
+// have two waves a SIMD, which wait 60 % of the time, with LDS at 35, VALU at 29 and
+// matrix engine at 23 %; the compiler spills 18 registers of theirs, and 10 of those of
+// 8-bit heads of 64.
 //
 // Weights for bf16 values enter the second product rounded to bf16 once:
 // independent roundings of 2^-9 at most, which leave 1.15 to 1.4 times the error of
-// the output's own rounding (the largest weight is often 1, which has none); as
-// pairs, as with few rows, they would cost half as many matrix instructions again.
+// the output's own rounding (the largest weight is often 1, which has none). As
+// pairs, as with few rows, they would add nothing to it, for half as many matrix instructions
+// again and the VALU's splitting (pairs / once, us: 8 of 2048, 20 heads of 64 194 / 157;
+// 2 of 4096, 32 query heads on 8 of 128 441 / 338; 4 of 2000, 5 heads of 256 125 / 105;
+// 64 of 20 to 100 21.5 / 19).
 // Weights for codes have the values' scales in them, none is exact, and the error
 // would come to 1.5 times: those enter as pairs (8 prompts of 2048, 20 heads of 64:
 // 224 us for 185, 1.0 times). The weights' sum is taken before the rounding, in fp32

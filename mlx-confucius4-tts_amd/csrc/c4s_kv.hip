@@ -10,10 +10,13 @@
 // The heads of a tile follow each other in the grid: a row's 128 bytes a head
 // are then read and written next to each other in time.
 //
-// Memory bounds both for prompts, reads nearly (24 prompts of 70 to 1500 tokens, 20
-// heads of 64, 8-bit: 224 MB in 41 us, 5.5 TB/s), writes less so (151 MB in 52 us:
-// the pages' rows that a tile's ends leave half full, and about half the time in
-// which the codes are computed, add to it).
+// Memory bounds both for prompts, and both move more than they need. 24 prompts of
+// 70 to 1500 tokens, 20 heads of 64, 8-bit, calls back to back: the read needs 179 MB
+// (62 of codes and scales, 117 of rows) and takes 41 us, 4.4 TB/s, in which 93 and
+// 159 MB pass, 6.1 TB/s; the write needs 148 MB (96 of rows, 51 of codes and scales)
+// and takes 51 us, 2.9 TB/s, in which 97 and 65 MB pass. What the write adds are the
+// lines of pages that a tile's ends leave half full; the VALU, which computes the
+// codes, is busy half of the time, and which of the two costs more is not known.
 
 #include <hip/hip_runtime.h>
 

@@ -466,9 +466,9 @@ __device__ __forceinline__ void write_tile(const ManyArgs& f, int m, int n, cons
 // fragments are double buffered in registers too: while one half of a stage is
 // multiplied, the next half's are read, so that the matrix engine waits only for
 // the other waves at the barrier, once a stage. Eight waves on 256 x 256 reach
-// 1265 TFLOP/s at 8192 x 8192 x 8192 (the rows in registers on the way and two
-// barriers a stage: 1030; stages of 32 inputs, four buffers: 1190; 128 x 128
-// and two workgroups a CU: 1060).
+// 1330 TFLOP/s at 8192 x 8192 x 8192 (1265 when the others were tried: the rows in
+// registers on the way and two barriers a stage 1030; stages of 32 inputs, four
+// buffers 1190; 128 x 128 and two workgroups a CU 1060).
 template <int NW, int MW, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM, WN * WM == 8 ? 1 : 2) void k_linear_many(ManyArgs f) {
   constexpr int kN = 16 * NW * WN, kM = 16 * MW * WM, kWaves = WN * WM, kStage = (kN + kM) * 128;
@@ -540,7 +540,10 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM == 8 ? 1 : 2) void k_linear_m
 
 // 8-bit codes: 128 x 128, four waves, two workgroups a CU. The codes pass through
 // registers on their way into LDS, where they become q - 128; a chunk's products
-// are scaled and added to the sums in fp32, as with few rows.
+// are scaled and added to the sums in fp32, as with few rows. 12345 x 5120 x 1280, group
+// 64: 325 us, 500 TFLOP/s (bf16 weights: 165). One buffer and two barriers a chunk, between
+// which nothing is multiplied; VALU 58 % busy with conversion and scaling, matrix engine 26 %,
+// a fifth of that the sums of x, LDS 32 %.
 __global__ __launch_bounds__(256, 2) void k_linear_many_q8(ManyArgs f) {
   constexpr int NW = 4, MW = 4, WN = 2, WM = 2, kN = 16 * NW * WN, kM = 16 * MW * WM;
   constexpr int kXLoads = kM / 32, kWLoads = kN / 64;
