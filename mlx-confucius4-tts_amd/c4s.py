@@ -294,23 +294,23 @@ def _i32(t, n, what, device):
     _refuse(t, what, device)
 
 
-def _rows(t, shape, what, device):
-    """(address, row stride, C4S_DTYPE_*) of a [rows][width] tensor of this shape on this device,
-    bfloat16 or float32, whose rows are contiguous; (0, 0, F32) of None."""
+def _rows(t, shape, what, device, own=False):
+    """(address, row stride, C4S_DTYPE_*) of a [rows][width] tensor of this shape (own: which is its own) on this
+    device, bfloat16 or float32, whose rows are contiguous; (0, 0, F32) of None."""
     if t is None:
         return 0, 0, F32
     kind = _Torch.kinds.get(t.dtype)
-    if kind is not None and t.shape == shape and t.get_device() == device:
+    if kind is not None and t.get_device() == device and (own or t.shape == shape):
         ld, one = t.stride()
         if one == 1 or shape[1] <= 1:
             return t.data_ptr(), (ld if shape[0] > 1 else shape[1]), kind
     _refuse(t, what, device)
 
 
-def _heads(t, shape, what, device):
+def _heads(t, shape, what, device, own=False):
     """As _rows, of a [rows][heads][dim] tensor."""
     kind = _Torch.kinds.get(t.dtype)
-    if kind is not None and t.shape == shape and t.get_device() == device:
+    if kind is not None and t.get_device() == device and (own or t.shape == shape):
         ld, dim, one = t.stride()
         if one == 1 and (dim == shape[2] or shape[1] == 1):
             return t.data_ptr(), (ld if shape[0] > 1 else shape[1] * shape[2]), kind
@@ -519,7 +519,7 @@ class Context:
         float32 [ceil(rows / gate_rows)][D]; without y, r = x."""
         shape, dev = x.shape, self.device
         M, D = shape
-        xp, ldx, xt = _rows(x, shape, "block_norm: x must be bfloat16 or float32, its rows contiguous", dev)
+        xp, ldx, xt = _rows(x, shape, "block_norm: x must be bfloat16 or float32, its rows contiguous", dev, True)
         yp, ldy, yt = _rows(y, shape, "block_norm: y must be bfloat16 or float32 of x's shape, its rows contiguous", dev)
         op, ldo, ot = _rows(out, shape, "block_norm: out must be bfloat16 or float32 of x's shape, its rows contiguous", dev)
         xo = ldxo = g = ldg = 0
@@ -549,7 +549,7 @@ class Context:
         xs, ws, dev = x.shape, weight.shape, self.device
         M, K = xs
         N = ws[0]
-        xp, ldx, t = _rows(x, xs, "linear: x must be bfloat16 [M][K], its rows contiguous", dev)
+        xp, ldx, t = _rows(x, xs, "linear: x must be bfloat16 [M][K], its rows contiguous", dev, True)
         if not (t == BF16 and ws == (N, K) and weight.is_contiguous() and weight.get_device() == dev):
             _refuse(weight, "linear: x must be bfloat16 [M][K], weight contiguous [N][K]", dev)
         sp = bp = group = 0
@@ -579,9 +579,9 @@ class Context:
     def _kv_rows(self, cache, k, v, lens, rows_off):
         shape, dev = k.shape, self.device
         rows, heads, dim = shape
-        _need(cache.device == dev, "kv rows: the cache is not on the context's device")
-        _need(heads == cache.n_kv_heads and dim == cache.head_dim, "kv rows: k must be [rows][n_kv_heads][head_dim]")
-        kp, ldk, t = _heads(k, shape, "kv rows: k must be bfloat16 or float32, a row contiguous", dev)
+        if not (heads == cache.n_kv_heads and dim == cache.head_dim and cache.device == dev):
+            raise ValueError(f"kv rows: k must be [rows][n_kv_heads][head_dim], the cache on the context's device, cuda:{dev}")
+        kp, ldk, t = _heads(k, shape, "kv rows: k must be bfloat16 or float32, a row contiguous", dev, True)
         vp, ldv, vt = _heads(v, shape, "kv rows: v must have k's shape and dtype, a row contiguous", dev)
         _need(vt == t, "kv rows: k and v must have one dtype")
         n = cache.n_seqs
@@ -609,11 +609,11 @@ class Context:
         1 / sqrt(head_dim) by default."""
         shape, dev = q.shape, self.device
         rows, heads, dim = shape
-        qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous", dev)
+        qp, ldq, qt = _heads(q, shape, "attn: q must be bfloat16 [rows][n_heads][head_dim], a row contiguous", dev, True)
         op, ldo, ot = _heads(out, shape, "attn: out must be bfloat16 of q's shape, a row contiguous", dev)
-        _need(cache.device == dev, "attn: the cache is not on the context's device")
-        _need(qt == BF16 and ot == BF16 and dim == cache.head_dim,
-              "attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's")
+        if not (qt == BF16 and ot == BF16 and dim == cache.head_dim and cache.device == dev):
+            raise ValueError("attn: q and out must be bfloat16 [rows][n_heads][head_dim], head_dim as the cache's, "
+                             f"the cache on the context's device, cuda:{dev}")
         n = cache.n_seqs
         rc = _lib.c4s_attn(
             self._h, cache.packed,
