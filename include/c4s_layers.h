@@ -5,7 +5,7 @@
  *
  *   c4s_block_norm   the block's output joins the residual stream, the norm in front of the next block
  *   c4s_linear       queries, keys and values (bias)
- *   c4s_kv_append    keys and values into the paged cache, as bf16 or 8-bit codes
+ *   c4s_kv_append    keys and values into the paged cache, as bf16 or 8- or 4-bit codes
  *   c4s_attn         the new tokens over the cache
  *   c4s_linear       onto the residual stream (bias, residual); into the MLP (bias, activation); out of it
  *
@@ -130,13 +130,13 @@ int c4s_linear(c4s_ctx* ctx, const c4s_linear_desc* lin, void* stream);
  * are the rows of sequence b's last tokens, the positions lens[b] - n .. lens[b] - 1
  * with n the number of rows (rows_off NULL: one row a sequence, row b). lens
  * counts the new tokens. */
-enum { C4S_KV_BF16 = 0, C4S_KV_Q8 = 1 };
+enum { C4S_KV_BF16 = 0, C4S_KV_Q8 = 1, C4S_KV_Q4 = 2 };
 
 typedef struct c4s_kv_cache {
   void* k;
   void* v;                      /* both 16-byte aligned */
-  float* k_scale;               /* C4S_KV_Q8, 16-byte aligned */
-  float* v_scale;
+  void* k_scale;                /* float (C4S_KV_Q8) or uint8_t (C4S_KV_Q4), 16-byte aligned */
+  void* v_scale;
   const int32_t* block_table;   /* [n_seqs][table_ld] */
   int64_t table_ld;
   int32_t n_seqs;               /* up to 65535 */
@@ -144,7 +144,7 @@ typedef struct c4s_kv_cache {
   int32_t n_pages;
   int32_t page_size;            /* 16, 32, 64, 128 or 256 */
   int32_t n_kv_heads;           /* n_kv_heads * page_size * head_dim up to 536870912 */
-  int32_t head_dim;             /* a multiple of 16, 16 .. 256 */
+  int32_t head_dim;             /* a multiple of 16 (C4S_KV_Q4: 32) up to 256 */
   int32_t store;                /* C4S_KV_* */
 } c4s_kv_cache;
 

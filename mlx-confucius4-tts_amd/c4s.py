@@ -1,5 +1,5 @@
-"""Python binding of libc4s_sampling.so (C ABI in include/c4s_sampling.h and,
-for the decoder layer's operators, include/c4s_layers.h).
+"""Python binding of libc4s_sampling.so (C ABI in include/c4s_sampling.h, for the
+decoder layer's operators include/c4s_layers.h, for a batch's include/c4s_batch.h).
 
 ctypes only; torch supplies device memory and streams, nothing else. Loading
 fails loudly when the library has not been built or no gfx950 device is
@@ -19,6 +19,7 @@ REPO = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "lib", "libc4s_sampling.so")
 HEADER = os.path.join(REPO, "include", "c4s_sampling.h")
 LAYERS_HEADER = os.path.join(REPO, "include", "c4s_layers.h")
+BATCH_HEADER = os.path.join(REPO, "include", "c4s_batch.h")
 
 OK, EINVAL, EHIP, ENOMEM, ETIMEOUT = 0, 1, 2, 3, 4
 F32, BF16 = 0, 1
@@ -32,7 +33,8 @@ STREAM_NO_SPECULATION = 2
 W_BF16, W_F32, W_Q8 = 0, 1, 2   # c4s_head.wdtype, c4s_linear_desc.wdtype
 NORM_LAYER, NORM_RMS = 0, 1
 ACTS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3}   # c4s_linear_desc.act
-KV_BF16, KV_Q8 = 0, 1
+KV_BF16, KV_Q8, KV_Q4 = 0, 1, 2
+ROPE_HALF, ROPE_PAIRS = 0, 1
 
 _vp = C.c_void_p
 
@@ -101,6 +103,40 @@ class Attn(C.Structure):
                 ("n_heads", C.c_int32), ("scale", C.c_float)]
 
 
+class Rope(C.Structure):
+    _fields_ = [("q", _vp), ("q_out", _vp), ("k", _vp), ("k_out", _vp), ("ldq", C.c_int64), ("ldq_out", C.c_int64),
+                ("ldk", C.c_int64), ("ldk_out", C.c_int64), ("freq", _vp), ("pos", _vp), ("lens", _vp),
+                ("rows_off", _vp), ("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("n_heads", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32),
+                ("dtype", C.c_int32), ("scale", C.c_float)]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [("block_table", _vp), ("table_ld", C.c_int64), ("lens", _vp), ("refs", _vp), ("free_bits", _vp),
+                ("missing", _vp), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32)]
+
+
+class Grow(C.Structure):
+    _fields_ = [("n_new", _vp), ("rows_off", _vp), ("row_pos", _vp), ("row_slot", _vp), ("copies", _vp),
+                ("n_rows", C.c_int32)]
+
+
+BEAM_STATES = 8
+
+
+class BeamState(C.Structure):
+    _fields_ = [("src", _vp), ("dst", _vp), ("ld_src", C.c_int64), ("ld_dst", C.c_int64), ("words", C.c_int64)]
+
+
+class Beam(C.Structure):
+    _fields_ = [("logits", _vp), ("ld", C.c_int64), ("dtype", C.c_int32), ("n_groups", C.c_int32),
+                ("width", C.c_int32), ("vocab", C.c_int32), ("stop_token", C.c_int32), ("n_states", C.c_int32),
+                ("temperature", _vp), ("rep_penalty", _vp), ("hist_bits", _vp), ("out_hist_bits", _vp),
+                ("score", _vp), ("done", _vp), ("out_score", _vp), ("out_done", _vp), ("out_parent", _vp),
+                ("out_token", _vp), ("states", BeamState * BEAM_STATES)]
+
+
 def header_functions(header: str = HEADER) -> list[str]:
     """Names of every function a public header declares."""
     txt = open(header).read()
@@ -160,8 +196,13 @@ def lib() -> C.CDLL:
     L.c4s_weights_last_error.restype = C.c_char_p
     for f in (L.c4s_block_norm, L.c4s_linear):   # descriptors as bytes (_packer)
         f.argtypes = [_vp, C.c_char_p, _vp]
-    for f in (L.c4s_kv_append, L.c4s_kv_read, L.c4s_attn):
+    for f in (L.c4s_kv_append, L.c4s_kv_read, L.c4s_attn, L.c4s_pages_grow):
         f.argtypes = [_vp, C.c_char_p, C.c_char_p, _vp]
+    L.c4s_rope.argtypes = [_vp, C.c_char_p, _vp]
+    L.c4s_pages_trim.argtypes = [_vp, C.c_char_p, _vp, _vp]
+    L.c4s_pages_fork.argtypes = [_vp, C.c_char_p, _vp, C.c_int32, _vp]
+    L.c4s_kv_copy.argtypes = [_vp, C.c_char_p, _vp, C.c_int32, _vp]
+    L.c4s_beam_step.argtypes = [_vp, C.c_char_p, _vp]
     _lib = L
     return L
 
@@ -251,17 +292,27 @@ def _packer(cls):
 
 
 _pack_norm, _pack_linear, _pack_rows, _pack_attn = (_packer(c) for c in (Norm, Linear, KvRows, Attn))
+_pack_rope, _pack_grow = _packer(Rope), _packer(Grow)
+_pack_state = _packer(BeamState)
+
+
+class _BeamHead(C.Structure):   # a Beam's fields in front of its states
+    _fields_ = Beam._fields_[:-1]
+
+
+_pack_beam = _packer(_BeamHead)
+assert C.sizeof(_BeamHead) == Beam.states.offset
 
 
 class _Torch:
     """torch's dtypes and its current stream, from the first context on."""
-    kinds, bf16, f32, i32, u8, raw_stream = {}, None, None, None, None, None
+    kinds, bf16, f32, i32, u8, f64, raw_stream = {}, None, None, None, None, None, None
 
     @classmethod
     def load(cls):
         import torch
         cls.kinds = {torch.float32: F32, torch.bfloat16: BF16}
-        cls.bf16, cls.f32, cls.i32, cls.u8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+        cls.bf16, cls.f32, cls.i32, cls.u8, cls.f64 = torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.float64
         cls.raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -290,6 +341,15 @@ def _i32(t, n, what, device):
     if t is None:
         return 0
     if t.dtype is _Torch.i32 and t.numel() == n and t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
+    _refuse(t, what, device)
+
+
+def _words(t, n, kind, what, device):
+    """The address of a contiguous tensor of n values of this dtype on this device; 0 of None."""
+    if t is None:
+        return 0
+    if t.dtype is kind and t.numel() == n and t.is_contiguous() and t.get_device() == device:
         return t.data_ptr()
     _refuse(t, what, device)
 
@@ -325,20 +385,32 @@ class KvCache:
     k_scale, v_scale  [n_pages][n_kv_heads][page_size]       float32, with int8 codes
     block_table  [n_seqs][max_pages]                         int32, shared by the layers
 
+    In 4 bits, two dims a byte, all of it uint8:
+
+    k            [n_pages][n_kv_heads][page_size][head_dim / 2]
+    v            [n_pages][n_kv_heads][head_dim / 2][page_size]
+    k_scale, v_scale  [n_pages][n_kv_heads][head_dim / 32][page_size]
+
     The object keeps the tensors and their addresses; their contents may change
     at any time."""
 
     def __init__(self, k, v, block_table, k_scale=None, v_scale=None):
         import torch
         _need(k.dim() == 4 and k.is_contiguous() and v.is_contiguous(), "KvCache: k and v must be contiguous, 4-d")
-        pages, heads, size, dim = k.shape
-        _need(tuple(v.shape) == (pages, heads, dim, size), "KvCache: v must be [n_pages][n_kv_heads][head_dim][page_size]")
-        _need(k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.int8), "KvCache: k and v must be bfloat16 or int8")
-        q8 = k.dtype == torch.int8
-        _need(q8 == (k_scale is not None) and q8 == (v_scale is not None), "KvCache: scales go with int8 codes")
+        pages, heads, size, width = k.shape
+        _need(tuple(v.shape) == (pages, heads, width, size),
+              "KvCache: v must be [n_pages][n_kv_heads][head_dim][page_size] (4 bits: [head_dim / 2])")
+        store = {torch.bfloat16: KV_BF16, torch.int8: KV_Q8, torch.uint8: KV_Q4}.get(k.dtype)
+        _need(k.dtype == v.dtype and store is not None, "KvCache: k and v must be bfloat16, int8 or (4 bits) uint8")
+        dim = 2 * width if store == KV_Q4 else width
+        _need((store != KV_BF16) == (k_scale is not None) and (store != KV_BF16) == (v_scale is not None),
+              "KvCache: scales go with codes")
+        kind, shape = ((torch.uint8, (pages, heads, dim // 32, size)) if store == KV_Q4 else
+                       (torch.float32, (pages, heads, size)))
         for s in (k_scale, v_scale):
-            _need(s is None or (s.dtype == torch.float32 and s.is_contiguous() and tuple(s.shape) == (pages, heads, size)),
-                  "KvCache: scales must be contiguous float32 [n_pages][n_kv_heads][page_size]")
+            _need(s is None or (s.dtype == kind and s.is_contiguous() and tuple(s.shape) == shape),
+                  "KvCache: scales must be contiguous float32 [n_pages][n_kv_heads][page_size], "
+                  "4 bits: uint8 [n_pages][n_kv_heads][head_dim / 32][page_size]")
         _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and
               (block_table.shape[1] <= 1 or block_table.stride(1) == 1), "KvCache: block_table must be int32 rows")
         self.device = k.get_device()
@@ -349,18 +421,86 @@ class KvCache:
         self.n_seqs, self.n_kv_heads, self.head_dim, self.page_size = n_seqs, heads, dim, size
         self.desc = KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), _p(block_table),
                                 block_table.stride(0) if n_seqs > 1 else max_pages, n_seqs, max_pages, pages, size,
-                                heads, dim, KV_Q8 if q8 else KV_BF16)
+                                heads, dim, store)
         self.packed = bytes(self.desc)
 
     @classmethod
-    def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, q8=False):
-        """A cache of its own on block_table's device; nothing in it is set."""
+    def empty(cls, n_pages, n_kv_heads, page_size, head_dim, block_table, q8=False, store=None):
+        """A cache of its own on block_table's device; nothing in it is set. store: "bf16", "q8" or "q4" (by default
+        what q8 says)."""
         import torch
-        t, d = torch.int8 if q8 else torch.bfloat16, block_table.device
-        k = torch.empty((n_pages, n_kv_heads, page_size, head_dim), dtype=t, device=d)
-        v = torch.empty((n_pages, n_kv_heads, head_dim, page_size), dtype=t, device=d)
-        scales = [torch.empty((n_pages, n_kv_heads, page_size), device=d) for _ in range(2)] if q8 else [None, None]
-        return cls(k, v, block_table, *scales)
+        store, d = store or ("q8" if q8 else "bf16"), block_table.device
+        _need(store in ("bf16", "q8", "q4") and (store != "q4" or head_dim % 32 == 0),
+              "KvCache: store must be bf16, q8 or q4, head_dim a multiple of 32 for q4")
+        e = lambda t, *s: torch.empty(s, dtype=t, device=d)  # noqa: E731
+        t, width = {"bf16": torch.bfloat16, "q8": torch.int8, "q4": torch.uint8}[store], head_dim // (2 if store == "q4" else 1)
+        k, v = e(t, n_pages, n_kv_heads, page_size, width), e(t, n_pages, n_kv_heads, width, page_size)
+        if store == "bf16":
+            return cls(k, v, block_table)
+        if store == "q8":
+            return cls(k, v, block_table, *(e(torch.float32, n_pages, n_kv_heads, page_size) for _ in "kv"))
+        return cls(k, v, block_table, *(e(torch.uint8, n_pages, n_kv_heads, head_dim // 32, page_size) for _ in "kv"))
+
+
+class Pages:
+    """Which sequence has which pages (c4s_pages in include/c4s_batch.h):
+
+    block_table  [n_seqs][max_pages]        int32, the caches' own; -1 behind a sequence's last page
+    lens         [n_seqs]                   int32
+    refs         [n_pages]                  int32, the sequences that hold a page
+    free_bits    [(n_pages + 31) // 32]     int32, bit p % 32 of word p // 32: page p is free
+    missing      [1]                        int32 or None, pages that were asked for in vain
+
+    The object keeps the tensors and their addresses; their contents are the calls'."""
+
+    def __init__(self, block_table, lens, refs, free_bits, page_size, missing=None):
+        import torch
+        _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and
+              (block_table.shape[1] <= 1 or block_table.stride(1) == 1), "Pages: block_table must be int32 rows")
+        n_seqs, max_pages = block_table.shape
+        self.device = block_table.get_device()
+        _need(self.device >= 0, "Pages: all tensors must be on one GPU")
+        n_pages = refs.numel()
+        vector = lambda t, n, name: _words(t, n, torch.int32, f"Pages: {name} must be an int32 vector", self.device)  # noqa: E731
+        self.block_table, self.lens, self.refs, self.free_bits, self.missing = block_table, lens, refs, free_bits, missing
+        self.n_seqs, self.max_pages, self.n_pages, self.page_size = n_seqs, max_pages, n_pages, page_size
+        self.desc = PagesDesc(_p(block_table), block_table.stride(0) if n_seqs > 1 else max_pages,
+                              vector(lens, n_seqs, "lens"), vector(refs, n_pages, "refs"),
+                              vector(free_bits, (n_pages + 31) // 32, "free_bits"), vector(missing, 1, "missing"),
+                              n_seqs, max_pages, n_pages, page_size)
+        self.packed = bytes(self.desc)
+
+    @classmethod
+    def empty(cls, n_seqs, max_pages, n_pages, page_size, device="cuda"):
+        """Sequences without tokens, every page free."""
+        import torch
+        full = lambda s, v: torch.full(s, v, dtype=torch.int32, device=device)  # noqa: E731
+        bits = full(((n_pages + 31) // 32,), -1)
+        if n_pages % 32:
+            bits[-1:].fill_((1 << n_pages % 32) - 1)
+        return cls(full((n_seqs, max_pages), -1), full((n_seqs,), 0), full((n_pages,), 0), bits, page_size, full((1,), 0))
+
+
+def rope_freqs(rot_dim, base=10000.0, factor=1.0, by="none", trained=0, slow=1.0, fast=4.0, device="cuda"):
+    """Frequencies for Context.rope, float64 [rot_dim / 2]: base^(-2 i / rot_dim), for contexts `factor` times as long as
+    trained with: by "linear", all divided by factor; "base", the base raised so that the slowest is; "parts", those
+    that turn less than `slow` times in `trained` positions divided, those that turn more than `fast` times kept, and
+    blended between."""
+    import math
+
+    import torch
+    _need(rot_dim >= 2 and rot_dim % 2 == 0 and base > 0 and factor > 0, "rope_freqs: rot_dim must be even, base and factor positive")
+    _need(by in ("none", "linear", "base", "parts"), "rope_freqs: by must be none, linear, base or parts")
+    if by == "base" and rot_dim > 2:
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = base ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    if by == "linear":
+        f = f / factor
+    if by == "parts":
+        _need(trained > 0 and fast > slow, "rope_freqs: parts need trained > 0 and fast > slow")
+        keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    return f.to(device)
 
 
 class Context:
@@ -626,6 +766,133 @@ class Context:
             self._queue(stream))
         if rc:
             self._check(rc, "attn")
+
+    # ---- the batch's operators (include/c4s_batch.h) ------------------------------------
+    def rope(self, q, k, freq, lens=None, rows_off=None, pos=None, q_out=None, k_out=None, pairs=False, scale=1.0,
+             stream=None):
+        """The first 2 * len(freq) dims of every head of q and k ([rows][heads][head_dim], bfloat16 or float32; k may be
+        None) turned by their rows' angles position * freq (float64, rope_freqs), times scale; into q_out and k_out,
+        or in place. pairs: dims 2 i and 2 i + 1 go together, else i and i + len(freq). Positions: pos (int32 [rows]), or
+        the last ones of lens[b] with rows_off as kv_append has them."""
+        x = k if q is None else q
+        _need(x is not None and (lens is not None or pos is not None), "rope: needs q or k, and lens or pos")
+        shape, dev = x.shape, self.device
+        rows, _, dim = shape
+        freq_n = freq.numel()
+        fp = _words(freq, freq_n, _Torch.f64, "rope: freq must be a float64 vector", dev)
+        t = ldq = ldqo = ldk = ldko = qp = qop = kp = kop = heads = kv_heads = 0
+        if q is not None:
+            heads = shape[1]
+            qp, ldq, t = _heads(q, shape, "rope: q must be bfloat16 or float32 [rows][heads][head_dim], a row contiguous", dev, True)
+            qop, ldqo, to = (qp, ldq, t) if q_out is None else _heads(q_out, shape, "rope: q_out must have q's shape and dtype, a row contiguous", dev)
+            _need(t == to, "rope: q_out must have q's dtype")
+        if k is not None:
+            ks = k.shape
+            _need(ks[0] == rows and ks[2] == dim, "rope: k must have q's rows and head_dim")
+            kv_heads = ks[1]
+            kp, ldk, tk = _heads(k, ks, "rope: k must be bfloat16 or float32 [rows][heads][head_dim], a row contiguous", dev, True)
+            kop, ldko, to = (kp, ldk, tk) if k_out is None else _heads(k_out, ks, "rope: k_out must have k's shape and dtype, a row contiguous", dev)
+            _need(tk == to and (q is None or tk == t), "rope: q, k and their outputs must have one dtype")
+            t = tk
+        n = 0 if lens is None else lens.numel()
+        rc = _lib.c4s_rope(
+            self._h, _pack_rope(qp, qop, kp, kop, ldq, ldqo, ldk, ldko, fp,
+                                _i32(pos, rows, "rope: pos must be an int32 vector of rows", dev),
+                                _i32(lens, n, "rope: lens must be an int32 vector", dev),
+                                _i32(rows_off, n + 1, "rope: rows_off must be an int32 vector of lens + 1", dev), n, rows,
+                                heads, kv_heads, dim, 2 * freq_n, ROPE_PAIRS if pairs else ROPE_HALF, t, scale),
+            self._queue(stream))
+        if rc:
+            self._check(rc, "rope")
+
+    def _pages(self, pages):
+        if pages.device != self.device:
+            raise ValueError(f"pages: they must be on the context's device, cuda:{self.device}")
+        return pages.packed
+
+    def pages_grow(self, pages, n_new=None, rows_off=None, row_pos=None, row_slot=None, copies=None, stream=None):
+        """Room for n_new[b] more tokens of every sequence (int32 [n_seqs]; one each by default); pages.lens counts them
+        then. The new rows' rows_off [n_seqs + 1], positions and slots (int32 [rows]), and, for beams, the pages to copy
+        before they are written (int32 [n_seqs][2]), are written where they are given."""
+        packed, n, dev = self._pages(pages), pages.n_seqs, self.device
+        rows = 0 if row_pos is None else row_pos.numel()
+        if row_slot is not None:
+            rows = row_slot.numel() if row_pos is None else min(rows, row_slot.numel())
+        rc = _lib.c4s_pages_grow(
+            self._h, packed,
+            _pack_grow(_i32(n_new, n, "pages_grow: n_new must be an int32 vector of n_seqs", dev),
+                       _i32(rows_off, n + 1, "pages_grow: rows_off must be an int32 vector of n_seqs + 1", dev),
+                       _i32(row_pos, 0 if row_pos is None else row_pos.numel(), "pages_grow: row_pos must be an int32 vector", dev),
+                       _i32(row_slot, 0 if row_slot is None else row_slot.numel(), "pages_grow: row_slot must be an int32 vector", dev),
+                       _i32(copies, 2 * n, "pages_grow: copies must be int32 [n_seqs][2]", dev), rows),
+            self._queue(stream))
+        if rc:
+            self._check(rc, "pages_grow")
+
+    def pages_trim(self, pages, n_drop, stream=None):
+        """The last n_drop[b] tokens of every sequence (int32 [n_seqs]) are taken back, and pages without a token."""
+        packed = self._pages(pages)
+        rc = _lib.c4s_pages_trim(self._h, packed,
+                                 _i32(n_drop, pages.n_seqs, "pages_trim: n_drop must be an int32 vector of n_seqs", self.device),
+                                 self._queue(stream))
+        if rc:
+            self._check(rc, "pages_trim")
+
+    def pages_fork(self, pages, parent, width, stream=None):
+        """In groups of width, sequence j becomes what sequence parent[j] (int32 [n_seqs], a number within the group) was:
+        its length and its pages."""
+        packed = self._pages(pages)
+        rc = _lib.c4s_pages_fork(self._h, packed,
+                                 _i32(parent, pages.n_seqs, "pages_fork: parent must be an int32 vector of n_seqs", self.device),
+                                 width, self._queue(stream))
+        if rc:
+            self._check(rc, "pages_fork")
+
+    def kv_copy(self, cache, copies, stream=None):
+        """Pages copies[i][0] of the cache into pages copies[i][1] (int32 [n][2], as pages_grow gives them)."""
+        _need(cache.device == self.device and copies.dim() == 2 and copies.shape[1] == 2,
+              f"kv_copy: copies must be int32 [n][2], the cache on the context's device, cuda:{self.device}")
+        rc = _lib.c4s_kv_copy(self._h, cache.packed,
+                              _i32(copies, copies.numel(), "kv_copy: copies must be contiguous int32 [n][2]", self.device),
+                              copies.shape[0], self._queue(stream))
+        if rc:
+            self._check(rc, "kv_copy")
+
+    def beam_step(self, logits, width, score, out_score, parent, token, done=None, out_done=None, stop_token=-1, temp=None,
+                  pen=None, hist_bits=None, out_hist_bits=None, states=(), stream=None):
+        """The best `width` continuations of every `width` rows of logits (bfloat16 or float32 [rows][vocab]), as
+        c4s_beam_step has it. score, out_score, temp, pen: float32 [rows]; parent, token: int32 [rows]; done,
+        out_done: uint8 [rows]; hist_bits, out_hist_bits: int32 words [rows][(vocab + 31) // 32]; states: pairs of
+        (source, destination), 32-bit tensors of [rows][..]. Outputs may be their inputs; out_hist_bits is
+        hist_bits by default."""
+        rows, vocab = logits.shape
+        dev = self.device
+        lp, ld, t = _rows(logits, logits.shape, "beam_step: logits must be bfloat16 or float32 [rows][vocab], a row contiguous", dev, True)
+        _need(width >= 1 and rows % width == 0, "beam_step: rows must be a multiple of width")
+        words = (vocab + 31) // 32
+        hp = _words(hist_bits, rows * words, _Torch.i32, "beam_step: hist_bits must be int32 [rows][(vocab + 31) // 32]", dev)
+        op = hp if out_hist_bits is None else _words(out_hist_bits, rows * words, _Torch.i32,
+                                                     "beam_step: out_hist_bits must be int32 [rows][(vocab + 31) // 32]", dev)
+        f = lambda x, name: _vector(x, rows, f"beam_step: {name} must be a float32 vector of rows", dev)  # noqa: E731
+        i = lambda x, name: _i32(x, rows, f"beam_step: {name} must be an int32 vector of rows", dev)  # noqa: E731
+        u = lambda x, name: _words(x, rows, _Torch.u8, f"beam_step: {name} must be a uint8 vector of rows", dev)  # noqa: E731
+        _need(len(states) <= BEAM_STATES, "beam_step: at most 8 states")
+        packed = b""
+        for src, dst in states:
+            for x in (src, dst):
+                if not (x.dim() == 2 and x.shape == src.shape and x.shape[0] == rows and x.element_size() == 4 and
+                        x.dtype is src.dtype and (x.shape[1] <= 1 or x.stride(1) == 1) and x.get_device() == dev):
+                    _refuse(x, "beam_step: states must be pairs of 32-bit tensors of one shape [rows][..], a row contiguous", dev)
+            n = src.shape[1]
+            packed += _pack_state(src.data_ptr(), dst.data_ptr(), src.stride(0) if rows > 1 else n, dst.stride(0) if rows > 1 else n, n)
+        packed += bytes(C.sizeof(BeamState) * (BEAM_STATES - len(states)))
+        rc = _lib.c4s_beam_step(
+            self._h, _pack_beam(lp, ld, t, rows // width, width, vocab, stop_token, len(states), f(temp, "temp"), f(pen, "pen"),
+                                hp, op, f(score, "score"), u(done, "done"), f(out_score, "out_score"),
+                                u(out_done, "out_done"), i(parent, "parent"), i(token, "token")) + packed,
+            self._queue(stream))
+        if rc:
+            self._check(rc, "beam_step")
 
     def hbm_probe(self, src, dst, nbytes, mode=0, stream=None):
         self._check(lib().c4s_hbm_probe(self._h, _p(src), _p(dst), nbytes, mode,

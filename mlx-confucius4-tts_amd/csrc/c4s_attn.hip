@@ -49,6 +49,34 @@ __device__ __forceinline__ uint4 codes(uint2 q) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// 4-bit codes as bf16 (exact: two significant bits times a power of two). The scale is a float's exponent, which is
+// all that the conversion looks at: what a byte's neighbours leave in the other bits does no harm.
+__device__ __forceinline__ float scale4(uint32_t bits) { return __uint_as_float(bits); }
+__device__ __forceinline__ uint4 codes4(uint32_t w, float s) {   // eight dims of a key
+  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3)));
+}
+// Eight positions of a pair of dims, a byte each, with their scales' bytes: the two dims' rows.
+__device__ __forceinline__ void pairs4(uint2 w, uint2 e, uint4& even, uint4& odd) {
+  uint32_t lo[4], hi[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = i ? w.y : w.x, x = i ? e.y : e.x;
+    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale4(x << 23), 0));
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale4(x << 15), 1));
+    const uint32_t c = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale4(x << 7), 2));
+    const uint32_t d = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale4(x >> 1), 3));
+    lo[2 * i] = __builtin_amdgcn_perm(b, a, 0x05040100);
+    hi[2 * i] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    lo[2 * i + 1] = __builtin_amdgcn_perm(d, c, 0x05040100);
+    hi[2 * i + 1] = __builtin_amdgcn_perm(d, c, 0x07060302);
+  }
+  even = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  odd = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+}
+
 // Keeps what is computed from w behind this place (the conversion of a block's
 // codes would otherwise move up to their load, at twice the registers).
 __device__ __forceinline__ void here(uint4& w) { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
@@ -145,8 +173,9 @@ struct FewArgs {
 };
 
 // DH: the head's dims rounded up to 64, 128 or 256; FULL: they are that many.
-template <int DH, bool Q8, bool FULL, int KEYS>
+template <int DH, int STORE, bool FULL, int KEYS>
 __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) void k_attn_few(FewArgs f) {
+  constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
   constexpr int kSteps = DH / 32, kTiles = DH / 16, kNT = KEYS / 16, kOwn = KEYS / 4;   // kOwn: a lane's positions of a block
   constexpr int kKLoads = Q8 ? kNT * kSteps / 2 : kNT * kSteps, kVLoads = Q8 || KEYS == 32 ? kTiles : 2 * kTiles;
   __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
@@ -185,22 +214,24 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   if (split >= parts) return;
   const int begin = max((first_chunk + split) * f.chunk, fst & ~(KEYS - 1)), end = (int)min((int64_t)(first_chunk + split + 1) * f.chunk, (int64_t)kend);
 
+  constexpr int k4Dims = DH == 64 ? 16 : 32, k4Steps = k4Dims / 8, k4Parts = kSteps / k4Steps;   // 4 bits: a lane's dims of a key in one piece; pieces
   uint4 q[kSteps];
   {
     const uint16_t* qp = a.q + (int64_t)(sq.row0 + token) * a.ldq + qh * dim;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      // codes come 16 dims a lane at a time, which are two steps of 8
-      const int d = Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
+      // codes come 16 dims a lane at a time, which are two steps of 8; in 4 bits up to 32 dims, a block of one scale
+      const int d = Q4 ? k4Dims * (s / k4Steps * 4 + g) + 8 * (s % k4Steps) : (Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g);
       q[s] = FULL || d < dim ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
     }
   }
   const float c2 = a.scale * kLog2e;
-  constexpr int kSize = Q8 ? 1 : 2;
-  const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;   // below 2^31
-  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head + 16 * g + (c % 4) * dim * kSize;
+  constexpr int kSize = Q8 || Q4 ? 1 : 2;
+  const int wide = Q4 ? dim / 2 : dim;   // codes of a row as the pages count them
+  const uint32_t head_bytes = (uint32_t)(wide * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;   // below 2^31
+  const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head + (Q4 ? 0 : 16 * g) + (c % 4) * wide * kSize;
   const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head + (uint64_t)(uint32_t)((c * kSize) << shift);
-  const uint32_t scale_bytes = 4u * (uint32_t)a.c.n_heads << shift;
+  const uint32_t scale_bytes = (Q4 ? (uint32_t)dim / 32 : 4u) * (uint32_t)a.c.n_heads << shift;
   const uint32_t tile_bytes = (16u * kSize) << shift;
   // A block's pages: of the key rows this lane loads, and of the positions it weighs (below 0: none).
   const int origin = (first_chunk + split) * f.chunk >> shift;
@@ -208,11 +239,46 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   auto pages_of = [&](int t) {
     return Pages{pages[((t + kOwn * (c / 4)) >> shift) - origin], pages[((t + kOwn * g) >> shift) - origin]};
   };
-  uint4 kr[kKLoads], vr[kVLoads];
+  uint4 kr[Q4 ? 1 : kKLoads], vr[Q4 ? 1 : kVLoads];
   float ks[Q8 ? kOwn : 1], vs[Q8 ? kOwn : 1];
+  // 4 bits: codes of keys and of pairs of dims, and a byte a position for each one's block
+  constexpr int kOwnWords = kOwn / 4;
+  uint32_t k4[Q4 ? kNT : 1][Q4 ? kSteps : 1], ke[Q4 ? k4Parts : 1][Q4 ? kOwnWords : 1];
+  uint32_t v4[Q4 ? kSteps : 1][Q4 ? kOwnWords : 1], ve[Q4 ? kSteps : 1][Q4 ? kOwnWords : 1];
+  auto own_words = [&](uint32_t (&to)[Q4 ? kOwnWords : 1], const char* p) {
+    if constexpr (Q4 && kOwn == 16) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+    } else if constexpr (Q4) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      to[0] = w.x, to[1] = w.y;
+    }
+  };
   auto load_keys = [&](int t, const Pages& p) {   // scores of what has no page are dropped
-    const uint32_t at = (uint32_t)((t + kOwn * (c / 4)) & (ps - 1)) * (uint32_t)(dim * kSize);
+    const uint32_t at = (uint32_t)((t + kOwn * (c / 4)) & (ps - 1)) * (uint32_t)(wide * kSize);
     const char* k = kbase + (uint64_t)(uint32_t)max(p.k, 0) * page_bytes + at;
+    if constexpr (Q4) {
+      const char* e = reinterpret_cast<const char*>(a.c.k_scale) + (uint64_t)(uint32_t)max(p.k, 0) * scale_bytes +
+                      (uint32_t)(((head * (dim / 32)) << shift) + ((t + kOwn * (c / 4)) & (ps - 1)));
+#pragma unroll
+      for (int part = 0; part < k4Parts; ++part) {
+        int d = k4Dims * (4 * part + g);
+        if (!FULL && d >= dim) d = part ? 32 * g : 0;   // times zeros of q
+        own_words(ke[part], e + (uint32_t)((d / 32) << shift));
+#pragma unroll
+        for (int tt = 0; tt < kNT; ++tt) {
+          const char* w = k + (4 * tt * dim + d) / 2;
+          if constexpr (k4Steps == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(w);
+            k4[tt][4 * part] = x.x, k4[tt][4 * part + 1] = x.y, k4[tt][4 * part + 2] = x.z, k4[tt][4 * part + 3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(w);
+            k4[tt][0] = x.x, k4[tt][1] = x.y;
+          }
+        }
+      }
+      return;
+    }
     constexpr int kRow = kSteps / (Q8 ? 2 : 1);
 #pragma unroll
     for (int tt = 0; tt < kNT; ++tt)
@@ -232,6 +298,19 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   auto load_values = [&](int t, const Pages& p) {
     const uint32_t at = (uint32_t)((t + kOwn * g) & (ps - 1));
     const char* v = vbase + (uint64_t)(uint32_t)max(p.v, 0) * page_bytes + at * kSize;
+    if constexpr (Q4) {
+      const char* e = reinterpret_cast<const char*>(a.c.v_scale) + (uint64_t)(uint32_t)max(p.v, 0) * scale_bytes + ((uint32_t)(head * (dim / 32)) << shift) + at;
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d) {
+        own_words(v4[d], v);
+        own_words(ve[d], e);
+        if (FULL || 32 * (d + 1) < dim) {   // blocks behind the last dim are not used
+          v += tile_bytes;
+          e += ps;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int d = 0; d < kTiles; ++d) {
       if constexpr (Q8) {
@@ -273,7 +352,11 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
           uint4 w;
-          if constexpr (Q8) {
+          if constexpr (Q4) {
+            uint32_t x = k4[tt][st];
+            asm volatile("" : "+v"(x));   // converted here, as codes of eight bits are
+            w = codes4(x, scale4(ke[st / k4Steps][tt] >> 8 * (c % 4) << 23));
+          } else if constexpr (Q8) {
             uint4 x = kr[tt * (kSteps / 2) + st / 2];
             here(x);
             w = codes(st % 2 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y));
@@ -281,7 +364,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
             w = kr[tt * kSteps + st];
           }
           s[tt] = mfma(w, q[st], s[tt]);
-          if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
+          if constexpr (Q8 || Q4) __builtin_amdgcn_sched_barrier(0);
         }
       __builtin_amdgcn_sched_barrier(0);
       // lane's scores are positions vt .. vt + kOwn - 1 of its row, in order
@@ -335,7 +418,42 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       }
       __builtin_amdgcn_sched_barrier(0);
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
-      if constexpr (!Q8) {
+      if constexpr (Q4) {
+        if (edge) {
+          // What is not there or not for any row may hold anything, and a block that is not finite is for those rows
+          // alone that see it: its scale becomes one that is, and those rows' results NaN, at whatever weight.
+          const int any_to = there ? min(kend, end) - vt : 0;
+#pragma unroll
+          for (int d = 0; d < kSteps; ++d) {
+            float strange = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+              const bool bad = (ve[d][j / 4] >> 8 * (j % 4) & 255u) == 255u;
+              if (bad && sees(j)) strange = __builtin_nanf("");
+              if (bad || j < from || j >= any_to) ve[d][j / 4] &= ~(255u << 8 * (j % 4));
+            }
+            strange = sum4(strange);
+            o[2 * d] += strange;
+            o[2 * d + 1] += strange;
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+#pragma unroll
+          for (int st = 0; st < KEYS / 32; ++st) {
+            uint32_t x = v4[d][2 * st], y = v4[d][2 * st + 1];
+            asm volatile("" : "+v"(x), "+v"(y));
+            uint4 even, odd;
+            pairs4(make_uint2(x, y), make_uint2(ve[d][2 * st], ve[d][2 * st + 1]), even, odd);
+            o[2 * d] = mfma(even, quad(hi + 4 * st), o[2 * d]);
+            o[2 * d + 1] = mfma(odd, quad(hi + 4 * st), o[2 * d + 1]);
+            o[2 * d] = mfma(even, quad(lo + 4 * st), o[2 * d]);
+            o[2 * d + 1] = mfma(odd, quad(lo + 4 * st), o[2 * d + 1]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      if constexpr (STORE == C4S_KV_BF16) {
         if (edge) {
           // What is not there or not for any row may hold anything: zeros. Where some of the rows see a
           // position and others do not, 0 times a value that is not finite would reach those: such
@@ -372,7 +490,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
         }
       }
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) {
+      for (int d = 0; d < (Q4 ? 0 : kTiles); ++d) {
 #pragma unroll
         for (int st = 0; st < KEYS / 32; ++st) {
           uint4 v;
@@ -400,7 +518,14 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
     sl[wave][c] = l;
   }
 #pragma unroll
-  for (int d = 0; d < kTiles; ++d) *reinterpret_cast<f32x4*>(&so[wave][c][16 * d + 4 * g]) = o[d];
+  for (int d = 0; d < kTiles; ++d) {
+    if constexpr (Q4) {   // tiles 2 i and 2 i + 1 have the even and the odd dims of a block
+      const f32x4 x = o[d & ~1], y = o[d | 1];
+      *reinterpret_cast<f32x4*>(&so[wave][c][32 * (d / 2) + 8 * g + 4 * (d % 2)]) = d % 2 ? f32x4{x[2], y[2], x[3], y[3]} : f32x4{x[0], y[0], x[1], y[1]};
+    } else {
+      *reinterpret_cast<f32x4*>(&so[wave][c][16 * d + 4 * g]) = o[d];
+    }
+  }
   __syncthreads();
   const int quads = dim / 4;   // a row
   const int64_t group = ((int64_t)seq * f.tiles + tile) * a.c.n_heads + head;
@@ -508,17 +633,18 @@ FewArgs few_args(const AttnArgs& a) {
   return f;
 }
 
-template <int DH, bool Q8, bool FULL, int KEYS>
+template <int DH, int STORE, bool FULL, int KEYS>
 hipError_t few(const FewArgs& f, hipStream_t s) {
-  hipLaunchKernelGGL((k_attn_few<DH, Q8, FULL, KEYS>), dim3((unsigned)((int64_t)f.tiles * f.splits * f.a.c.n_heads), f.a.c.n_seqs),
+  hipLaunchKernelGGL((k_attn_few<DH, STORE, FULL, KEYS>), dim3((unsigned)((int64_t)f.tiles * f.splits * f.a.c.n_heads), f.a.c.n_seqs),
                      dim3(kAttnThreads), 0, s, f);
   return hipGetLastError();
 }
-template <int DH, int BKEYS, int QKEYS>
-hipError_t few(const FewArgs& f, hipStream_t s) {
+template <int DH, int BKEYS, int QKEYS, int HKEYS>   // positions a block: bf16, 8 bits, 4 bits
+hipError_t few_by_store(const FewArgs& f, hipStream_t s) {
   const bool full = f.a.c.dim == DH;
-  if (f.a.c.store == C4S_KV_Q8) return full ? few<DH, true, true, QKEYS>(f, s) : few<DH, true, false, QKEYS>(f, s);
-  return full ? few<DH, false, true, BKEYS>(f, s) : few<DH, false, false, BKEYS>(f, s);
+  if (f.a.c.store == C4S_KV_Q8) return full ? few<DH, C4S_KV_Q8, true, QKEYS>(f, s) : few<DH, C4S_KV_Q8, false, QKEYS>(f, s);
+  if (f.a.c.store == C4S_KV_Q4) return full ? few<DH, C4S_KV_Q4, true, HKEYS>(f, s) : few<DH, C4S_KV_Q4, false, HKEYS>(f, s);
+  return full ? few<DH, C4S_KV_BF16, true, BKEYS>(f, s) : few<DH, C4S_KV_BF16, false, BKEYS>(f, s);
 }
 
 // ---- many rows ----------------------------------------------------------------------------
@@ -574,10 +700,13 @@ __device__ __forceinline__ int value_piece(int r, int p) {
   return (r * 8 + (p ^ (((r >> 1) & 1) << 1 | ((r >> 2) & 1) | ((r >> 3) & 1) << 2))) * 16;
 }
 
-template <int DH, bool Q8, int NB, int W, int OCC>
+// (In 4 bits a thread's piece is 16 codes: 16 dims of a key, or 8 positions of a pair of dims. They are in LDS as the
+// bf16 values that they stand for, and from there on such pages are bf16 pages.)
+template <int DH, int STORE, int NB, int W, int OCC>
 __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
+  constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
   constexpr int kSteps = DH / 32, kTiles = DH / 16, kNP = DH / 8;   // kNP: pieces of a key
-  constexpr int kThreads = 64 * W, kPieces = kBlock * DH / (Q8 ? 16 : 8);      // of a block's keys, and of its values
+  constexpr int kThreads = 64 * W, kPieces = kBlock * DH / (Q8 || Q4 ? 16 : 8);      // of a block's keys, and of its values
   constexpr int kLoads = kPieces < kThreads ? 1 : kPieces / kThreads;               // a thread's
   constexpr int kStagers = kPieces < kThreads ? kPieces : kThreads;                 // threads that have some
   constexpr int kBuf = 2 * kBlock * DH * 2;
@@ -634,8 +763,9 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
       q[b][s] = make_uint4(w.x ^ turn, w.y ^ turn, w.z ^ turn, w.w ^ turn);
     }
 
-  constexpr int kSize = Q8 ? 1 : 2;
-  const uint32_t head_bytes = (uint32_t)(dim * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;
+  constexpr int kSize = Q8 || Q4 ? 1 : 2;
+  const int wide = Q4 ? dim / 2 : dim;   // codes of a row as the pages count them
+  const uint32_t head_bytes = (uint32_t)(wide * kSize) << shift, page_bytes = head_bytes * (uint32_t)a.c.n_heads;
   const char* kbase = static_cast<const char*>(a.c.k) + (uint64_t)head_bytes * head;
   const char* vbase = static_cast<const char*>(a.c.v) + (uint64_t)head_bytes * head;
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_ld;
@@ -665,30 +795,47 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < W; ++w) missing |= gaps[w] != 0;
-    uint4 kst[kLoads], vst[kLoads];
+    uint4 kst[Q4 ? 1 : kLoads], vst[Q4 ? 1 : kLoads];
+    uint2 k4[Q4 ? kLoads : 1], v4[Q4 ? kLoads : 1], ve[Q4 ? kLoads : 1];   // 4 bits: codes, the blocks' bytes
+    uint8_t ke[Q4 ? kLoads : 1];
     float sst = 0.0f;
     // A thread's pieces of a block: of the keys in order; of the values in the order in which a page has them.
     // A block begins at a multiple of 64, so that of a piece's place in its page and in the table only what
     // the block adds changes.
-    constexpr int kKP = Q8 ? DH / 16 : DH / 8, kPer = Q8 ? 16 : 8;   // a key's pieces; dims or positions a piece
+    constexpr int kKP = Q8 || Q4 ? DH / 16 : DH / 8, kPer = Q8 || Q4 ? 16 : 8;   // a key's pieces; dims a piece
+    constexpr int kVPer = Q8 ? 16 : 8, kVRows = Q4 ? DH / 2 : DH;    // positions a piece of values; its rows (4 bits: of pairs)
     const int row_shift = min(shift, 6) - (Q8 ? 4 : 3);              // log2 of the pieces a page's row has in a block
     auto key_of = [&](int i) { return (tid + kThreads * i) / kKP; };
-    auto dim_of = [&](int i) { return ((tid + kThreads * i) >> row_shift) % DH; };   // of a piece of values, and which of its row
+    auto dim_of = [&](int i) { return ((tid + kThreads * i) >> row_shift) % kVRows; };   // of a piece of values, and which of its row
     auto piece_of = [&](int i) {
       const int at = tid + kThreads * i;
-      return (at >> row_shift) / DH << row_shift | (at & ((1 << row_shift) - 1));
+      return (at >> row_shift) / kVRows << row_shift | (at & ((1 << row_shift) - 1));
     };
     auto page_at = [&](int t, int in) { return (uint64_t)(uint32_t)max(pages[((t - seg) >> shift) + (in >> shift)], 0); };   // what has no page is dropped
     auto load = [&](int t) {
-      const uint32_t key_add = (uint32_t)((t & (ps - 1)) * dim * kSize), value_add = (uint32_t)((t & (ps - 1)) * kSize);
+      const uint32_t key_add = (uint32_t)((t & (ps - 1)) * wide * kSize), value_add = (uint32_t)((t & (ps - 1)) * kSize);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         if (kStagers < kThreads && tid >= kStagers) break;
         const int d = tid % kKP * kPer;   // the threads are a multiple of a key's pieces
+        if constexpr (Q4) {
+          const int key = key_of(i), pos = piece_of(i) * kVPer, pair = min(dim_of(i), wide - 1);
+          const uint32_t blocks = (uint32_t)(dim / 32), in_k = (uint32_t)((t + key) & (ps - 1)), in_v = (uint32_t)((t + pos) & (ps - 1));
+          const uint64_t kp = page_at(t, key), vp = page_at(t, pos);
+          k4[i] = make_uint2(0, 0);
+          ke[i] = 0;
+          if (d < dim) {
+            k4[i] = *reinterpret_cast<const uint2*>(kbase + kp * page_bytes + (in_k * (uint32_t)dim + (uint32_t)d) / 2);
+            ke[i] = reinterpret_cast<const uint8_t*>(a.c.k_scale)[(((kp * a.c.n_heads + head) * blocks + d / 32) << shift) + in_k];
+          }
+          v4[i] = *reinterpret_cast<const uint2*>(vbase + vp * page_bytes + ((uint32_t)(pair << shift) + in_v));
+          ve[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.c.v_scale) + (((vp * a.c.n_heads + head) * blocks + pair / 16) << shift) + in_v);
+          continue;
+        }
         kst[i] = make_uint4(0, 0, 0, 0);
         if (d < dim)
           kst[i] = *reinterpret_cast<const uint4*>(kbase + key_add + page_at(t, key_of(i)) * page_bytes + (uint32_t)(((key_of(i) & (ps - 1)) * dim + d) * kSize));
-        const int pos = piece_of(i) * kPer;
+        const int pos = piece_of(i) * kVPer;
         vst[i] = *reinterpret_cast<const uint4*>(vbase + value_add + page_at(t, pos) * page_bytes + (uint32_t)(((min(dim_of(i), dim - 1) << shift) + (pos & (ps - 1))) * kSize));
       }
       if constexpr (Q8) {
@@ -709,29 +856,41 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
       for (int i = 0; i < kLoads; ++i) {
         if (kStagers < kThreads && tid >= kStagers) break;
         const int vd = dim_of(i), piece = piece_of(i);
-        if constexpr (Q8) {
+        // Eight positions' values of a dim.
+        auto put_values = [&](int vd, uint4& v) {
+          if (edge) {
+            const int pos = t + 8 * piece;
+            if (t < fst || t + kBlock > kend || missing)
+              v = keep(v, 0, fst - pos, pages[(pos - seg) >> shift] >= 0 ? kend - pos : 0);
+            if (any_odd(v)) {
+              strange = 1;
+              uint32_t w[4] = {v.x, v.y, v.z, v.w}, was;
+#pragma unroll
+              for (int j = 3; j >= 0; --j) {
+                part_odd(w[j], was);
+                if (was) atomicMin(&bad[vd], pos + 2 * j + (was & 0xFFFFu ? 0 : 1));
+              }
+              v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          *reinterpret_cast<uint4*>(vl + value_piece(vd, piece)) = v;
+        };
+        if constexpr (Q4) {
+          const float scale = scale4((uint32_t)ke[i] << 23);
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2)) = codes4(k4[i].x, scale);
+          *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2 + 1)) = codes4(k4[i].y, scale);
+          uint4 even, odd;
+          pairs4(v4[i], ve[i], even, odd);
+          put_values(2 * vd, even);
+          put_values(2 * vd + 1, odd);
+        } else if constexpr (Q8) {
           *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2)) = codes(make_uint2(kst[i].x, kst[i].y));
           *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP * 2 + 1)) = codes(make_uint2(kst[i].z, kst[i].w));
           *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece)) = codes(make_uint2(vst[i].x, vst[i].y));
           *reinterpret_cast<uint4*>(vl + value_piece(vd, 2 * piece + 1)) = codes(make_uint2(vst[i].z, vst[i].w));
         } else {
           *reinterpret_cast<uint4*>(kl + key_piece<kNP>(key_of(i), tid % kKP)) = kst[i];
-          if (edge) {
-            const int pos = t + 8 * piece;
-            if (t < fst || t + kBlock > kend || missing)
-              vst[i] = keep(vst[i], 0, fst - pos, pages[(pos - seg) >> shift] >= 0 ? kend - pos : 0);
-            if (any_odd(vst[i])) {
-              strange = 1;
-              uint32_t w[4] = {vst[i].x, vst[i].y, vst[i].z, vst[i].w}, was;
-#pragma unroll
-              for (int j = 3; j >= 0; --j) {
-                part_odd(w[j], was);
-                if (was) atomicMin(&bad[vd], pos + 2 * j + (was & 0xFFFFu ? 0 : 1));
-              }
-              vst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-          *reinterpret_cast<uint4*>(vl + value_piece(vd, piece)) = vst[i];
+          put_values(vd, vst[i]);
         }
       }
       if constexpr (Q8) {
@@ -902,16 +1061,23 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   }
 }
 
-template <int DH, bool Q8, int NB, int W, int OCC>
+template <int DH, int STORE, int NB, int W, int OCC>
 hipError_t many(const AttnArgs& a, hipStream_t s) {
   const int tiles = (int)(((int64_t)a.max_new * a.shared + 16 * NB * W - 1) / (16 * NB * W));
   // 64 sequences, or what the grid has room for (2^32 threads in a dimension)
   const int64_t room = (int64_t)(UINT32_MAX / (64 * W)) / ((int64_t)tiles * a.c.n_heads);
   const int together = (int)std::min<int64_t>(std::min(a.c.n_seqs, 64), std::max<int64_t>(room, 1));
   const ManyArgs f{a, tiles, together};
-  hipLaunchKernelGGL((k_attn_many<DH, Q8, NB, W, OCC>), dim3((unsigned)((int64_t)f.tiles * a.c.n_heads * together), (a.c.n_seqs + together - 1) / together),
+  hipLaunchKernelGGL((k_attn_many<DH, STORE, NB, W, OCC>), dim3((unsigned)((int64_t)f.tiles * a.c.n_heads * together), (a.c.n_seqs + together - 1) / together),
                      dim3(64 * W), 0, s, f);
   return hipGetLastError();
+}
+
+template <int DH, int NB, int OCC>
+hipError_t many_by_store(const AttnArgs& a, hipStream_t s) {
+  if (a.c.store == C4S_KV_Q8) return many<DH, C4S_KV_Q8, NB, 8, OCC>(a, s);
+  if (a.c.store == C4S_KV_Q4) return many<DH, C4S_KV_Q4, NB, 8, OCC>(a, s);
+  return many<DH, C4S_KV_BF16, NB, 8, OCC>(a, s);
 }
 
 // Few rows' tiles re-read the positions but share them out over the chip: they win while they are few, and where
@@ -942,16 +1108,16 @@ LayerSpace attn_space(const AttnArgs& a) {
 
 hipError_t launch_attn(const AttnArgs& a, uint32_t* counters, float* space, hipStream_t s) {
   if (many_pays(a)) {
-    if (a.c.dim <= 64) return a.c.store == C4S_KV_Q8 ? many<64, true, 1, 8, 4>(a, s) : many<64, false, 1, 8, 4>(a, s);
-    if (a.c.dim <= 128) return a.c.store == C4S_KV_Q8 ? many<128, true, 2, 8, 2>(a, s) : many<128, false, 2, 8, 2>(a, s);
-    return a.c.store == C4S_KV_Q8 ? many<256, true, 1, 8, 2>(a, s) : many<256, false, 1, 8, 2>(a, s);
+    if (a.c.dim <= 64) return many_by_store<64, 1, 4>(a, s);
+    if (a.c.dim <= 128) return many_by_store<128, 2, 2>(a, s);
+    return many_by_store<256, 1, 2>(a, s);
   }
   FewArgs f = few_args(a);
   f.arrived = counters;
   f.part = space;
-  if (a.c.dim <= 64) return few<64, 32, 32>(f, s);
-  if (a.c.dim <= 128) return few<128, 32, 64>(f, s);
-  return few<256, 32, 32>(f, s);
+  if (a.c.dim <= 64) return few_by_store<64, 32, 32, 64>(f, s);
+  if (a.c.dim <= 128) return few_by_store<128, 32, 64, 64>(f, s);
+  return few_by_store<256, 32, 32, 32>(f, s);
 }
 
 }  // namespace c4s

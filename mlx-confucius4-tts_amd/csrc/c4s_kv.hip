@@ -1,5 +1,5 @@
-// The paged key-value cache: rows written as bf16 or as 8-bit codes, and read
-// back (include/c4s_layers.h has the layout).
+// The paged key-value cache: rows written as bf16 or as 8- or 4-bit codes, and
+// read back (include/c4s_layers.h has the layout).
 //
 // Both kernels take tiles of packed rows of one head, four lanes a row. Keys keep
 // their order: pieces of eight dims go to and from the page as they are. Values
@@ -127,14 +127,32 @@ __device__ __forceinline__ void swap_halves(uint32_t& x, uint32_t& y) {
   x = lo;
 }
 
+// Eight values as codes of four bits, and back: a block's scale is 2^(e - 127), e its byte, which is a float's exponent.
+__device__ __forceinline__ float scale4(uint32_t e) { return __uint_as_float(e << 23); }
+__device__ __forceinline__ uint32_t codes4(const Piece& w, float scale) {
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(Pair, (uint32_t)w[0]), scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(Pair, (uint32_t)w[1]), scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(Pair, (uint32_t)w[2]), scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(Pair, (uint32_t)w[3]), scale, 3);
+}
+__device__ __forceinline__ Piece values4(uint32_t c, float scale) {
+  return Piece{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3))};
+}
+
 // A tile of values in LDS, a row as it is outside the cache. An odd row length puts
 // the words that a wave moves between it and the pages in banks of their own.
-template <bool Q8, int PIECES, int TILE>
+// (4-bit codes move as 8-bit ones of half as many dims: a byte is a pair of dims.)
+template <int STORE, int PIECES, int TILE>
 struct Values {
-  static constexpr int kThreads = 4 * TILE, kGroups = TILE / 4;
-  uint32_t words[TILE][PIECES * (Q8 ? 8 : 16) + 1];
+  static constexpr bool Q8 = STORE != C4S_KV_BF16;
+  static constexpr int kThreads = 4 * TILE, kGroups = TILE / 4, kDims = STORE == C4S_KV_Q4 ? 8 : (Q8 ? 4 : 2);   // of a word
+  uint32_t words[TILE][PIECES * 32 / kDims + 1];
 
-  __device__ __forceinline__ uint32_t* piece(int row, int d) { return &words[row][Q8 ? d / 4 : d / 2]; }
+  __device__ __forceinline__ uint32_t* piece(int row, int d) { return &words[row][d / kDims]; }
 
   // To (TO_PAGES) or from the pages' rows of positions; v0: where a place's position
   // of dim 0 lies. Then words of four dims (Q8) or two for four positions at once.
@@ -203,10 +221,14 @@ struct Values {
 // leaves the range; adding 1.5 * 2^23 then leaves the integer to nearest even in
 // the sum's low bits. (With divisions the prompts above take 58 us for 52, a
 // step's 64 rows 4.8 for 4.1.)
-template <bool Q8, int PIECES, int TILE>
+// In 4 bits a block's 32 dims are one piece of each of a row's four lanes. Its scale's
+// exponent comes from the bits of the largest magnitude: 6 is 1.5 * 2^2, so adding 0x3F
+// to the 7 bits of the mantissa carries into the exponent just above 1.5.
+template <int STORE, int PIECES, int TILE>
 __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs rows) {
+  constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
   __shared__ Tile<TILE> tile;
-  __shared__ Values<Q8, PIECES, TILE> values;
+  __shared__ Values<STORE, PIECES, TILE> values;
   const int row = threadIdx.x / 4, l = threadIdx.x % 4, dim = c.dim, ps = 1 << c.page_shift;
   const int head = blockIdx.x % c.n_heads;
   const int64_t r = (int64_t)(blockIdx.x / c.n_heads) * TILE + row;
@@ -260,13 +282,28 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs 
                                                    __builtin_amdgcn_perm(sum[4 * j + 1], sum[4 * j], 0x0C0C0400), 0x05040100);
       }
     }
+    if (Q4) {
+      uint8_t* scales = reinterpret_cast<uint8_t*>(which ? c.v_scale : c.k_scale) + (p.page * c.n_heads + head) * (int64_t)(dim / 32) * ps + p.at;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        Halves top = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(Halves, raw[which][i][j] & 0x7FFF7FFFu));
+        const uint32_t most = max4(max(top[0], top[1]));
+        const uint32_t e = most >= 0x7F80u ? 255u : (uint32_t)max((int)((most + 0x3Fu) >> 7) - 2, 0);
+        raw[which][i][0] = codes4(raw[which][i], scale4(e));
+        if (p.page >= 0 && l == i % 4 && 32 * i < dim) scales[(uint32_t)i << c.page_shift] = (uint8_t)e;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int d = 32 * i + 8 * l;
       if (p.page < 0 || d >= dim) continue;
       if (which) {
 #pragma unroll
-        for (int j = 0; j < (Q8 ? 2 : 4); ++j) values.piece(row, d)[j] = raw[1][i][j];
+        for (int j = 0; j < (Q4 ? 1 : (Q8 ? 2 : 4)); ++j) values.piece(row, d)[j] = raw[1][i][j];
+      } else if (Q4) {
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(c.k) + (slot * dim + d) / 2) = raw[0][i][0];
       } else if (Q8) {
         *reinterpret_cast<Codes*>(static_cast<uint8_t*>(c.k) + slot * dim + d) = Codes{raw[0][i][0], raw[0][i][1]};
       } else {
@@ -275,15 +312,17 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs 
     }
   }
   __syncthreads();
-  values.template move<true>(tile, dim, c.page_shift, [&](const Place& q) {
-    return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * dim + q.at) * (Q8 ? 1 : 2);
+  const int wide = Q4 ? dim / 2 : dim;   // of a page's rows of positions
+  values.template move<true>(tile, wide, c.page_shift, [&](const Place& q) {
+    return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * wide + q.at) * (STORE == C4S_KV_BF16 ? 2 : 1);
   });
 }
 
-template <bool Q8, int PIECES, int TILE>
+template <int STORE, int PIECES, int TILE>
 __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs rows) {
+  constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
   __shared__ Tile<TILE> tile;
-  __shared__ Values<Q8, PIECES, TILE> values;
+  __shared__ Values<STORE, PIECES, TILE> values;
   tile.find(c, rows);
   const int row = threadIdx.x / 4, l = threadIdx.x % 4, dim = c.dim, ps = 1 << c.page_shift;
   const int head = blockIdx.x % c.n_heads;
@@ -295,21 +334,34 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
     scale[0] = c.k_scale[slot];
     scale[1] = c.v_scale[slot];
   }
+  uint32_t e[2][Q4 ? PIECES : 1];
+  if (Q4 && p.page >= 0) {
+    const int64_t first = (p.page * c.n_heads + head) * (int64_t)(dim / 32) * ps + p.at;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      if (32 * i >= dim) break;
+      e[0][i] = reinterpret_cast<const uint8_t*>(c.k_scale)[first + ((uint32_t)i << c.page_shift)];
+      e[1][i] = reinterpret_cast<const uint8_t*>(c.v_scale)[first + ((uint32_t)i << c.page_shift)];
+    }
+  }
   Piece raw[2][PIECES];   // without a page: zeros
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int d = 32 * i + 8 * l;
     raw[0][i] = raw[1][i] = Piece{};
     if (p.page < 0 || d >= dim) continue;
-    if (Q8) {
+    if (Q4) {
+      raw[0][i][0] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.k) + (slot * dim + d) / 2);
+    } else if (Q8) {
       const Codes w = *reinterpret_cast<const Codes*>(static_cast<const uint8_t*>(c.k) + slot * dim + d);
       raw[0][i] = Piece{w[0], w[1], 0, 0};
     } else {
       raw[0][i] = *reinterpret_cast<const Piece*>(static_cast<const uint16_t*>(c.k) + slot * dim + d);
     }
   }
-  values.template move<false>(tile, dim, c.page_shift, [&](const Place& q) {
-    return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * dim + q.at) * (Q8 ? 1 : 2);
+  const int wide = Q4 ? dim / 2 : dim;   // of a page's rows of positions
+  values.template move<false>(tile, wide, c.page_shift, [&](const Place& q) {
+    return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * wide + q.at) * (STORE == C4S_KV_BF16 ? 2 : 1);
   });
   // a row between two sequences' rows, or behind the last, is not the call's to write
   const bool mine = r < rows.n_rows && (!rows.off || (r >= rows.off[0] && r < rows.off[c.n_seqs]));
@@ -326,8 +378,9 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
       Piece w = raw[which][i];
       if (which && p.page >= 0) {
 #pragma unroll
-        for (int j = 0; j < (Q8 ? 2 : 4); ++j) w[j] = values.piece(row, d)[j];
+        for (int j = 0; j < (Q4 ? 1 : (Q8 ? 2 : 4)); ++j) w[j] = values.piece(row, d)[j];
       }
+      if (Q4 && p.page >= 0) w = values4(w[0], scale4(e[which][i]));
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -355,34 +408,35 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
 // 4.1 us, in tiles of 64 in 6.5). `launch` gets the store, the pieces of a lane and the tile's rows.
 template <class Launch>
 hipError_t by_kind(const KvArgs& c, const KvRowsArgs& r, Launch launch) {
-  auto tile = [&](auto q8, auto pieces) {
-    if ((int64_t)(r.n_rows / 64) * c.n_heads >= 256) launch(q8, pieces, std::integral_constant<int, 64>());
-    else launch(q8, pieces, std::integral_constant<int, 16>());
+  auto tile = [&](auto store, auto pieces) {
+    if ((int64_t)(r.n_rows / 64) * c.n_heads >= 256) launch(store, pieces, std::integral_constant<int, 64>());
+    else launch(store, pieces, std::integral_constant<int, 16>());
   };
-  auto pieces = [&](auto q8) {
-    if (c.dim <= 64) tile(q8, std::integral_constant<int, 2>());
-    else if (c.dim <= 128) tile(q8, std::integral_constant<int, 4>());
-    else tile(q8, std::integral_constant<int, 8>());
+  auto pieces = [&](auto store) {
+    if (c.dim <= 64) tile(store, std::integral_constant<int, 2>());
+    else if (c.dim <= 128) tile(store, std::integral_constant<int, 4>());
+    else tile(store, std::integral_constant<int, 8>());
   };
-  if (c.store == C4S_KV_Q8) pieces(std::true_type());
-  else pieces(std::false_type());
+  if (c.store == C4S_KV_Q8) pieces(std::integral_constant<int, C4S_KV_Q8>());
+  else if (c.store == C4S_KV_Q4) pieces(std::integral_constant<int, C4S_KV_Q4>());
+  else pieces(std::integral_constant<int, C4S_KV_BF16>());
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv_append(const KvArgs& c, const KvRowsArgs& r, hipStream_t s) {
-  return by_kind(c, r, [&](auto q8, auto pieces, auto tile) {
+  return by_kind(c, r, [&](auto store, auto pieces, auto tile) {
     constexpr int kTile = decltype(tile)::value;
-    hipLaunchKernelGGL((k_kv_append<decltype(q8)::value, decltype(pieces)::value, kTile>),
+    hipLaunchKernelGGL((k_kv_append<decltype(store)::value, decltype(pieces)::value, kTile>),
                        dim3((r.n_rows + kTile - 1) / kTile * c.n_heads), dim3(4 * kTile), 0, s, c, r);
   });
 }
 
 hipError_t launch_kv_read(const KvArgs& c, const KvRowsArgs& r, hipStream_t s) {
-  return by_kind(c, r, [&](auto q8, auto pieces, auto tile) {
+  return by_kind(c, r, [&](auto store, auto pieces, auto tile) {
     constexpr int kTile = decltype(tile)::value;
-    hipLaunchKernelGGL((k_kv_read<decltype(q8)::value, decltype(pieces)::value, kTile>),
+    hipLaunchKernelGGL((k_kv_read<decltype(store)::value, decltype(pieces)::value, kTile>),
                        dim3((r.n_rows + kTile - 1) / kTile * c.n_heads), dim3(4 * kTile), 0, s, c, r);
   });
 }

@@ -1,0 +1,169 @@
+// Rotary positions (c4s_rope, include/c4s_batch.h).
+//
+// A workgroup has one row, or a part of its heads: its first threads turn the
+// position into cosines and sines, once for all heads, and leave them in LDS
+// while every thread's first piece of queries or keys is on its way. A piece is
+// eight bf16 or four floats (of either half of the pairs, with C4S_ROPE_HALF), or
+// single pairs where sizes or alignment do not allow that.
+//
+// The angle is reduced in 64 bits: position * frequency / 2 pi, less its whole
+// turns, has an absolute error of 2^-52 of the number of turns; the rest, at most
+// half a turn, is exact enough in 32 bits (2^-25 of a turn, 2e-7 radians).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "c4s_batch.hpp"
+
+namespace c4s {
+namespace {
+
+constexpr int kRopePairs = 512;   // head_dim / 2 at most
+
+// The sequence's position of packed row r; -1: it has none.
+__device__ __forceinline__ int64_t position_of(const c4s_rope_desc& a, int r) {
+  if (a.pos) return a.pos[r];
+  int seq = r, left = 1;
+  if (a.rows_off) {
+    int lo = 0, hi = a.n_seqs;   // the last sequence that starts at or before r, eight parts a step
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 7) / 8;
+      int behind = 0;
+#pragma unroll
+      for (int j = 1; j < 8; ++j) behind += (lo + j * step < hi) & (a.rows_off[min(lo + j * step, hi - 1)] <= r);
+      lo += behind * step;
+      hi = min(lo + step, hi);
+    }
+    seq = lo;
+    left = a.rows_off[seq + 1] - r;
+    if (a.n_seqs == 0 || r < a.rows_off[seq] || left < 1) return -1;
+  } else if (seq >= a.n_seqs) {
+    return -1;
+  }
+  return max((int64_t)a.lens[seq] - left, (int64_t)-1);
+}
+
+typedef __bf16 bf16_t;
+// N values of T, in memory that is aligned for them, or (one value or pair) for one.
+template <class T, int N>
+struct alignas(N <= 2 ? sizeof(T) : sizeof(T) * N) Few {
+  T v[N];
+};
+
+struct RopeArgs {
+  c4s_rope_desc d;
+  int parts;   // workgroups of a row
+};
+
+// T: of the tensors; N: values a piece; PAIRS: the layout.
+template <class T, int N, bool PAIRS>
+__global__ __launch_bounds__(256) void k_rope(RopeArgs f) {
+  __shared__ float cs[kRopePairs], sn[kRopePairs];
+  const c4s_rope_desc& a = f.d;
+  const int row = blockIdx.x / f.parts, part = blockIdx.x % f.parts;
+  const int half = a.rot_dim / 2;
+  const int turned = PAIRS ? a.rot_dim / N : half / N;          // pieces of a head that are turned; the others
+  const int per = turned + (a.head_dim - a.rot_dim) / N;        // (copied) follow them
+  const int heads = (a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0), all = heads * per;
+  const int step = blockDim.x * f.parts;
+
+  struct Piece {
+    const T* from;
+    T* to;
+    int pair;    // the first one it has; -1: copied
+  };
+  auto piece = [&](int i) {
+    const int head = i / per, p = i - head * per;
+    const bool is_q = a.q && head < a.n_heads;
+    const int h = is_q || !a.q ? head : head - a.n_heads;
+    const int64_t r = row;
+    const T* from = static_cast<const T*>(is_q ? a.q : a.k) + r * (is_q ? a.ldq : a.ldk) + (int64_t)h * a.head_dim;
+    T* to = static_cast<T*>(is_q ? a.q_out : a.k_out) + r * (is_q ? a.ldq_out : a.ldk_out) + (int64_t)h * a.head_dim;
+    const int at = p < turned ? p * N : a.rot_dim + (p - turned) * N;
+    return Piece{from + at, to + at, p < turned ? (PAIRS ? at / 2 : at) : -1};
+  };
+  using V = Few<T, N>;
+  int i = part * blockDim.x + threadIdx.x;
+  Piece now{};
+  V x{}, y{};
+  auto load = [&] {
+    now = piece(i);
+    x = *reinterpret_cast<const V*>(now.from);
+    if (!PAIRS && now.pair >= 0) y = *reinterpret_cast<const V*>(now.from + half);
+  };
+  if (i < all) load();
+
+  const int64_t pos = position_of(a, row);
+  if (pos < 0) return;
+  for (int p = threadIdx.x; p < half; p += blockDim.x) {
+    double turns = (double)pos * a.freq[p] * 0.15915494309189535;
+    turns -= rint(turns);
+    float s, c;
+    sincospif(2.0f * (float)turns, &s, &c);
+    cs[p] = c * a.scale;
+    sn[p] = s * a.scale;
+  }
+  __syncthreads();
+  while (i < all) {
+    if (now.pair < 0) {
+      if (now.to != now.from) *reinterpret_cast<V*>(now.to) = x;
+    } else if (PAIRS) {
+      V o;
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        const float c = cs[now.pair + j / 2], s = sn[now.pair + j / 2], u = (float)x.v[j], w = (float)x.v[j + 1];
+        o.v[j] = (T)(u * c - w * s);
+        o.v[j + 1] = (T)(u * s + w * c);
+      }
+      *reinterpret_cast<V*>(now.to) = o;
+    } else {
+      V o, e;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float c = cs[now.pair + j], s = sn[now.pair + j], u = (float)x.v[j], w = (float)y.v[j];
+        o.v[j] = (T)(u * c - w * s);
+        e.v[j] = (T)(u * s + w * c);
+      }
+      *reinterpret_cast<V*>(now.to) = o;
+      *reinterpret_cast<V*>(now.to + half) = e;
+    }
+    i += step;
+    if (i < all) load();
+  }
+}
+
+template <class T, int N, bool PAIRS>
+hipError_t rope(const c4s_rope_desc& a, hipStream_t s) {
+  const int per = (PAIRS ? a.rot_dim : a.rot_dim / 2) / N + (a.head_dim - a.rot_dim) / N;
+  const int64_t all = (int64_t)((a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0)) * per;
+  const int threads = (int)std::min<int64_t>((all + 63) / 64 * 64, 256);
+  // rows alone fill the chip, or every thread has one piece
+  const int parts = a.n_rows >= 1024 ? 1 : (int)std::min<int64_t>((all + threads - 1) / threads, std::max(2048 / a.n_rows, 1));
+  hipLaunchKernelGGL((k_rope<T, N, PAIRS>), dim3((unsigned)(a.n_rows * parts)), dim3(threads), 0, s, RopeArgs{a, parts});
+  return hipGetLastError();
+}
+
+// Whether every piece of N values starts on its own size: sizes, strides, addresses.
+bool fits(const c4s_rope_desc& a, int n, int size) {
+  uint64_t odd = (uint64_t)a.head_dim | (uint64_t)(a.layout == C4S_ROPE_PAIRS ? a.rot_dim : a.rot_dim / 2) | (uint64_t)(a.head_dim - a.rot_dim);
+  uint64_t at = 0;
+  if (a.q) odd |= (uint64_t)(a.ldq | a.ldq_out), at |= (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.q_out;
+  if (a.k) odd |= (uint64_t)(a.ldk | a.ldk_out), at |= (uint64_t)(uintptr_t)a.k | (uint64_t)(uintptr_t)a.k_out;
+  return odd % n == 0 && at % (n * size) == 0;
+}
+
+template <class T, int N>
+hipError_t by_layout(const c4s_rope_desc& a, hipStream_t s) {
+  const bool wide = fits(a, N, sizeof(T));
+  if (a.layout == C4S_ROPE_HALF) return wide ? rope<T, N, false>(a, s) : rope<T, 1, false>(a, s);
+  return wide ? rope<T, N, true>(a, s) : rope<T, 2, true>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_rope(const c4s_rope_desc& a, hipStream_t s) {
+  return a.dtype == C4S_DTYPE_BF16 ? by_layout<bf16_t, 8>(a, s) : by_layout<float, 4>(a, s);
+}
+
+}  // namespace c4s
