@@ -151,7 +151,7 @@ typedef struct c4s_beam_state {
   const void* src;           /* [rows][ld_src] 32-bit words, 4-byte aligned */
   void* dst;                 /* [rows][ld_dst], or src itself with its stride */
   int64_t ld_src, ld_dst;    /* >= words */
-  int64_t words;             /* of a row */
+  int64_t words;             /* of a row, up to 2147483647; ceil(all states' and the history's words / 256) * n_groups up to 16777215 */
 } c4s_beam_state;
 
 enum { C4S_BEAM_STATES = 8 };

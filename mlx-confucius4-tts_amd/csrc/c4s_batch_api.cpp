@@ -86,6 +86,7 @@ int check_beam(c4s_ctx* ctx, const c4s_beam* a) {
   if (bits(a->logits) & (a->dtype == C4S_DTYPE_F32 ? 3u : 1u)) return fail(ctx, C4S_EINVAL, "beam_step: logits are not aligned to their type");
   if (!a->hist_bits != !a->out_hist_bits || (a->rep_penalty && !a->hist_bits))
     return fail(ctx, C4S_EINVAL, "beam_step: rep_penalty needs hist_bits, and hist_bits and out_hist_bits go together");
+  int64_t words = a->hist_bits ? (a->vocab + 31) / 32 : 0;
   for (int i = 0; i < a->n_states; ++i) {
     const c4s_beam_state& s = a->states[i];
     if (s.words < 0 || s.ld_src < s.words || s.ld_dst < s.words)
@@ -94,7 +95,11 @@ int check_beam(c4s_ctx* ctx, const c4s_beam* a) {
       return fail(ctx, C4S_EINVAL, "beam_step: a state is NULL or not 4-byte aligned");
     if (s.words && s.src == s.dst && s.ld_src != s.ld_dst)
       return fail(ctx, C4S_EINVAL, "beam_step: a state in place has one stride");
+    if (s.words > INT32_MAX) return fail(ctx, C4S_EINVAL, "beam_step: a state has more than 2147483647 words a row");
+    words += s.words;
   }
+  if ((words + 255) / 256 * a->n_groups > (1 << 24) - 1)   // a grid has up to 2^32 threads
+    return fail(ctx, C4S_EINVAL, "beam_step: more than 16777215 times 256 words of states, each group's rounded up");
   return C4S_OK;
 }
 

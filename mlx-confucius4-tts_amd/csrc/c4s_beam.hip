@@ -1,21 +1,26 @@
 // One step of beam search (c4s_beam_step, include/c4s_batch.h).
 //
 // The logits are read once. A wave has a slice of a row and goes through it in
-// chunks of 1024 values, 16 a lane: it keeps the running maximum and sum of exp a
-// lane, and a list in LDS of the slice's `width` best tokens. Of a row's tokens
-// only those can win, since within a row totals are ordered as the logits are.
-// A chunk costs the list nothing unless a value beats its last place; then a bound
-// keeps the newcomers few: of the lanes whose best value does, the width-th best of
-// those, which at most width lanes' 16 values reach.
-// The last workgroup of a group to arrive joins the slices' sums (64 bits, in the
-// slices' order), and takes the group's best from the slices' lists: all lists'
-// first places, then all second ones, until a round brings nothing. It then brings
-// the states into their new order, a thread a column: it reads that of all rows
-// before it writes one, so that outputs may be the inputs.
+// chunks of 1024 values, 16 a lane: a lane keeps the running maximum and sum of
+// exp, and leaves each chunk's largest value in LDS. Of a row's tokens only the
+// slice's `width` best can win, since within a row totals are ordered as the logits
+// are: the width-th largest of the lanes' maxima bounds them from below, and where a
+// lane's chunk reaches that bound (a few do) its 16 values are read once more, 16 such
+// sets at a time, and ranked into a list. A list that is full raises the bound.
+// The last workgroup of a group to arrive joins the slices' sums (in the slices'
+// order). Its threads look at the slices' first places alone: the width-th best of a
+// wave's threads' best bounds what can win, and the few places that reach the bound
+// are ranked together.
+// A second kernel brings the states into their new order, a thread a column: it
+// reads that of all rows before it writes one, so that outputs may be the inputs.
+// (In the first kernel's last workgroups it was a chain of waits: 9 us of 33 for 64
+// groups of 4 with 1757 words a row, 40 of 85 for 24 of 8 with 5348.)
 //
 // Orders are on (value, index) pairs, equal values by the lower index, so results
-// do not depend on how rows are cut, but for the sums' rounding (2^-24 of a lane's
-// part; the totals are 64-bit).
+// do not depend on how rows are cut, but for the sums' rounding: exp(z - m) as
+// 2^((z - m) log2 e) is off by 2^-23 |z - m| of itself, least where it counts most.
+// (One fused operation, z log2 e - m log2 e, would save a tenth of the VALU's work and
+// overflow on a row whose logits are all the type's lowest value.)
 
 #include <hip/hip_runtime.h>
 
@@ -31,13 +36,19 @@ namespace {
 
 constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / 64;
 constexpr int kPer = 16, kChunk = 64 * kPer;   // values of a lane, and of a wave, at a time
+constexpr int kMostChunks = 32;                // of a slice
+constexpr int kQueue = 128;                    // a lane's chunks that wait to be looked at
+constexpr int kFound = 1024;                   // places that are ranked together
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamArgs {
   c4s_beam a;
   int slices, chunks;    // of a row; chunks of a slice
   int wgs;               // workgroups of a group
   uint32_t* arrived;     // [n_groups]
-  uint64_t* parts;       // [rows][slices][2 + width]: maximum, sum, keys
+  int state_wgs;         // workgroups of a group's states
+  int32_t* joined;       // [rows] the token that joins a row's history, -1: none; with states
+  uint64_t* parts;       // [rows][slices][1 + width]: maximum and sum, keys
 };
 
 __device__ __forceinline__ void wave_order() {   // this wave's writes to LDS before its reads behind it
@@ -45,328 +56,466 @@ __device__ __forceinline__ void wave_order() {   // this wave's writes to LDS be
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
-}
+__device__ __forceinline__ int lanes_before(uint64_t mask, int lane) { return __popcll(mask & ((1ull << lane) - 1)); }
 
 // A token's value as it ranks in its row: larger is better, equal values by the lower token; 0: no token.
 __device__ __forceinline__ uint64_t token_key(float z, int v) { return (uint64_t)fkey(z) << 32 | (uint32_t)~v; }
 __device__ __forceinline__ float key_value(uint64_t k) { return kfloat((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int key_token(uint64_t k) { return (int)~(uint32_t)k; }
 
-// The same of a total.
+// The same of a total: its bits in an order that unsigned numbers have, and the lower (beam, token) first.
 struct Total {
-  double t;
-  int32_t at;   // beam * vocab + token; -1: none
-  __device__ __forceinline__ bool beats(const Total& o) const { return at >= 0 && (o.at < 0 || t > o.t || (t == o.t && at < o.at)); }
+  uint64_t t;
+  uint32_t at;   // ~(beam * vocab + token)
+  __device__ __forceinline__ bool beats(const Total& o) const { return (t > o.t) | ((t == o.t) & (at > o.at)); }
+};
+constexpr uint64_t kTotalNegInf = 0x000FFFFFFFFFFFFFull;
+__device__ __forceinline__ Total no_total() { return Total{0, 0}; }
+__device__ __forceinline__ Total total_of(double t, int at) {   // what is not a number counts as -inf, so that all totals have an order
+  const uint64_t u = (uint64_t)__double_as_longlong(t + 0.0);   // one zero
+  return Total{t == t ? (u >> 63 ? ~u : u | 1ull << 63) : kTotalNegInf, (uint32_t)~at};
+}
+__device__ __forceinline__ double total_value(const Total& x) {
+  return __longlong_as_double((long long)(x.t >> 63 ? x.t ^ 1ull << 63 : ~x.t));
+}
+
+// A number that at least n of the wave's lanes reach, and the n-th largest of them but for its last bits (0: fewer
+// lanes have one). Twenty bits from the top: a comparison, a count of lanes and a choice each.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+  uint32_t at = 0;
+#pragma unroll
+  for (int b = 31; b >= 12; --b) {
+    const uint32_t up = at | 1u << b;
+    at = __popcll(__ballot(v >= up)) >= n ? up : at;
+  }
+  return at;
+}
+
+// The first `most` of list[0 .. n), in order, at its front; n up to 128. One wave's.
+__device__ __forceinline__ void keep_best(uint64_t* list, int n, int most, int lane) {
+  wave_order();
+  const uint64_t a = lane < n ? list[lane] : 0, b = 64 + lane < n ? list[64 + lane] : 0;
+  int pa = lane < n ? 0 : most, pb = 64 + lane < n ? 0 : most;
+  for (int j = 0; j < n; j += 4) {   // four reads on their way (behind n there may be anything)
+    uint64_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = list[j + k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (j + k >= n) o[k] = 0;
+      pa += o[k] > a;
+      pb += o[k] > b;
+    }
+  }
+  wave_order();
+  if (pa < most) list[pa] = a;
+  if (pb < most) list[pb] = b;
+  wave_order();
+}
+
+// 16 bytes of logits, in memory that is aligned for one.
+template <class T>
+struct alignas(sizeof(T)) Some {
+  T v[16 / sizeof(T)];
 };
 
-template <int N, class T>
-struct alignas(sizeof(T)) Row {
-  T v[N];
+// A row's logits after penalty and temperature.
+template <bool BF16>
+struct Logits {
+  using T = std::conditional_t<BF16, uint16_t, float>;
+  static constexpr int kSome = 16 / sizeof(T), kSets = kPer / kSome;   // values of a load; loads of a lane and chunk
+  const T* x;
+  const uint32_t* hist;   // null: nothing to penalise
+  float pen, temp;
+
+  __device__ __forceinline__ Logits(const c4s_beam& a, int64_t row) {
+    x = static_cast<const T*>(a.logits) + row * a.ld;
+    pen = a.rep_penalty ? a.rep_penalty[row] : 1.0f;
+    temp = a.temperature ? a.temperature[row] : 1.0f;
+    hist = pen != 1.0f ? a.hist_bits + row * ((a.vocab + 31) / 32) : nullptr;
+    if (!(temp > 0.0f)) temp = 1.0f;
+  }
+  // Tokens v .. v + kSome - 1, v a multiple of that, as they are in memory; what lies behind `end` is not read.
+  __device__ __forceinline__ Some<T> raw(int v, int end) const {
+    Some<T> r{};
+    if (v + kSome <= end) {
+      r = *reinterpret_cast<const Some<T>*>(x + v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSome; ++j)
+        if (v + j < end) r.v[j] = x[v + j];
+    }
+    return r;
+  }
+  __device__ __forceinline__ uint32_t bits(int v, int end) const { return hist && v < end ? hist[v >> 5] >> (v & 31) : 0; }
+  __device__ __forceinline__ void value(const Some<T>& r, uint32_t bits, float* z) const {
+#pragma unroll
+    for (int j = 0; j < kSome; ++j) {
+      if constexpr (BF16) z[j] = __uint_as_float((uint32_t)r.v[j] << 16);
+      else z[j] = r.v[j];
+    }
+    if (hist) {
+#pragma unroll
+      for (int j = 0; j < kSome; ++j) z[j] = bits >> j & 1 ? (z[j] < 0.0f ? z[j] * pen : z[j] / pen) : z[j];
+    }
+    if (temp != 1.0f) {
+#pragma unroll
+      for (int j = 0; j < kSome; ++j) z[j] = z[j] / temp;
+    }
+  }
 };
 
 template <bool BF16>
-__global__ __launch_bounds__(kBeamThreads) void k_beam(BeamArgs f) {
-  // A wave's list and its newcomers; the last workgroup's rows and states
-  constexpr int kList = kBeamWidth * (kPer + 1);
+__global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   __shared__ __align__(16) union {
-    uint64_t keys[kBeamWaves][kList];
     struct {
-      Total best[kBeamWaves][kBeamWidth + 64];
-      double lse[kBeamWidth];
-      float score[kBeamWidth];
-      uint8_t done[kBeamWidth];
-      Total won[kBeamWidth];
-      int counts[kBeamWaves];
-    } last;
-    uint32_t column[kBeamWidth * kBeamThreads];
+      uint64_t list[kBeamWaves][128];
+      uint32_t tops[kBeamWaves][kMostChunks][64];   // keys of the lanes' largest values by chunk
+      uint16_t queue[kBeamWaves][kQueue];           // chunk * 64 + lane
+    } wave;
+    Total found[kFound];
   } lds;
-  __shared__ int parents[kBeamWidth];
+  __shared__ Total won[kBeamWidth];
+  __shared__ uint32_t bounds[kBeamWaves];
+  __shared__ double logs[kBeamWidth];                    // the rows' log sum exp(z - tops)
+  __shared__ float score[kBeamWidth], tops[kBeamWidth];
+  __shared__ int n_found;
+  __shared__ uint8_t done[kBeamWidth];
   const c4s_beam& a = f.a;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, W = a.width, V = a.vocab;
   const int group = blockIdx.x / f.wgs, units = W * f.slices, unit = blockIdx.x % f.wgs * kBeamWaves + wave;
   const int64_t row0 = (int64_t)group * W;
-  const int words = 2 + W;
+  const int words = 1 + W;
 
   if (unit < units) {
     const int64_t row = row0 + unit / f.slices;
     const int slice = unit % f.slices;
-    uint64_t* part = f.parts + (row * f.slices + slice) * words;
+    const Logits<BF16> x(a, row);
+    using T = typename Logits<BF16>::T;
+    constexpr int kSome = Logits<BF16>::kSome, kSets = Logits<BF16>::kSets;
+    const int begin = slice * f.chunks * kChunk, end = min(begin + f.chunks * kChunk, V);
+    // value kSome i + j of the lane: token v0 + 64 kSome i + kSome lane + j; two chunks are on their way
+    Some<T> ahead[2][kSets];
+    uint32_t ahead_bits[2][kSets];
+    auto token = [&](int v0, int i, int l) { return v0 + 64 * kSome * i + kSome * l; };
+    auto load = [&](int which, int v0) {
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        ahead[which][i] = x.raw(token(v0, i, lane), end);
+        ahead_bits[which][i] = x.bits(token(v0, i, lane), end);
+      }
+    };
+    load(0, begin);
+    if (begin + kChunk < end) load(1, begin + kChunk);
     const bool idle = (a.done && a.done[row]) || a.score[row] == -__builtin_inff();   // its logits do not matter
     if (!idle) {
-      using T = typename std::conditional<BF16, uint16_t, float>::type;
-      const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-      const uint32_t* hist = a.rep_penalty && a.rep_penalty[row] != 1.0f ? a.hist_bits + row * ((V + 31) / 32) : nullptr;
-      const float pen = hist ? a.rep_penalty[row] : 1.0f;
-      float temp = a.temperature ? a.temperature[row] : 1.0f;
-      if (!(temp > 0.0f)) temp = 1.0f;
-      uint64_t* list = lds.keys[wave];
-      int kept = 0;
-      uint64_t least = 0;   // what a key has to beat
+      uint32_t (*chunk_tops)[64] = lds.wave.tops[wave];
       float m = -__builtin_inff(), sum = 0.0f;
-      const int begin = slice * f.chunks * kChunk, end = min(begin + f.chunks * kChunk, V);
-      for (int v0 = begin; v0 < end; v0 += kChunk) {
-        float z[kPer];   // value 4 i + j of the lane: token v0 + 256 i + 4 lane + j
+      uint32_t most = 0;   // key of the lane's largest value; 0: it has none
+      float z[kPer];
+      auto chunk = [&](int which, int v0, int at) {
 #pragma unroll
-        for (int i = 0; i < kPer / 4; ++i) {
-          const int v = v0 + 256 * i + 4 * lane;
-          Row<4, T> raw;
-          if (v + 4 <= end) {
-            raw = *reinterpret_cast<const Row<4, T>*>(x + v);
-          } else {
+        for (int i = 0; i < kSets; ++i) x.value(ahead[which][i], ahead_bits[which][i], z + kSome * i);
+        if (v0 + 2 * kChunk < end) load(which, v0 + 2 * kChunk);
+        if (v0 + kChunk > end) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) raw.v[j] = v + j < end ? x[v + j] : T();
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (BF16) z[4 * i + j] = __uint_as_float((uint32_t)raw.v[j] << 16);
-            else z[4 * i + j] = raw.v[j];
-          }
-          if (hist && v < end) {
-            const uint32_t bits = hist[v >> 5] >> (v & 31);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float y = z[4 * i + j];
-              if (bits >> j & 1) z[4 * i + j] = y < 0.0f ? y * pen : y / pen;
-            }
-          }
+          for (int i = 0; i < kPer; ++i)
+            if (token(v0, i / kSome, lane) + i % kSome >= end) z[i] = -__builtin_inff();   // adds nothing
         }
-        if (temp != 1.0f) {
+        float top = z[0];
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) z[i] = z[i] / temp;
-        }
-        auto token = [&](int i) { return v0 + 256 * (i / 4) + 4 * lane + i % 4; };
-        uint64_t best = 0;
-        float top = m;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int v = token(i);
-          if (v >= end) {
-            z[i] = -__builtin_inff();   // adds nothing
-          } else {
-            const uint64_t k = token_key(z[i], v);
-            best = k > best ? k : best;
-            top = fmaxf(top, z[i]);
-          }
-        }
-        if (top > -__builtin_inff()) {
-          sum *= expf(m - top);
+        for (int i = 1; i < kPer; ++i) top = fmaxf(top, z[i]);
+        const uint32_t key = token(v0, 0, lane) < end ? fkey(top) : 0;
+        chunk_tops[at][lane] = key;
+        most = max(most, key);
+        if (top > m) {
+          sum *= __builtin_amdgcn_exp2f((m - top) * kLog2e);
           m = top;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) sum += expf(z[i] - m);
         }
-        const uint64_t ask = __ballot(best > least);
-        if (!ask) continue;
-        uint64_t bound = least;
-        if (__popcll(ask) > W) {
-          int before = 0;   // lanes whose best is better
-#pragma unroll 8
-          for (int l = 0; l < 64; ++l) before += lane_u64(best, l) > best;
-          const uint64_t at = __ballot(best > least && before == W - 1);
-          bound = lane_u64(best, __ffsll((unsigned long long)at) - 1) - 1;
-        }
-        int n = kept;
+        if (m > -__builtin_inff()) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int v = token(i);
-          const uint64_t k = v < end ? token_key(z[i], v) : 0;
-          const uint64_t in = __ballot(k > bound);
-          if (k > bound) list[n + __popcll(in & ((1ull << lane) - 1))] = k;
-          n += __popcll(in);
+          for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((z[i] - m) * kLog2e);
         }
-        wave_order();
-        // every key's place among all; the first W stay, in order
-        uint64_t mine[(kList + 63) / 64];
-        int place[(kList + 63) / 64];
-#pragma unroll
-        for (int c = 0; c < (kList + 63) / 64; ++c) {
-          const int i = 64 * c + lane;
-          place[c] = W;
-          if (64 * c < n && i < n) {
-            mine[c] = list[i];
-            int p = 0;
-            for (int j = 0; j < n; ++j) p += list[j] > mine[c];
-            place[c] = p;
-          }
+      };
+      for (int v0 = begin, at = 0; v0 < end; v0 += 2 * kChunk, at += 2) {
+        chunk(0, v0, at);
+        if (v0 + kChunk < end) chunk(1, v0 + kChunk, at + 1);
+      }
+      // what a place in the list takes at least: the W-th largest of the lanes' values (0: not so many lanes have one)
+      const uint32_t bound = nth_largest(most, W);
+      uint64_t* list = lds.wave.list[wave];
+      uint16_t* queue = lds.wave.queue[wave];
+      int kept = 0, waiting = 0;
+      uint64_t least = 0;   // a full list's last place
+      auto add = [&](uint64_t key, int& n) {   // one of each lane
+        const bool take = key > least && (uint32_t)(key >> 32) >= bound;
+        const uint64_t some = __ballot(take);
+        if (n + __popcll(some) > 128) {   // no room: what there is, ranked
+          keep_best(list, n, W, lane);
+          n = min(n, W);
+          if (n == W) least = list[W - 1];
         }
-        wave_order();
-#pragma unroll
-        for (int c = 0; c < (kList + 63) / 64; ++c)
-          if (place[c] < W) list[place[c]] = mine[c];
-        wave_order();
+        if (take) list[n + lanes_before(some, lane)] = key;
+        n += __popcll(some);
+      };
+      auto rank = [&](int n) {
+        keep_best(list, n, W, lane);
         kept = min(n, W);
         if (kept == W) least = list[W - 1];
+      };
+      constexpr int kAtOnce = 64 / kSets;
+      if (begin + kChunk >= end) {   // one chunk: its values are still here
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int v = token(begin, i / kSome, lane) + i % kSome;
+          add(v < end ? token_key(z[i], v) : 0, n);
+        }
+        rank(n);
+      } else {
         wave_order();
+        for (int v0 = begin, at = 0; v0 < end; v0 += kChunk, ++at) {
+          const uint32_t top = chunk_tops[at][lane];
+          // (the highest key that the lane's values may have)
+          const bool reaches = top >= bound && top != 0 && (kept < W || token_key(kfloat(top), v0) > least);
+          const uint64_t in = __ballot(reaches);
+          if (reaches) queue[waiting + lanes_before(in, lane)] = (uint16_t)(at * 64 + lane);
+          waiting += __popcll(in);
+          const bool last = v0 + kChunk >= end;
+          // as many lanes' values as a wave reads at once, kSets lanes each
+          while (waiting >= kAtOnce || (last && waiting)) {
+            wave_order();
+            const int now = min(waiting, kAtOnce);
+            const int what = lane / kSets < now ? queue[lane / kSets] : -1;
+            const int move = now + lane < waiting ? queue[now + lane] : 0, move2 = now + 64 + lane < waiting ? queue[now + 64 + lane] : 0;
+            const int v = token(begin + (what >> 6) * kChunk, lane % kSets, what & 63);
+            float y[kSome];
+            if (what >= 0) x.value(x.raw(v, end), x.bits(v, end), y);
+            wave_order();
+            if (now + lane < waiting) queue[lane] = (uint16_t)move;
+            if (now + 64 + lane < waiting) queue[64 + lane] = (uint16_t)move2;
+            waiting -= now;
+            int n = kept;
+#pragma unroll
+            for (int j = 0; j < kSome; ++j) add(what >= 0 && v + j < end ? token_key(y[j], v + j) : 0, n);
+            rank(n);
+          }
+        }
       }
       // the slice's maximum, sum and list
-      float top = m;
-#pragma unroll
-      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-      double s = top == -__builtin_inff() ? 0.0 : (double)sum * exp((double)m - (double)top);
-#pragma unroll
-      for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+      const float top = wave_max_dpp(m);
+      const float s = (float)wave_sum_dpp(top == -__builtin_inff() ? 0.0 : (double)(sum * __builtin_amdgcn_exp2f((m - top) * kLog2e)));
+      uint64_t* part = f.parts + (row * f.slices + slice) * words;
       uint64_t w = 0;
       if (lane < kept) w = list[lane];
-      if (lane < W) __hip_atomic_store(part + 2 + lane, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (lane == 0) {
-        __hip_atomic_store(part, (uint64_t)__float_as_uint(top), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(part + 1, (uint64_t)__double_as_longlong(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      if (lane < W) __hip_atomic_store(part + 1 + lane, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (lane == 0)
+        __hip_atomic_store(part, (uint64_t)__float_as_uint(top) << 32 | __float_as_uint(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   if (!last_to_arrive(f.arrived + group, f.wgs)) return;
 
-  auto get = [](const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  auto& la = lds.last;
-  if (threadIdx.x < W) {
-    la.score[threadIdx.x] = a.score[row0 + threadIdx.x];
-    la.done[threadIdx.x] = a.done ? a.done[row0 + threadIdx.x] : 0;
+  // What this needs of memory is asked for at once: a thread's slice's first places, the sums.
+  const uint64_t* parts = f.parts + row0 * f.slices * words;
+  auto word = [&](int u, int i) { return __hip_atomic_load(parts + (int64_t)u * words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  const int tid = threadIdx.x;
+  uint64_t first[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) first[i] = tid < units && i < W ? word(tid, 1 + i) : 0;
+  // A wave has every fourth row; of up to 64 slices all sums are on their way.
+  constexpr int kRowsOfWave = kBeamWidth / kBeamWaves;
+  const uint64_t none = (uint64_t)__float_as_uint(-__builtin_inff()) << 32;
+  uint64_t stat[kRowsOfWave];
+#pragma unroll
+  for (int i = 0; i < kRowsOfWave; ++i) {
+    const int j = wave + kBeamWaves * i;
+    stat[i] = j < W && lane < f.slices ? word(j * f.slices + lane, 0) : none;
   }
-  __syncthreads();
-  for (int j = wave; j < W; j += kBeamWaves) {   // a wave a row
-    if (la.done[j] || la.score[j] == -__builtin_inff()) continue;
-    const uint64_t* part = f.parts + (row0 + j) * f.slices * words;
-    float top = -__builtin_inff();
-    for (int s = lane; s < f.slices; s += 64) top = fmaxf(top, __uint_as_float((uint32_t)get(part + (int64_t)s * words)));
+  if (tid < W) {
+    score[tid] = a.score[row0 + tid];
+    done[tid] = a.done ? a.done[row0 + tid] : 0;
+  }
+  if (tid == 0) n_found = 0;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  for (int i = 0; i < kRowsOfWave; ++i) {
+    const int j = wave + kBeamWaves * i;
+    if (j >= W) break;   // (of a row whose logits do not matter, whatever there is)
+    float m = -__builtin_inff();
     double sum = 0.0;
-    if (top > -__builtin_inff())
-      for (int s = lane; s < f.slices; s += 64)
-        sum += __longlong_as_double((long long)get(part + (int64_t)s * words + 1)) *
-               exp((double)__uint_as_float((uint32_t)get(part + (int64_t)s * words)) - (double)top);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    if (lane == 0) la.lse[j] = sum > 0.0 ? (double)top + log(sum) : 0.0;
+    for (int s0 = 0; s0 < f.slices; s0 += 64) {
+      if (s0) stat[i] = s0 + lane < f.slices ? word(j * f.slices + s0 + lane, 0) : none;
+      const float mine = __uint_as_float((uint32_t)(stat[i] >> 32)), part = __uint_as_float((uint32_t)stat[i]);
+      const float t = fmaxf(m, wave_max_dpp(mine));
+      if (t == -__builtin_inff()) continue;
+      sum = sum * (double)__builtin_amdgcn_exp2f((m - t) * kLog2e) + wave_sum_dpp((double)(part * __builtin_amdgcn_exp2f((mine - t) * kLog2e)));
+      m = t;
+    }
+    if (lane == 0) {
+      tops[j] = m;
+      logs[j] = sum > 0.0 ? log(sum) : 0.0;
+    }
   }
   __syncthreads();
 
-  // A wave's list from its share of the slices' lists, a place of each a round.
-  Total* list = la.best[wave];
-  int kept = 0;
-  Total least{0.0, -1};
-  const Total none{0.0, -1};
-  for (int place = 0; place < W; ++place) {
-    bool news = false;
-    for (int u0 = wave * 64; u0 < units; u0 += kBeamThreads) {
-      const int u = u0 + lane;
-      Total t = none;
-      if (u < units) {
-        const int j = u / f.slices, slice = u % f.slices;
-        if (la.done[j]) {
-          if (slice == 0 && place == 0) t = Total{(double)la.score[j], j * V + a.stop_token};
-        } else if (la.score[j] == -__builtin_inff()) {
-          if (slice == 0 && place < V) t = Total{-__builtin_inf(), j * V + place};
-        } else {
-          const uint64_t k = get(f.parts + ((row0 + j) * f.slices + slice) * words + 2 + place);
-          if (k) {
-            const float z = key_value(k);
-            t = Total{z == -__builtin_inff() ? -__builtin_inf() : (double)la.score[j] + ((double)z - la.lse[j]), j * V + key_token(k)};
+  // Place `at` of slice u, whose key is k where the row's logits matter.
+  auto total = [&](int u, int at, uint64_t k) {
+    const int j = u / f.slices;
+    if (done[j]) return u == j * f.slices && at == 0 ? total_of(score[j], j * V + a.stop_token) : no_total();
+    if (score[j] == -__builtin_inff()) return u == j * f.slices && at < V ? total_of(-__builtin_inf(), j * V + at) : no_total();
+    if (!k) return no_total();
+    const float z = key_value(k);
+    return total_of(z == -__builtin_inff() ? -__builtin_inf() : (double)score[j] + (((double)z - (double)tops[j]) - logs[j]), j * V + key_token(k));
+  };
+  Total* found = lds.found;
+  {
+    Total mine = no_total();
+    for (int u = tid; u < units; u += kBeamThreads) {
+      const Total t = total(u, 0, u < kBeamThreads ? first[0] : word(u, 1));
+      if (t.beats(mine)) mine = t;
+    }
+    // (of a total's bits the upper half: a bound a little lower does as well)
+    const uint32_t of_wave = nth_largest((uint32_t)(mine.t >> 32), W);
+    if (lane == 0) bounds[wave] = of_wave;
+  }
+  __syncthreads();
+  const uint32_t bound = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+  static_assert(kBeamWaves == 4, "the waves' bounds");
+  for (int u = tid; u < units; u += kBeamThreads) {
+    for (int at0 = 0; at0 < W; at0 += 4) {   // places are in order: behind one that does not reach the bound none does
+      uint64_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = at0 == 0 && u < kBeamThreads ? first[i] : (at0 + i < W ? word(u, 1 + at0 + i) : 0);
+      bool more = true;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Total t = at0 + i < W ? total(u, at0 + i, k[i]) : no_total();
+        more = more && t.at && (uint32_t)(t.t >> 32) >= bound;
+        if (more) {
+          const int n = atomicAdd(&n_found, 1);
+          if (n < kFound) found[n] = t;
+        }
+      }
+      if (!more) break;
+    }
+  }
+  __syncthreads();
+  if (n_found <= kFound) {
+    const int n = n_found;
+    for (int i = tid; i < n; i += kBeamThreads) {
+      const Total mine = found[i];
+      int at = 0;
+      for (int o = 0; o < n; o += 4) {
+        Total x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = found[min(o + k, kFound - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) at += (o + k < n) & x[k].beats(mine);
+      }
+      if (at < W) won[at] = mine;
+    }
+  } else {
+    // too many places reach the bound (lists whose totals hardly differ): the best, the best behind it, and so on
+    Total last = no_total();
+    for (int i = 0; i < W; ++i) {
+      Total mine = no_total();
+      for (int u = threadIdx.x; u < units; u += kBeamThreads)
+        for (int at = 0; at < W; ++at) {
+          const Total t = total(u, at, word(u, 1 + at));
+          if (!t.at) break;
+          if (i == 0 || last.beats(t)) {
+            if (t.beats(mine)) mine = t;
+            break;
           }
         }
+      __syncthreads();
+      found[threadIdx.x] = mine;
+      __syncthreads();
+      for (int d = kBeamThreads / 2; d; d /= 2) {
+        if ((int)threadIdx.x < d && found[threadIdx.x + d].beats(found[threadIdx.x])) found[threadIdx.x] = found[threadIdx.x + d];
+        __syncthreads();
       }
-      if (!(t.t == t.t)) t.t = -__builtin_inf();   // so that all totals have an order
-      const bool in = t.beats(kept == W ? least : none);
-      const uint64_t ask = __ballot(in);
-      if (!ask) continue;
-      news = true;
-      if (in) list[kept + __popcll(ask & ((1ull << lane) - 1))] = t;
-      const int n = kept + __popcll(ask);
-      wave_order();
-      Total mine[2];
-      int at[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int i = 64 * c + lane;
-        at[c] = W;
-        if (i < n) {
-          mine[c] = list[i];
-          at[c] = 0;
-          for (int o = 0; o < n; ++o) at[c] += list[o].beats(mine[c]);
-        }
-      }
-      wave_order();
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (at[c] < W) list[at[c]] = mine[c];
-      wave_order();
-      kept = min(n, W);
-      least = list[kept - 1];
-      wave_order();
-    }
-    if (!news) break;   // lists are in order: deeper places are worse
-  }
-  if (lane == 0) la.counts[wave] = kept;
-  __syncthreads();
-  {
-    // the waves' lists: every total's place among all
-    const int i = threadIdx.x % kBeamWidth, w = threadIdx.x / kBeamWidth;
-    if (w < kBeamWaves && i < la.counts[w]) {
-      const Total mine = la.best[w][i];
-      int at = 0;
-      for (int o = 0; o < kBeamWaves; ++o)
-        for (int p = 0; p < la.counts[o]; ++p) at += la.best[o][p].beats(mine);
-      if (at < W) la.won[at] = mine;
+      last = found[0];
+      if (threadIdx.x == 0) won[i] = last;
+      __syncthreads();
     }
   }
   __syncthreads();
-  Total won{0.0, 0};
-  int parent = 0, token = 0;
-  bool was = false;
-  if (threadIdx.x < W) {
-    won = la.won[threadIdx.x];
-    parent = won.at / V;
-    token = won.at - parent * V;
-    was = la.done[parent];
-  }
-  __syncthreads();   // (the states' columns lie where the totals did)
-  uint32_t* column = lds.column;
-  const int cols = kBeamWidth * kBeamThreads / W / kBeamThreads * kBeamThreads;   // columns at a time
-  if (threadIdx.x < W) {
-    const int64_t r = row0 + threadIdx.x;
-    parents[threadIdx.x] = parent;
+  if (tid < W) {
+    const Total t = won[tid];
+    const int at = (int)~t.at, parent = at / V, token = at - parent * V;
+    const int64_t r = row0 + tid;
     a.out_parent[r] = parent;
     a.out_token[r] = token;
-    a.out_score[r] = (float)won.t;
-    if (a.out_done) a.out_done[r] = was || token == a.stop_token;
-  }
-  __syncthreads();
-  auto carry = [&](const uint32_t* src, int64_t ld_src, uint32_t* dst, int64_t ld_dst, int64_t n) {
-    for (int64_t c0 = 0; c0 < n; c0 += cols) {
-      for (int c = threadIdx.x; c < cols && c0 + c < n; c += kBeamThreads)
-        for (int j = 0; j < W; ++j) column[j * cols + c] = src[(row0 + j) * ld_src + c0 + c];
-      for (int c = threadIdx.x; c < cols && c0 + c < n; c += kBeamThreads)
-        for (int j = 0; j < W; ++j) dst[(row0 + j) * ld_dst + c0 + c] = column[parents[j] * cols + c];
-    }
-  };
-  for (int i = 0; i < a.n_states; ++i) {
-    const c4s_beam_state& s = a.states[i];
-    carry(static_cast<const uint32_t*>(s.src), s.ld_src, static_cast<uint32_t*>(s.dst), s.ld_dst, s.words);
-  }
-  if (a.hist_bits) {
-    const int64_t n = (V + 31) / 32;
-    carry(a.hist_bits, n, a.out_hist_bits, n, n);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the rows are written
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (threadIdx.x < W && !was && token != a.stop_token) {
-      uint32_t* word = a.out_hist_bits + (row0 + threadIdx.x) * n + token / 32;
-      *word |= 1u << (token % 32);
-    }
+    a.out_score[r] = (float)total_value(t);
+    if (a.out_done) a.out_done[r] = done[parent] || token == a.stop_token;
+    if (f.joined) f.joined[r] = done[parent] || token == a.stop_token ? -1 : token;
   }
 }
 
-// How a row is cut: into slices for 4096 waves together, sixteen a CU, of at least a chunk.
+// A workgroup has a group's rows over 256 columns of the history and the states, in this order.
+__global__ __launch_bounds__(kBeamThreads) void k_beam_states(BeamArgs f) {
+  __shared__ uint32_t column[kBeamWidth][kBeamThreads];
+  __shared__ int parents[kBeamWidth], tokens[kBeamWidth];
+  const c4s_beam& a = f.a;
+  const int tid = threadIdx.x, W = a.width;
+  const int64_t row0 = (int64_t)(blockIdx.x / f.state_wgs) * W;
+  int64_t c = (int64_t)(blockIdx.x % f.state_wgs) * kBeamThreads + tid;
+  const uint32_t* src = nullptr;
+  uint32_t* dst = nullptr;
+  int64_t ld_src = 0, ld_dst = 0;
+  int hist = -1;   // the word of the history that this is
+  if (a.hist_bits) {
+    const int64_t words = (a.vocab + 31) / 32;
+    if (c < words) {
+      src = a.hist_bits + c, dst = a.out_hist_bits + c;
+      ld_src = ld_dst = words;
+      hist = (int)c;
+    }
+    c -= words;
+  }
+  for (int i = 0; i < a.n_states; ++i) {
+    const c4s_beam_state& s = a.states[i];
+    if (c >= 0 && c < s.words) {
+      src = static_cast<const uint32_t*>(s.src) + c, dst = static_cast<uint32_t*>(s.dst) + c;
+      ld_src = s.ld_src, ld_dst = s.ld_dst;
+    }
+    c -= s.words;
+  }
+  if (tid < W) {
+    parents[tid] = a.out_parent[row0 + tid];
+    tokens[tid] = f.joined[row0 + tid];
+  }
+  if (src) {
+    for (int j0 = 0; j0 < W; j0 += 8) {   // eight rows' reads on their way
+      uint32_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = src[(row0 + min(j0 + j, W - 1)) * ld_src];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < W) column[j0 + j][tid] = v[j];
+    }
+  }
+  __syncthreads();
+  if (!src) return;
+  for (int j = 0; j < W; ++j) {
+    uint32_t v = column[parents[j]][tid];
+    if (hist >= 0 && tokens[j] >= 0 && tokens[j] / 32 == hist) v |= 1u << (tokens[j] % 32);
+    dst[(row0 + j) * ld_dst] = v;
+  }
+}
+
+// How a row is cut: into slices for 4096 waves together, sixteen a CU, of 1 to kMostChunks chunks.
 BeamArgs beam_args(const c4s_beam& a) {
   BeamArgs f{};
   f.a = a;
   const int64_t rows = (int64_t)a.n_groups * a.width, chunks = (a.vocab + kChunk - 1) / kChunk;
-  const int64_t slices = std::min(std::max<int64_t>(4096 / rows, 1), chunks);
+  const int64_t slices = std::max(std::min(std::max<int64_t>(4096 / rows, 1), chunks), (chunks + kMostChunks - 1) / kMostChunks);
   f.chunks = (int)((chunks + slices - 1) / slices);
   f.slices = (int)((chunks + f.chunks - 1) / f.chunks);
   f.wgs = (a.width * f.slices + kBeamWaves - 1) / kBeamWaves;
+  int64_t words = a.hist_bits ? (a.vocab + 31) / 32 : 0;
+  for (int i = 0; i < a.n_states; ++i) words += a.states[i].words;
+  f.state_wgs = (int)((words + kBeamThreads - 1) / kBeamThreads);
   return f;
 }
 
@@ -374,16 +523,20 @@ BeamArgs beam_args(const c4s_beam& a) {
 
 LayerSpace beam_space(const c4s_beam& a) {
   const BeamArgs f = beam_args(a);
-  return {a.n_groups, (int64_t)a.n_groups * a.width * f.slices * (2 + a.width) * 2};
+  return {a.n_groups, (int64_t)a.n_groups * a.width * (f.slices * (1 + a.width) * 2 + 1)};
 }
 
 hipError_t launch_beam(const c4s_beam& a, uint32_t* counters, float* space, hipStream_t s) {
   BeamArgs f = beam_args(a);
   f.arrived = counters;
   f.parts = reinterpret_cast<uint64_t*>(space);
+  f.joined = f.state_wgs ? reinterpret_cast<int32_t*>(f.parts + (int64_t)a.n_groups * a.width * f.slices * (1 + a.width)) : nullptr;
   const dim3 grid((unsigned)(a.n_groups * f.wgs)), block(kBeamThreads);
   if (a.dtype == C4S_DTYPE_BF16) hipLaunchKernelGGL(k_beam<true>, grid, block, 0, s, f);
   else hipLaunchKernelGGL(k_beam<false>, grid, block, 0, s, f);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || f.state_wgs == 0) return e;
+  hipLaunchKernelGGL(k_beam_states, dim3((unsigned)((int64_t)a.n_groups * f.state_wgs)), block, 0, s, f);
   return hipGetLastError();
 }
 

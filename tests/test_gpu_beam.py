@@ -110,6 +110,12 @@ def test_infinities(gpu_ctx):
     _check(gpu_ctx, z, 4, score, done=np.ones(8), stop=299)
     got = _run(gpu_ctx, np.full((2, 3), -np.inf, np.float32), 2, np.zeros(2, np.float32))
     assert got[0].tolist() == [0, 0] and got[1].tolist() == [0, 1] and np.isneginf(got[2]).all()
+    low = np.full((4, 5000), np.finfo(np.float32).min, np.float32)    # masked by the type's lowest value: a row alone, and whole rows
+    low[0, 70], low[1, ::1700] = 2.0, -3.0
+    got = _check(gpu_ctx, low, 4, np.array([-1, -2, -30, -0.5], np.float32))
+    assert got[0].tolist() == [0, 1, 1, 1]
+    _check(gpu_ctx, torch.from_numpy(low).to(torch.bfloat16).cuda(), 2, np.array([-1, -2, -30, -0.5], np.float32))
+    _check(gpu_ctx, -low, 4, np.array([-1, -2, -30, -0.5], np.float32))
     one = np.full((3, 40), -np.inf, np.float32)
     one[:, 11] = 4.0             # log-probability 0
     got = _check(gpu_ctx, one, 3, np.array([-1, -2, -3], np.float32), stop=11)
