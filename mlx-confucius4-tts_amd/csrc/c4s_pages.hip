@@ -2,8 +2,12 @@
 //
 // Handing out is one workgroup's work: sums over the sequences of the pages that
 // each needs, then a walk over the words of free bits, in which every free page
-// finds its number among all, and by it its sequence and table entry. Nothing
-// depends on the order in which threads come, so tables are the same in every run.
+// finds its number among all. The pages pass through LDS in that order, so that
+// all threads share in handing them out. (With each thread handing out what its words
+// hold, 1000 sequences' 17000 pages took 71 us, and the 150 of 256 beams, all from a
+// few words, 52.)
+// Who shares a last page with whom is found in a hash table in LDS. Nothing depends on
+// the order in which threads come, so tables are the same in every run.
 // All of it is latency: a step's call is a chain of a few dependent reads.
 
 #include <hip/hip_runtime.h>
@@ -17,17 +21,6 @@ namespace {
 
 constexpr int kGrowThreads = 1024;
 
-__device__ __forceinline__ int32_t count_of(const int32_t* refs, int page) {
-  return __hip_atomic_load(refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// Waits until this wave's writes and atomics are done, for all that the workgroup does behind the barrier.
-__device__ __forceinline__ void barrier_after_memory() {
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
-  __syncthreads();
-}
-
 __device__ __forceinline__ int wave_prefix(int v) {   // inclusive
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -37,21 +30,26 @@ __device__ __forceinline__ int wave_prefix(int v) {   // inclusive
   return v;
 }
 
-// Sums before this thread over the workgroup, and over all of it. Every thread calls it.
+// Sums before this thread over the workgroup, and over all of it, of two numbers. Every thread calls it, and
+// between two calls with one `which` there is a barrier.
 struct Prefix {
-  int waves[2][kGrowThreads / 64];
-  __device__ __forceinline__ int operator()(int v, int* total, int which) {
-    const int in = wave_prefix(v), wave = threadIdx.x / 64;
+  int2 waves[2][kGrowThreads / 64];
+  __device__ __forceinline__ int2 operator()(int2 v, int2* total, int which) {
+    const int2 in = make_int2(wave_prefix(v.x), wave_prefix(v.y));
+    const int wave = threadIdx.x / 64;
     if (threadIdx.x % 64 == 63) waves[which][wave] = in;
     __syncthreads();
-    int before = 0, sum = 0;
+    int2 before = make_int2(0, 0), sum = before;
 #pragma unroll
     for (int w = 0; w < kGrowThreads / 64; ++w) {
-      before += w < wave ? waves[which][w] : 0;
-      sum += waves[which][w];
+      const int2 o = waves[which][w];
+      before.x += w < wave ? o.x : 0;
+      before.y += w < wave ? o.y : 0;
+      sum.x += o.x;
+      sum.y += o.y;
     }
     *total = sum;
-    return before + in - v;
+    return make_int2(before.x + in.x - v.x, before.y + in.y - v.y);
   }
 };
 
@@ -65,14 +63,28 @@ struct GrowArgs {
   int shift;
 };
 
+constexpr int kHash = 2 * kPagesSeqs;   // places of the table of shared pages
+constexpr int kBatch = 16384;           // pages in LDS at a time
+
 __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
-  __shared__ int32_t off[kPagesSeqs + 1];   // pages asked for by the sequences before
-  __shared__ int32_t last[kPagesSeqs];      // a last page that must not be written: its number; -1: none
+  __shared__ union {
+    struct {
+      int32_t page[kHash], users[kHash], last[kHash];   // a shared page (-1: none), how many go on, the last of them
+    } hash;
+    struct {
+      int32_t off[kPagesSeqs + 1];   // pages asked for by the sequences before
+      int32_t page[kBatch];          // free pages in order
+      uint4 words[kGrowThreads];     // the free bits that are looked at,
+      int32_t before[kGrowThreads];  // and how many free pages lie before each four words
+    } give;
+  } lds;
+  __shared__ int32_t lens[kPagesSeqs];
+  __shared__ int32_t here[kPagesSeqs];    // the page of a sequence's first new token, where there is one
+  __shared__ int32_t old[kPagesSeqs];     // a last page that must not be written; -1: none
   __shared__ Prefix prefix;
-  __shared__ int any_shared;
   const c4s_pages& p = f.p;
   const c4s_grow& g = f.g;
-  const int tid = threadIdx.x, n = p.n_seqs, shift = f.shift, ps = 1 << shift;
+  const int tid = threadIdx.x, lane = tid % 64, n = p.n_seqs, shift = f.shift, ps = 1 << shift;
   const int words = (p.n_pages + 31) / 32;
   // the free bits' first words are underway while the sequences are looked at
   uint4 bits = make_uint4(0, 0, 0, 0);
@@ -89,52 +101,57 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
 
   auto pages_of = [&](int64_t tokens) { return (int)min((tokens + ps - 1) >> shift, (int64_t)p.max_pages); };
   auto news_of = [&](int b) { return g.n_new ? max(g.n_new[b], 0) : 1; };
-  auto len_of = [&](int b) { return max(p.lens[b], 0); };
+  auto is_page = [&](int page) { return page >= 0 && page < p.n_pages; };
 
-  if (g.copies) {
-    if (tid == 0) any_shared = 0;
-    __syncthreads();
-    for (int b = tid; b < n; b += kGrowThreads) {
-      const int len = len_of(b), at = len >> shift;
-      int page = -1;
-      if ((len & (ps - 1)) && at < p.max_pages && news_of(b) > 0) {
-        page = p.block_table[b * p.table_ld + at];
-        if (page < 0 || page >= p.n_pages || count_of(p.refs, page) < 2) page = -1;
-      }
-      last[b] = page;
-      if (page >= 0) any_shared = 1;
-      reinterpret_cast<int2*>(g.copies)[b] = make_int2(-1, -1);
-    }
-    __syncthreads();
-    if (any_shared) {
-      // Every sharer gives up its hold; a page that none is left of stays with the last of them, whose
-      // number (+ 1) is the largest that the count is raised to.
-      for (int b = tid; b < n; b += kGrowThreads)
-        if (last[b] >= 0) atomicSub(p.refs + last[b], 1);
-      barrier_after_memory();
-      for (int b = tid; b < n; b += kGrowThreads) {   // kept by others: 0 .. - 1 is no page and stays so
-        const int page = last[b];
-        if (page >= 0 && count_of(p.refs, page) != 0) last[b] = page | 1 << 30;
-      }
-      barrier_after_memory();
-      for (int b = tid; b < n; b += kGrowThreads)
-        if (last[b] >= 0 && !(last[b] >> 30)) atomicMax(p.refs + last[b], b + 1);
-      barrier_after_memory();
-      for (int b = tid; b < n; b += kGrowThreads)
-        if (last[b] >= 0 && !(last[b] >> 30) && count_of(p.refs, last[b]) == b + 1) last[b] = -2 - last[b];
-      barrier_after_memory();
-      for (int b = tid; b < n; b += kGrowThreads) {
-        if (last[b] < -1) {
-          __hip_atomic_store(p.refs - 2 - last[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          last[b] = -1;
-        } else if (last[b] >= 0) {
-          last[b] &= (1 << 30) - 1;
-        }
-      }
-    }
-  } else {
-    for (int b = tid; b < n; b += kGrowThreads) last[b] = -1;
+  if (g.copies)
+    for (int i = tid; i < kHash; i += kGrowThreads) lds.hash.page[i] = -1, lds.hash.users[i] = 0, lds.hash.last[i] = -1;
+  for (int b = tid; b < n; b += kGrowThreads) {
+    const int len = max(p.lens[b], 0), at = len >> shift;
+    lens[b] = len;
+    here[b] = (len & (ps - 1)) && at < p.max_pages ? p.block_table[b * p.table_ld + at] : -1;
+    old[b] = -1;
   }
+  if (g.copies) {
+    // Pages of several holders that are about to be written: who has them, and of those who go on the last. If they
+    // are all the holders, the last keeps the page; the others give up their hold on it.
+    __syncthreads();
+    constexpr int kMine = kPagesSeqs / kGrowThreads;
+    int place[kMine], holders[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int b = tid + i * kGrowThreads;
+      place[i] = -1;
+      holders[i] = 0;
+      if (b < n && is_page(here[b]) && news_of(b) > 0) holders[i] = p.refs[here[b]];
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if (holders[i] < 2) continue;
+      const int b = tid + i * kGrowThreads, page = here[b];
+      int at = (int)((uint32_t)page * 2654435761u >> 19);   // 13 bits
+      static_assert(kHash == 1 << 13, "the hash's bits");
+      for (;;) {   // there are more places than sequences
+        const int was = atomicCAS(&lds.hash.page[at], -1, page);
+        if (was == -1 || was == page) break;
+        at = (at + 1) % kHash;
+      }
+      place[i] = at;
+      atomicAdd(&lds.hash.users[at], 1);
+      atomicMax(&lds.hash.last[at], b);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int b = tid + i * kGrowThreads;
+      if (b >= n) break;
+      reinterpret_cast<int2*>(g.copies)[b] = make_int2(-1, -1);
+      if (place[i] < 0 || (lds.hash.users[place[i]] == holders[i] && lds.hash.last[place[i]] == b)) continue;
+      old[b] = here[b];
+      here[b] = -1;
+      atomicSub(p.refs + old[b], 1);
+    }
+  }
+  __syncthreads();
 
   int64_t rows = 0;   // of the sequences before these
   int asked = 0;
@@ -142,81 +159,125 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
   for (int b0 = 0; b0 < n; b0 += kGrowThreads) {
     const int b = b0 + tid;
     int need = 0, fresh = 0;
-    int64_t len = 0;
     if (b < n) {
-      len = len_of(b);
+      const int64_t len = lens[b];
       fresh = news_of(b);
-      const int64_t whole = (len + fresh + ps - 1) >> shift;
-      need = pages_of(len + fresh) - pages_of(len) + (last[b] >= 0);
-      lost += (int)(whole - ((len + ps - 1) >> shift) - (pages_of(len + fresh) - pages_of(len)));
+      const int more = pages_of(len + fresh) - pages_of(len);
+      need = more + (old[b] >= 0);
+      lost += (int)(((len + fresh + ps - 1) >> shift) - ((len + ps - 1) >> shift)) - more;
     }
-    int sum;
-    const int before = prefix(need, &sum, 0);
-    if (b < n) off[b] = asked + before;
-    asked += sum;
-    if (g.rows_off) {
-      int fresh_sum;
-      const int fresh_before = prefix(fresh, &fresh_sum, 1);
-      if (b < n) g.rows_off[b] = (int32_t)(rows + fresh_before);
-      rows += fresh_sum;
+    int2 sum;
+    const int2 before = prefix(make_int2(need, fresh), &sum, 0);
+    if (b < n) {
+      lds.give.off[b] = asked + before.x;
+      if (g.rows_off) g.rows_off[b] = (int32_t)(rows + before.y);
     }
+    asked += sum.x;
+    rows += sum.y;
     __syncthreads();
   }
   if (tid == 0) {
-    off[n] = asked;
+    lds.give.off[n] = asked;
     if (g.rows_off) g.rows_off[n] = (int32_t)rows;
   }
   __syncthreads();
 
-  // Table entry number `rank` of those asked for.
-  auto give = [&](int rank, int page) {
-    int lo = 0, hi = n;   // the last sequence that begins at or before it (those that ask for none begin with the next)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (off[mid] <= rank) lo = mid;
-      else hi = mid;
+  // The pages asked for from number `first` on, `count` of them, -1 where there are none, into sequence b's entries:
+  // those with numbers begin .. end - 1 and every step-th.
+  auto put = [&](int b, int begin, int end, int step, int first, bool there) {
+    const int off = lds.give.off[b], own = old[b] >= 0, len = lens[b];
+    int32_t* row = p.block_table + b * p.table_ld;
+    if (begin >= end) return;
+    if (begin == off) {
+      const int page = there ? lds.give.page[begin - first] : -1;
+      here[b] = page;
+      if (own) {
+        row[len >> shift] = page;
+        if (page >= 0) reinterpret_cast<int2*>(g.copies)[b] = make_int2(old[b], page);
+        begin += step;
+      }
     }
-    const int own = last[lo] >= 0, nth = rank - off[lo], len = len_of(lo);
-    const int at = own && nth == 0 ? len >> shift : pages_of(len) + nth - own;
-    p.block_table[lo * p.table_ld + at] = page;
-    if (own && nth == 0 && page >= 0) reinterpret_cast<int2*>(g.copies)[lo] = make_int2(last[lo], page);
+    row += pages_of(len) - own - off;
+    for (int rank = begin; rank < end; rank += step) row[rank] = there ? lds.give.page[rank - first] : -1;
+  };
+  // Few: a page a thread, which searches its sequence; many: sixteen threads a sequence, which write its entries next to
+  // each other.
+  auto give = [&](int first, int count, bool there) {
+    if (count <= 2 * kGrowThreads) {
+      for (int i = tid; i < count; i += kGrowThreads) {
+        int lo = 0, hi = n;   // the last sequence that begins at or before it (those that ask for none begin with the next)
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (lds.give.off[mid] <= first + i) lo = mid;
+          else hi = mid;
+        }
+        put(lo, first + i, first + i + 1, 1, first, there);
+      }
+    } else {
+      for (int b = tid / 16; b < n; b += kGrowThreads / 16)
+        put(b, max(lds.give.off[b], first) + tid % 16, min(lds.give.off[b + 1], first + count), 16, first, there);
+    }
   };
   int found = 0;
-  for (int w0 = 0; w0 < words && found < asked; w0 += 4 * kGrowThreads) {
+  for (int w0 = 0, turn = 0; w0 < words && found < asked; w0 += 4 * kGrowThreads, ++turn) {
     const int word = w0 + 4 * tid;
-    if (w0) load_bits(word);
     uint32_t v[4] = {bits.x, bits.y, bits.z, bits.w};
-    int sum;
-    int rank = found + prefix(__popc(v[0]) + __popc(v[1]) + __popc(v[2]) + __popc(v[3]), &sum, w0 / (4 * kGrowThreads) & 1);
-    found += sum;
+    if (w0 + 4 * kGrowThreads < words) load_bits(word + 4 * kGrowThreads);
+    int2 sum;
+    const int mine = found + prefix(make_int2(__popc(v[0]) + __popc(v[1]) + __popc(v[2]) + __popc(v[3]), 0), &sum, turn & 1).x;
+    const int upto = min(found + sum.x, asked);
+    lds.give.words[tid] = make_uint4(v[0], v[1], v[2], v[3]);
+    lds.give.before[tid] = mine;
+    __syncthreads();
+    for (int first = found; first < upto; first += kBatch) {
+      const int count = min(upto - first, kBatch);
+      // a wave takes every sixteenth four words, two at a time, a lane a bit (a thread on its own words' bits would write
+      // as many places apart: all lanes in one bank)
+      constexpr int kWaves = kGrowThreads / 64;
+      const int q = lane * kWaves + tid / 64, q_before = lds.give.before[q], q_next = q + 1 < kGrowThreads ? lds.give.before[q + 1] : found + sum.x;
+      uint64_t lanes = __ballot(q_before < first + count && q_next > first);
+      while (lanes) {
+        const int l = __ffsll((unsigned long long)lanes) - 1, at4 = l * kWaves + tid / 64;
+        lanes &= lanes - 1;
+        const uint4 w = lds.give.words[at4];
+        int rank = lds.give.before[at4] - first;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const uint64_t pair = i ? (uint64_t)w.w << 32 | w.z : (uint64_t)w.y << 32 | w.x;
+          const int at = rank + __popcll(pair & ((1ull << lane) - 1));
+          if ((pair >> lane & 1) && at >= 0 && at < count) lds.give.page[at] = 32 * (w0 + 4 * at4 + i) + lane;
+          rank += __popcll(pair);
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < count; i += kGrowThreads) p.refs[lds.give.page[i]] = 1;
+      give(first, count, true);
+      __syncthreads();
+    }
+    int rank = mine;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t left = v[i];
-      while (left && rank < asked) {
-        const int page = 32 * (word + i) + __ffs(left) - 1;
-        left &= left - 1;
-        if (page >= p.n_pages) break;
-        p.refs[page] = 1;
-        give(rank++, page);
-      }
-      if (left != v[i]) p.free_bits[word + i] = left;
+      const int have = __popc(v[i]), taken = min(max(upto - rank, 0), have);
+      rank += have;
+      if (!taken) continue;
+      uint32_t left = taken == have ? 0 : v[i];
+      for (int t = 0; left && t < taken; ++t) left &= left - 1;
+      p.free_bits[word + i] = left;
     }
+    found += sum.x;
   }
-  for (int rank = found + tid; rank < asked; rank += kGrowThreads) give(rank, -1);
+  if (found < asked) give(found, asked - found, false);
   if (p.missing) {
     if (lost) atomicAdd(p.missing, lost);
     if (tid == 0 && asked > found) atomicAdd(p.missing, asked - found);
   }
-  barrier_after_memory();   // every table entry is written, every length read
+  __syncthreads();
   for (int b = tid; b < n; b += kGrowThreads) {
-    const int len = len_of(b), fresh = news_of(b);
-    p.lens[b] = (int32_t)min((int64_t)len + fresh, (int64_t)INT32_MAX);
+    const int len = lens[b];
+    p.lens[b] = (int32_t)min((int64_t)len + news_of(b), (int64_t)INT32_MAX);
     if (!g.n_new && b < g.n_rows) {   // row b: the sequence's one new token
       if (g.row_pos) g.row_pos[b] = len;
-      if (g.row_slot) {
-        const int at = len >> shift, page = at < p.max_pages ? p.block_table[b * p.table_ld + at] : -1;
-        g.row_slot[b] = page < 0 || page >= p.n_pages ? -1 : (page << shift) + (len & (ps - 1));
-      }
+      if (g.row_slot) g.row_slot[b] = is_page(here[b]) ? (here[b] << shift) + (len & (ps - 1)) : -1;
     }
   }
 }
@@ -294,31 +355,36 @@ __global__ __launch_bounds__(kForkThreads) void k_pages_fork(c4s_pages p, const 
 // ---- pages copied ---------------------------------------------------------------------
 
 struct CopyArgs {
-  const char* tensor[4];   // keys, values and their scales; bytes of a page of each, all multiples of 16
-  uint32_t units[4];       // of 16 bytes
+  char* tensor[4];         // keys, values and their scales
+  uint32_t begin[5];       // their units of 16 bytes in a page, one behind the other
   const int32_t* copies;
   int n_pages;
 };
 
-// A workgroup copies a part of a pair's 16-byte units, four of a thread's in flight.
+typedef uint32_t Unit __attribute__((ext_vector_type(4)));
+
+// A workgroup copies 1024 of a pair's units, a thread's four together on their way.
 __global__ __launch_bounds__(256) void k_kv_copy(CopyArgs f) {
   const int2 pair = reinterpret_cast<const int2*>(f.copies)[blockIdx.y];
   if (pair.x < 0 || pair.x >= f.n_pages || pair.y < 0 || pair.y >= f.n_pages || pair.x == pair.y) return;
+  for (uint32_t first = blockIdx.x * 1024; first < f.begin[4]; first += 1024 * gridDim.x) {
+    Unit v[4];
+    char* to[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t n = f.units[t];
-    const uint4* from = reinterpret_cast<const uint4*>(f.tensor[t]) + (uint64_t)pair.x * n;
-    uint4* to = reinterpret_cast<uint4*>(const_cast<char*>(f.tensor[t])) + (uint64_t)pair.y * n;
-    const uint32_t step = 256 * gridDim.x;
-    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 4 * step) {
-      uint4 v[4];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-        if (i + j * step < n) v[j] = from[i + j * step];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j)
-        if (i + j * step < n) to[i + j * step] = v[j];
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t i = first + 256 * j + threadIdx.x;
+      const bool there = i < f.begin[4];   // (else the first unit, which is not written)
+      const int t = there ? (i >= f.begin[1]) + (i >= f.begin[2]) + (i >= f.begin[3]) : 0;
+      const uint32_t begin = t == 0 ? 0 : (t == 1 ? f.begin[1] : (t == 2 ? f.begin[2] : f.begin[3]));
+      const uint32_t end = t == 0 ? f.begin[1] : (t == 1 ? f.begin[2] : (t == 2 ? f.begin[3] : f.begin[4]));
+      char* tensor = t == 0 ? f.tensor[0] : (t == 1 ? f.tensor[1] : (t == 2 ? f.tensor[2] : f.tensor[3]));
+      const uint64_t bytes = 16ull * (end - begin), at = there ? 16ull * (i - begin) : 0;
+      v[j] = *reinterpret_cast<const Unit*>(tensor + pair.x * bytes + at);
+      to[j] = there ? tensor + pair.y * bytes + at : nullptr;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (to[j]) *reinterpret_cast<Unit*>(to[j]) = v[j];
   }
 }
 
@@ -355,10 +421,9 @@ hipError_t launch_kv_copy(const KvArgs& c, const int32_t* copies, int n, hipStre
   const uint64_t page = c.store == C4S_KV_BF16 ? 2 * values : (c.store == C4S_KV_Q8 ? values : values / 2);
   const uint64_t scales = c.store == C4S_KV_BF16 ? 0 : (c.store == C4S_KV_Q8 ? 4 * rows : rows * (c.dim / 32));
   const uint32_t a = (uint32_t)(page / 16), b = (uint32_t)(scales / 16);
-  const CopyArgs f{{static_cast<const char*>(c.k), static_cast<const char*>(c.v), reinterpret_cast<const char*>(c.k_scale),
-                    reinterpret_cast<const char*>(c.v_scale)}, {a, a, b, b}, copies, c.n_pages};
-  // a part is 1024 units of the keys, up to as many parts as a grid has room for
-  hipLaunchKernelGGL(k_kv_copy, dim3(std::min<uint32_t>((a + 1023) / 1024, 4096), n), dim3(256), 0, s, f);
+  const CopyArgs f{{static_cast<char*>(c.k), static_cast<char*>(c.v), reinterpret_cast<char*>(c.k_scale), reinterpret_cast<char*>(c.v_scale)},
+                   {0, a, 2 * a, 2 * a + b, 2 * a + 2 * b}, copies, c.n_pages};
+  hipLaunchKernelGGL(k_kv_copy, dim3(std::min<uint32_t>((2 * a + 2 * b + 1023) / 1024, 4096), n), dim3(256), 0, s, f);
   return hipGetLastError();
 }
 
