@@ -118,6 +118,16 @@ int c4s_linear(c4s_ctx* ctx, const c4s_linear_desc* lin, void* stream);
  * of which code * scale is the value: scale = max |row| / 127, code =
  * round to even(value / scale); a row of zeros has scale 0. A row with a value
  * that is not finite reads back as NaN.
+ * C4S_KV_Q4: e2m1 codes (a sign, then 0, 0.5, 1, 1.5, 2, 3, 4 or 6), two a byte, and
+ * a byte e for every 32 dims of a position and head, their scale 2^(e - 127):
+ *   k        [n_pages][n_kv_heads][page_size][head_dim / 2]   dims 2 i (low) and 2 i + 1
+ *   v        [n_pages][n_kv_heads][head_dim / 2][page_size]   likewise
+ *   k_scale, v_scale  uint8 [n_pages][n_kv_heads][head_dim / 32][page_size].
+ * The scale is the least of which the greatest magnitude of the 32 is at most six
+ * times as large (2^-127 at least), a code the nearest (of two the even one); the 32
+ * read back as NaN where one is not finite (e = 255). All values are bf16 numbers but 4
+ * or 6 times 2^126, which read back as infinite, or count in c4s_attn as what they are.
+ * There values of a scale of 2^-127 may count as 0.
  * (The values lie with their positions next to each other because that is how
  * the product of weights and values reads them: no transpose in the decode.)
  *

@@ -98,6 +98,18 @@ __device__ __forceinline__ float sum4(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Over the wave.
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return max4(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+  return sum4(v);
+}
+
 // Dwords of two bf16, of which those at index lo .. hi - 1 stay and the others become zero.
 __device__ __forceinline__ uint4 keep(uint4 w, int at, int lo, int hi) {
   uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -160,6 +172,7 @@ constexpr int kRows = 16;   // rows of a workgroup
 // The weights enter the second product as bf16 pairs (hi + lo, about 2^-17
 // relative), which costs nothing here: rounded once to bf16 they would add an
 // error of the size of the output's own rounding.
+constexpr float kFewSlack = 8.0f;   // with up to four rows: the greatest weight stays between 2^-kFewSlack and 1
 constexpr int kWaves = 4;
 constexpr int kAttnThreads = 64 * kWaves;
 constexpr int kMaxParts = 128;       // chunks of a sequence
@@ -173,9 +186,20 @@ struct FewArgs {
 };
 
 // DH: the head's dims rounded up to 64, 128 or 256; FULL: they are that many.
-template <int DH, int STORE, bool FULL, int KEYS>
+//
+// With 4-bit pages the bytes are so few that the VALU is what bounds it, and of a matrix's 16 columns a token of a
+// head of its own fills one. For up to four rows (ROWS) the first product is therefore K's on the right, S = Q K^T, with
+// the rows repeated four times: each lane group has all of a tile's scores, and takes those of another tile, so that
+// a lane has one position's scores, of ROWS rows. What the weights are relative to lies up to 2^kFewSlack above the
+// greatest, so that a vote finds nothing to do in most blocks, sums stay a lane's own until the end, and the values'
+// scales join the weights, a product a row and block of 32 dims (a scale of 2^-127 counts as 0 there); the weights then
+// go through LDS, as pairs of bf16 for each such block, into the second product's operand. The codes themselves need no
+// scale there: two positions' bytes give a dim's pair by an exchange of nibbles and one conversion. 64 rows of 50 to 1500
+// positions, 20 heads of 64: 18.0 us (as with more rows 22.4; its 36 MB in 6.4); 64 of 4000, 5 heads of 256: 95 (119).
+template <int DH, int STORE, bool FULL, int KEYS, int ROWS>
 __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) void k_attn_few(FewArgs f) {
   constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
+  static_assert(ROWS == 0 || (Q4 && KEYS == 64 && ROWS <= 4), "few rows of 4-bit pages");
   constexpr int kSteps = DH / 32, kTiles = DH / 16, kNT = KEYS / 16, kOwn = KEYS / 4;   // kOwn: a lane's positions of a block
   constexpr int kKLoads = Q8 ? kNT * kSteps / 2 : kNT * kSteps, kVLoads = Q8 || KEYS == 32 ? kTiles : 2 * kTiles;
   __shared__ float sm[kWaves][kRows], sl[kWaves][kRows];
@@ -203,7 +227,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   const int n_all = sq.n_new * a.shared, r0 = tile * kRows;
   if (r0 >= n_all) return;
   const int valid = min(kRows, n_all - r0);
-  const int r = r0 + min(c, valid - 1);
+  const int r = r0 + min(ROWS ? c % 4 : c, valid - 1);
   auto token_of = [&](int r) { return a.shared == 1 ? r : r / a.shared; };
   const int token = token_of(r), qh = head * a.shared + r - token * a.shared;
   const int lim = min(sq.past + token + 1, sq.cap);                            // this row sees positions before it
@@ -216,6 +240,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
 
   constexpr int k4Dims = DH == 64 ? 16 : 32, k4Steps = k4Dims / 8, k4Parts = kSteps / k4Steps;   // 4 bits: a lane's dims of a key in one piece; pieces
   uint4 q[kSteps];
+  const uint32_t turn = ROWS && a.scale < 0.0f ? 0x80008000u : 0u;
   {
     const uint16_t* qp = a.q + (int64_t)(sq.row0 + token) * a.ldq + qh * dim;
 #pragma unroll
@@ -223,6 +248,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       // codes come 16 dims a lane at a time, which are two steps of 8; in 4 bits up to 32 dims, a block of one scale
       const int d = Q4 ? k4Dims * (s / k4Steps * 4 + g) + 8 * (s % k4Steps) : (Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g);
       q[s] = FULL || d < dim ? *reinterpret_cast<const uint4*>(qp + d) : make_uint4(0, 0, 0, 0);
+      if constexpr (ROWS > 0) q[s] = make_uint4(q[s].x ^ turn, q[s].y ^ turn, q[s].z ^ turn, q[s].w ^ turn);
     }
   }
   const float c2 = a.scale * kLog2e;
@@ -243,9 +269,9 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   float ks[Q8 ? kOwn : 1], vs[Q8 ? kOwn : 1];
   // 4 bits: codes of keys and of pairs of dims, and a byte a position for each one's block
   constexpr int kOwnWords = kOwn / 4;
-  uint32_t k4[Q4 ? kNT : 1][Q4 ? kSteps : 1], ke[Q4 ? k4Parts : 1][Q4 ? kOwnWords : 1];
-  uint32_t v4[Q4 ? kSteps : 1][Q4 ? kOwnWords : 1], ve[Q4 ? kSteps : 1][Q4 ? kOwnWords : 1];
-  auto own_words = [&](uint32_t (&to)[Q4 ? kOwnWords : 1], const char* p) {
+  uint32_t k4[Q4 && !ROWS ? kNT : 1][Q4 && !ROWS ? kSteps : 1], ke[Q4 && !ROWS ? k4Parts : 1][Q4 ? kOwnWords : 1];
+  uint32_t v4[Q4 && !ROWS ? kSteps : 1][Q4 ? kOwnWords : 1], ve[Q4 && !ROWS ? kSteps : 1][Q4 ? kOwnWords : 1];
+  auto own_words = [](uint32_t (&to)[Q4 ? kOwnWords : 1], const char* p) {
     if constexpr (Q4 && kOwn == 16) {
       const uint4 w = *reinterpret_cast<const uint4*>(p);
       to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
@@ -257,7 +283,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   auto load_keys = [&](int t, const Pages& p) {   // scores of what has no page are dropped
     const uint32_t at = (uint32_t)((t + kOwn * (c / 4)) & (ps - 1)) * (uint32_t)(wide * kSize);
     const char* k = kbase + (uint64_t)(uint32_t)max(p.k, 0) * page_bytes + at;
-    if constexpr (Q4) {
+    if constexpr (Q4 && !ROWS) {
       const char* e = reinterpret_cast<const char*>(a.c.k_scale) + (uint64_t)(uint32_t)max(p.k, 0) * scale_bytes +
                       (uint32_t)(((head * (dim / 32)) << shift) + ((t + kOwn * (c / 4)) & (ps - 1)));
 #pragma unroll
@@ -298,7 +324,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   auto load_values = [&](int t, const Pages& p) {
     const uint32_t at = (uint32_t)((t + kOwn * g) & (ps - 1));
     const char* v = vbase + (uint64_t)(uint32_t)max(p.v, 0) * page_bytes + at * kSize;
-    if constexpr (Q4) {
+    if constexpr (Q4 && !ROWS) {
       const char* e = reinterpret_cast<const char*>(a.c.v_scale) + (uint64_t)(uint32_t)max(p.v, 0) * scale_bytes + ((uint32_t)(head * (dim / 32)) << shift) + at;
 #pragma unroll
       for (int d = 0; d < kSteps; ++d) {
@@ -342,9 +368,175 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   __syncthreads();
   int t = begin + wave * KEYS;
   if (t < end) {
-    Pages now = pages_of(t);
-    load_keys(t, now);
-    load_values(t, now);
+    if constexpr (ROWS > 0) {
+      // A block's codes, and its scales' bytes: of the keys as the lane has them, of the values for the lane's position.
+      // (With two or three blocks on their way there are fewer waves, and it is slower: 6 rows of 12000 to 50001, heads of
+      // 128, 47 us with one, 56 and 59; 64 of 50 to 1500, heads of 64, 18.0, 20.4 and 21.9.)
+      struct Block {
+        uint32_t k[4][kSteps], ke[k4Parts][4], v[kSteps][4];
+        uint8_t ve[kSteps];
+        bool there;             // whether that position has a page
+      } b;
+      const int one = 16 * (c / 4) + 4 * g + c % 4;   // this lane's position of a block
+      auto load_k = [&](int t, const Pages& p) {
+        const uint32_t at = (uint32_t)((t + 16 * (c / 4)) & (ps - 1));
+        const char* k = kbase + (uint64_t)(uint32_t)max(p.k, 0) * page_bytes + at * (uint32_t)wide;
+        const char* e = reinterpret_cast<const char*>(a.c.k_scale) + (uint64_t)(uint32_t)max(p.k, 0) * scale_bytes + ((uint32_t)(head * (dim / 32)) << shift) + at;
+#pragma unroll
+        for (int part = 0; part < k4Parts; ++part) {
+          int d = k4Dims * (4 * part + g);
+          if (!FULL && d >= dim) d = part ? 32 * g : 0;   // times zeros of q
+          own_words(b.ke[part], e + (uint32_t)((d / 32) << shift));
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            const char* w = k + (4 * tt * dim + d) / 2;
+            if constexpr (k4Steps == 4) {
+              const uint4 x = *reinterpret_cast<const uint4*>(w);
+              b.k[tt][4 * part] = x.x, b.k[tt][4 * part + 1] = x.y, b.k[tt][4 * part + 2] = x.z, b.k[tt][4 * part + 3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(w);
+              b.k[tt][0] = x.x, b.k[tt][1] = x.y;
+            }
+          }
+        }
+      };
+      auto load_v = [&](int t, const Pages& p) {
+        const char* v = vbase + (uint64_t)(uint32_t)max(p.v, 0) * page_bytes + (uint32_t)((t + 16 * g) & (ps - 1));
+        const uint8_t* e = reinterpret_cast<const uint8_t*>(a.c.v_scale) + (uint64_t)(uint32_t)max(p.k, 0) * scale_bytes +
+                           ((uint32_t)(head * (dim / 32)) << shift) + (uint32_t)((t + one) & (ps - 1));
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          b.ve[d] = *e;
+          if (FULL || 32 * (d + 1) < dim) e += ps;   // blocks behind the last dim are not used
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          own_words(b.v[d], v);
+          if (FULL || 32 * (d + 1) < dim) v += tile_bytes;
+        }
+        b.there = p.k >= 0;
+      };
+      {
+        const Pages first = pages_of(t);
+        load_k(t, first);
+        load_v(t, first);
+      }
+      uint16_t* weights = reinterpret_cast<uint16_t*>(&so[wave][0][0]);   // [block of dims][high, low][row][72]
+      static_assert(sizeof(so) / kWaves >= kSteps * 2 * ROWS * 72 * 2, "the weights in LDS");
+      auto weight_at = [&](int d, int low, int row, int at) { return weights + ((d * 2 + low) * ROWS + row) * 72 + at; };
+      const int slot = (one & ~7) + ((one & 3) << 1) + (one >> 2 & 1);    // a conversion's two codes are four positions apart
+      const float c2p = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-100f);          // (q has the sign)
+      float top_m[ROWS], sum[ROWS];
+      int lims[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        top_m[i] = -__builtin_inff();
+        sum[i] = 0.0f;
+        lims[i] = min(sq.past + token_of(r0 + min(i, valid - 1)) + 1, sq.cap);
+      }
+      for (; t < end; t += kStride) {
+        f32x4 s = {};
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          f32x4 x = {};
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            const uint4 w = codes4(b.k[tt][st], scale4(b.ke[st / k4Steps][tt] >> 8 * (c % 4) << 23));
+            x = mfma(q[st], w, x);
+          }
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) s[i] = tt == 0 || g == tt ? x[i] : s[i];
+        }
+        const bool there = b.there;
+        const int pos = t + one;
+        const bool edge = t < fst || t + KEYS > min(least, end) || __any(!there);
+        uint32_t seen[ROWS];   // all bits, or none
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          seen[i] = ~0u;
+          if (edge) {
+            const bool sees = there & (pos >= fst) & (pos < min(lims[i], end));
+            seen[i] = sees ? ~0u : 0u;
+            s[i] = sees ? s[i] : -__builtin_inff();
+          }
+        }
+        float scales[kSteps];
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) scales[d] = !FULL && 32 * d >= dim ? 0.0f : (b.ve[d] == 255 ? __builtin_nanf("") : __uint_as_float((uint32_t)b.ve[d] << 23));
+        __builtin_amdgcn_sched_barrier(0);
+        const int tn = t + kStride < end ? t + kStride : t;   // (behind the last block that one again, as below)
+        const Pages ahead = pages_of(tn);
+        load_k(tn, ahead);
+        __builtin_amdgcn_sched_barrier(0);
+        float worst = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) worst = fmaxf(worst, s[i] * c2p - top_m[i]);
+        if (__any(worst > 0.0f)) {   // seldom, after the first block
+          float olds[ROWS];
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const float top = fmaxf(wave_max(s[i]) * c2p + kFewSlack, top_m[i]);
+            olds[i] = __builtin_amdgcn_exp2f(top_m[i] - (top == -__builtin_inff() ? 0.0f : top));
+            sum[i] *= olds[i];
+            top_m[i] = top;
+          }
+          float old = olds[0];   // of column c's row
+#pragma unroll
+          for (int i = 1; i < ROWS; ++i) old = c >= i ? olds[i] : old;
+#pragma unroll
+          for (int d = 0; d < kTiles; ++d) o[d] *= old;
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2p, -(top_m[i] == -__builtin_inff() ? 0.0f : top_m[i])));
+          sum[i] += p;
+#pragma unroll
+          for (int d = 0; d < kSteps; ++d) {
+            const float w = __uint_as_float(__float_as_uint(p * scales[d]) & seen[i]);   // what is not seen may have any scale
+            const uint32_t both = pack(w, 0.0f);
+            *weight_at(d, 0, i, slot) = (uint16_t)both;
+            *weight_at(d, 1, i, slot) = (uint16_t)pack(w - low(both), 0.0f);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const int row = min(c, ROWS - 1);
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint32_t x = b.v[d][2 * st], y = b.v[d][2 * st + 1];
+            const uint4 even = codes4((x & 0x0F0F0F0Fu) | (y << 4 & 0xF0F0F0F0u), 1.0f), odd = codes4((x >> 4 & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), 1.0f);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              const uint4 w = *reinterpret_cast<const uint4*>(weight_at(d, part, row, 16 * g + 8 * st));
+              o[2 * d] = mfma(even, w, o[2 * d]);
+              o[2 * d + 1] = mfma(odd, w, o[2 * d + 1]);
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(tn, ahead);
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const float all = wave_sum(sum[i]);
+        if (lane == i) {   // as the lanes of column i have them below
+          m = top_m[i];
+          l = all;
+        }
+      }
+    }
+    Pages now{};
+    if constexpr (ROWS == 0) {
+      now = pages_of(t);
+      load_keys(t, now);
+      load_values(t, now);
+    }
     for (; t < end; t += kStride) {
       f32x4 s[kNT] = {};
 #pragma unroll
@@ -419,23 +611,24 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
       __builtin_amdgcn_sched_barrier(0);
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
       if constexpr (Q4) {
+        // What is not there or not for any row may hold anything: the smallest scale, with which every code is finite.
+        // Where some of the rows see a position and others do not, values that are not finite are taken out, as of
+        // bf16 pages below; only the three largest scales can have such.
+        bool strange = false;
         if (edge) {
-          // What is not there or not for any row may hold anything, and a block that is not finite is for those rows
-          // alone that see it: its scale becomes one that is, and those rows' results NaN, at whatever weight.
           const int any_to = there ? min(kend, end) - vt : 0;
+          uint32_t high = 0;
 #pragma unroll
-          for (int d = 0; d < kSteps; ++d) {
-            float strange = 0.0f;
+          for (int w = 0; w < kOwnWords; ++w) {
+            auto bytes = [&](int n) { return n >= 4 ? ~0u : (n <= 0 ? 0u : (1u << 8 * n) - 1u); };   // the first n
+            const uint32_t stay = bytes(any_to - 4 * w) & ~bytes(from - 4 * w);
 #pragma unroll
-            for (int j = 0; j < kOwn; ++j) {
-              const bool bad = (ve[d][j / 4] >> 8 * (j % 4) & 255u) == 255u;
-              if (bad && sees(j)) strange = __builtin_nanf("");
-              if (bad || j < from || j >= any_to) ve[d][j / 4] &= ~(255u << 8 * (j % 4));
+            for (int d = 0; d < kSteps; ++d) {
+              ve[d][w] &= stay;
+              high |= ((ve[d][w] & 0x7F7F7F7Fu) + 0x03030303u) & ve[d][w];   // a byte's top bit: it is 253 or more
             }
-            strange = sum4(strange);
-            o[2 * d] += strange;
-            o[2 * d + 1] += strange;
           }
+          strange = least != kend && __any((high & 0x80808080u) != 0);
         }
 #pragma unroll
         for (int d = 0; d < kSteps; ++d) {
@@ -443,12 +636,29 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
           for (int st = 0; st < KEYS / 32; ++st) {
             uint32_t x = v4[d][2 * st], y = v4[d][2 * st + 1];
             asm volatile("" : "+v"(x), "+v"(y));
-            uint4 even, odd;
-            pairs4(make_uint2(x, y), make_uint2(ve[d][2 * st], ve[d][2 * st + 1]), even, odd);
-            o[2 * d] = mfma(even, quad(hi + 4 * st), o[2 * d]);
-            o[2 * d + 1] = mfma(odd, quad(hi + 4 * st), o[2 * d + 1]);
-            o[2 * d] = mfma(even, quad(lo + 4 * st), o[2 * d]);
-            o[2 * d + 1] = mfma(odd, quad(lo + 4 * st), o[2 * d + 1]);
+            uint4 v[2];
+            pairs4(make_uint2(x, y), make_uint2(ve[d][2 * st], ve[d][2 * st + 1]), v[0], v[1]);
+            if (strange) {
+              uint32_t mine[4];   // ones where this row sees
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mine[j] = (sees(8 * st + 2 * j) ? 0x3F80u : 0u) | (sees(8 * st + 2 * j + 1) ? 0x3F800000u : 0u);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                uint4 ones;
+                part_odd(v[i].x, ones.x);
+                part_odd(v[i].y, ones.y);
+                part_odd(v[i].z, ones.z);
+                part_odd(v[i].w, ones.w);
+                const f32x4 seen = mfma(ones, quad(mine), f32x4{});
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                  if (seen[u] != 0.0f) o[2 * d + i][u] = __builtin_nanf("");
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[2 * d + i] = mfma(v[i], quad(hi + 4 * st), o[2 * d + i]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[2 * d + i] = mfma(v[i], quad(lo + 4 * st), o[2 * d + i]);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -512,7 +722,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   }
 
   // The waves' parts: of output quad (row, dims 4 i ..) by the thread that has it.
-  l = sum4(l);
+  if constexpr (ROWS == 0) l = sum4(l);
   if (g == 0) {
     sm[wave][c] = m;
     sl[wave][c] = l;
@@ -619,23 +829,25 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
 // or more, into 2048 (they even out what the lengths do not). Measured, in us,
 // for 512 / 1024 / 2048: 64 rows of 1024, 8 heads of 128: 54 / 72 / 68 (8-bit 32
 // / 41 / 44); 8 rows of 2000, 20 heads of 64: 17.7 / 18.5 / 19.9; 6 rows of 12000
-// to 50001, 8 heads of 128, 8-bit: 95 / 94 / 87.
+// to 50001, 8 heads of 128, 8-bit: 95 / 94 / 87. With 4-bit pages, of half the bytes, pieces of 2560: the last 46 us
+// (with 1280 48), 64 of 4000, 5 heads of 256, 95 (107).
 FewArgs few_args(const AttnArgs& a) {
   FewArgs f{};
   f.a = a;
   f.tiles = (int)(((int64_t)a.max_new * a.shared + kRows - 1) / kRows);
   const int64_t cap = (int64_t)a.c.max_pages << a.c.page_shift, groups = (int64_t)f.tiles * a.c.n_heads * a.c.n_seqs;
   const int64_t coarse = std::max<int64_t>(512 / groups, 1), fine = std::max<int64_t>(2048 / groups, 1);
-  int64_t chunk = std::min(cap / coarse, std::max<int64_t>(1280, cap / fine)) + 255;
+  const int64_t least = a.c.store == C4S_KV_Q4 ? 2560 : 1280;
+  int64_t chunk = std::min(cap / coarse, std::max<int64_t>(least, cap / fine)) + 255;
   chunk = std::max(chunk, (cap + kMaxParts - 1) / kMaxParts + 255) / 256 * 256;
   f.chunk = (int)std::min<int64_t>(std::max<int64_t>(chunk, 256), (int64_t)kMaxPages << a.c.page_shift);
   f.splits = (int)std::max<int64_t>((cap + f.chunk - 1) / f.chunk, 1);
   return f;
 }
 
-template <int DH, int STORE, bool FULL, int KEYS>
+template <int DH, int STORE, bool FULL, int KEYS, int ROWS = 0>
 hipError_t few(const FewArgs& f, hipStream_t s) {
-  hipLaunchKernelGGL((k_attn_few<DH, STORE, FULL, KEYS>), dim3((unsigned)((int64_t)f.tiles * f.splits * f.a.c.n_heads), f.a.c.n_seqs),
+  hipLaunchKernelGGL((k_attn_few<DH, STORE, FULL, KEYS, ROWS>), dim3((unsigned)((int64_t)f.tiles * f.splits * f.a.c.n_heads), f.a.c.n_seqs),
                      dim3(kAttnThreads), 0, s, f);
   return hipGetLastError();
 }
@@ -643,7 +855,13 @@ template <int DH, int BKEYS, int QKEYS, int HKEYS>   // positions a block: bf16,
 hipError_t few_by_store(const FewArgs& f, hipStream_t s) {
   const bool full = f.a.c.dim == DH;
   if (f.a.c.store == C4S_KV_Q8) return full ? few<DH, C4S_KV_Q8, true, QKEYS>(f, s) : few<DH, C4S_KV_Q8, false, QKEYS>(f, s);
-  if (f.a.c.store == C4S_KV_Q4) return full ? few<DH, C4S_KV_Q4, true, HKEYS>(f, s) : few<DH, C4S_KV_Q4, false, HKEYS>(f, s);
+  if (f.a.c.store == C4S_KV_Q4) {
+    const int64_t rows = (int64_t)f.a.max_new * f.a.shared;   // of a sequence and key head
+    if (rows <= 1) return full ? few<DH, C4S_KV_Q4, true, 64, 1>(f, s) : few<DH, C4S_KV_Q4, false, 64, 1>(f, s);
+    if (rows <= 2) return full ? few<DH, C4S_KV_Q4, true, 64, 2>(f, s) : few<DH, C4S_KV_Q4, false, 64, 2>(f, s);
+    if (rows <= 4) return full ? few<DH, C4S_KV_Q4, true, 64, 4>(f, s) : few<DH, C4S_KV_Q4, false, 64, 4>(f, s);
+    return full ? few<DH, C4S_KV_Q4, true, HKEYS>(f, s) : few<DH, C4S_KV_Q4, false, HKEYS>(f, s);
+  }
   return full ? few<DH, C4S_KV_BF16, true, BKEYS>(f, s) : few<DH, C4S_KV_BF16, false, BKEYS>(f, s);
 }
 
@@ -1087,10 +1305,13 @@ hipError_t many_by_store(const AttnArgs& a, hipStream_t s) {
 // 50. 8-bit codes are converted for each block of the many rows' kernel by all its waves: 20 heads of 64: 4 of 128 over
 // 1000, 640, 21 / 30; 2 of 600, 1520, 17.9 / 18.9; 4 of 300 over 500, 1520, 27 / 24; 64 of 48 and of 64 over 300,
 // three and four tiles a sequence, 35 / 39 and 45 / 42; 8 heads of 128: 2 of 200 over 1000, 800, 43 / 65; 2 of 400 over 400, 1600, 48 / 48; 5 heads of 256: 4
-// of 200 over 200, 500, 30 / 29; 4 of 500 over 500, 1260, 107 / 59.
+// of 200 over 200, 500, 30 / 29; 4 of 500 over 500, 1260, 107 / 59. 4-bit codes, 20 heads of 64: 4 of 128 over 1000, 640,
+// 16 / 23; 2 of 600, 1520, 15.2 / 15.5; 4 of 300 over 500, 1520, 21 / 19; 64 of 48 over 300, three tiles a sequence, 29 / 33; 8 heads
+// of 128: 2 of 400 over 400, 1600, 35 / 38; 4 of 300 over 500, 2400, 51 / 39; 5 heads of 256: 64 of 17 over 300, 640, 30 / 34;
+// 64 of 48 over 300, 960, 41 / 41.
 bool many_pays(const AttnArgs& a) {
   const int64_t tiles = ((int64_t)a.max_new * a.shared + kRows - 1) / kRows, all = tiles * a.c.n_heads * a.c.n_seqs;
-  if (a.c.store == C4S_KV_Q8 && a.c.dim <= 128) return tiles > 3 && all > 1500;
+  if (a.c.store != C4S_KV_BF16 && a.c.dim <= 128) return tiles > 3 && all > 1500;
   return tiles > 1 && all > 700;
 }
 

@@ -139,6 +139,8 @@ PROMPTS = [  # new, past, heads, kv_heads, dim, page
     ([70, 140], [7, 120], 40, 40, 256, 16),
     ([61, 17, 40], [64, 1000, 0], 64, 16, 192, 256),
     ([40, 3], [0, 50], 4, 4, 64, 16),
+    ([210, 1, 64, 70, 129], [0, 150, 17, 3, 63], 24, 24, 64, 16),
+    ([100, 31, 97, 5], [29, 0, 200, 300], 80, 20, 96, 128),
 ]
 
 
@@ -168,7 +170,7 @@ def test_attn_first(gpu_ctx, new, past, first, heads):
     _check_attn(cache, q, out, lse, new, 2 * heads, first=first, prompts=True)
 
 
-@pytest.mark.parametrize("n,past,heads", [(4, 70, 2), (100, 3, 2), (40, 200, 2), (700, 3, 20), (3, 600, 2)])
+@pytest.mark.parametrize("n,past,heads", [(4, 70, 2), (100, 3, 2), (40, 200, 2), (700, 3, 20), (3, 600, 2), (700, 3, 40)])
 def test_attn_later_rows_do_not_reach_earlier_ones(gpu_ctx, n, past, heads):
     """Blocks that are not finite in later positions: a value's own dims, and all of a row whose key it is."""
     mk = lambda: B.Cache4([n + past], heads, 64, 16, seed=6)  # noqa: E731
@@ -187,7 +189,7 @@ def test_attn_later_rows_do_not_reach_earlier_ones(gpu_ctx, n, past, heads):
 
 def test_attn_a_value_that_is_not_finite_at_no_weight(gpu_ctx):
     """Rows that see it are NaN in its dims also where its weight underflows."""
-    for n in (1, 4, 300):
+    for n in (1, 4, 300, 700):
         heads = 2 if n < 100 else 40
         cache = B.Cache4([n + 200], heads, 64, 16, seed=7)
         cache.spoil("v", 0, 3, 1, 0)
@@ -205,7 +207,7 @@ def test_attn_a_value_that_is_not_finite_at_no_weight(gpu_ctx):
         assert torch.isnan(out[:, 1, :32]).all() and torch.isfinite(out[:, 1, 32:]).all() and torch.isfinite(out[:, 0]).all()
 
 
-@pytest.mark.parametrize("heads,new", [(2, [1, 1, 20]), (20, [200, 30, 150])])
+@pytest.mark.parametrize("heads,new", [(2, [1, 1, 20]), (20, [200, 30, 150]), (60, [200, 30, 150])])
 def test_attn_missing_pages(gpu_ctx, heads, new):
     cache = B.Cache4([300, 30, 150], heads, 64, 16, seed=8, junk=True)
     cache.table[0, 3:7] = -1
