@@ -139,8 +139,8 @@ int c4s_kv_copy(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* copies, 
  * temperature, as c4s_sample_rows applies them, every row r = g * width + j offers its
  * group for every token v the total
  *   score[r] + z[v] - log sum_u exp z[u]
- * (in 64 bits; -inf where score or z is, and where it would be NaN), a row that is done only its stop token, with
- * its score as it is. The `width` largest totals of a group, equal ones by the lowest
+ * (in 64 bits; -inf where score or z is, and where it would be NaN, as for all of a row with NaN or +inf among its
+ * z), a row that is done only its stop token, with its score as it is. The `width` largest totals of a group, equal ones by the lowest
  * (j, v), become its rows: parent j, token v, out_score the total, out_done whether the
  * parent was done or v is the stop token.
  * hist_bits and the states are carried along: row g * width + i of each output is row

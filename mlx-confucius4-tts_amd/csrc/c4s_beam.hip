@@ -235,6 +235,9 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
         if (m > -__builtin_inff()) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((z[i] - m) * kLog2e);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) sum = z[i] != z[i] ? z[i] : sum;   // NaN among the logits is NaN here
         }
       };
       for (int v0 = begin, at = 0; v0 < end; v0 += 2 * kChunk, at += 2) {
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       }
       // the slice's maximum, sum and list
       const float top = wave_max_dpp(m);
-      const float s = (float)wave_sum_dpp(top == -__builtin_inff() ? 0.0 : (double)(sum * __builtin_amdgcn_exp2f((m - top) * kLog2e)));
+      const float s = (float)wave_sum_dpp((double)(m == top ? sum : sum * __builtin_amdgcn_exp2f((m - top) * kLog2e)));
       uint64_t* part = f.parts + (row * f.slices + slice) * words;
       uint64_t w = 0;
       if (lane < kept) w = list[lane];
@@ -346,13 +349,13 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       if (s0) stat[i] = s0 + lane < f.slices ? word(j * f.slices + s0 + lane, 0) : none;
       const float mine = __uint_as_float((uint32_t)(stat[i] >> 32)), part = __uint_as_float((uint32_t)stat[i]);
       const float t = fmaxf(m, wave_max_dpp(mine));
-      if (t == -__builtin_inff()) continue;
-      sum = sum * (double)__builtin_amdgcn_exp2f((m - t) * kLog2e) + wave_sum_dpp((double)(part * __builtin_amdgcn_exp2f((mine - t) * kLog2e)));
+      const double more = wave_sum_dpp((double)(mine == t ? part : part * __builtin_amdgcn_exp2f((mine - t) * kLog2e)));
+      sum = (m == t ? sum : sum * (double)__builtin_amdgcn_exp2f((m - t) * kLog2e)) + more;
       m = t;
     }
     if (lane == 0) {
       tops[j] = m;
-      logs[j] = sum > 0.0 ? log(sum) : 0.0;
+      logs[j] = sum == 0.0 ? 0.0 : log(sum);
     }
   }
   __syncthreads();
@@ -361,7 +364,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   auto total = [&](int u, int at, uint64_t k) {
     const int j = u / f.slices;
     if (done[j]) return u == j * f.slices && at == 0 ? total_of(score[j], j * V + a.stop_token) : no_total();
-    if (score[j] == -__builtin_inff()) return u == j * f.slices && at < V ? total_of(-__builtin_inf(), j * V + at) : no_total();
+    if (!(score[j] > -__builtin_inff()) | (logs[j] != logs[j])) return u == j * f.slices && at < V ? total_of(-__builtin_inf(), j * V + at) : no_total();
     if (!k) return no_total();
     const float z = key_value(k);
     return total_of(z == -__builtin_inff() ? -__builtin_inf() : (double)score[j] + (((double)z - (double)tops[j]) - logs[j]), j * V + key_token(k));

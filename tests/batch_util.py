@@ -230,7 +230,9 @@ def beams(logits, width, score, done=None, stop=-1, temp=None, pen=None, bits=No
                 offered[j, stop], total[j, stop] = True, score[r]
             elif score[r] > -np.inf and z[r].max() > -np.inf:
                 x = z[r].astype(np.float64)
-                total[j] = np.float64(score[r]) + ((x - x.max()) - np.log(np.exp(x - x.max()).sum()))   # (the log counts beside 1e38 too)
+                with np.errstate(invalid="ignore"):
+                    t = np.float64(score[r]) + ((x - x.max()) - np.log(np.exp(x - x.max()).sum()))   # (the log counts beside 1e38 too)
+                total[j] = np.where(np.isnan(t), -np.inf, t)
         at = np.flatnonzero(offered)
         best = at[np.argsort(-total.reshape(-1)[at], kind="stable")[:width]]
         for i, c in enumerate(best):

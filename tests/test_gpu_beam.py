@@ -122,6 +122,25 @@ def test_infinities(gpu_ctx):
     assert got[2].tolist() == [-1, -2, -3] and got[3].all()
 
 
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_what_is_not_a_number(gpu_ctx, vocab):
+    """Rows with NaN or +inf anywhere, alone or beside masked tokens, and such scores: no total but -inf."""
+    r = np.random.default_rng(9)
+    for bad in (math.nan, -math.nan, math.inf):
+        for at in (0, 17, vocab - 1):
+            z = r.standard_normal((12, vocab)).astype(np.float32)
+            z[1, at] = z[6, at] = bad
+            z[4] = -np.inf
+            z[4, at] = bad                # beside nothing but masked tokens
+            z[8:] = bad                   # nothing else in the group
+            score = r.standard_normal(12).astype(np.float32)
+            _check(gpu_ctx, z, 4, score)
+            _check(gpu_ctx, torch.from_numpy(z).to(torch.bfloat16).cuda(), 3, score)
+            _check(gpu_ctx, z, 4, score, done=np.arange(12) % 3 == 0, stop=5)
+            score[5] = score[8] = math.nan
+            _check(gpu_ctx, z, 4, score)
+
+
 def test_strides_and_alignment(gpu_ctx):
     """Rows that start anywhere, wider than the vocabulary; states with strides; what lies behind is left alone."""
     r = np.random.default_rng(7)
