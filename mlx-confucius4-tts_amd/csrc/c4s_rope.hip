@@ -2,9 +2,14 @@
 //
 // A workgroup has one row, or a part of its heads: its first threads turn the
 // position into cosines and sines, once for all heads, and leave them in LDS
-// while every thread's first piece of queries or keys is on its way. A piece is
+// while every thread's first pieces of queries or keys are on their way. A piece is
 // eight bf16 or four floats (of either half of the pairs, with C4S_ROPE_HALF), or
-// single pairs where sizes or alignment do not allow that.
+// single pairs where sizes or alignment do not allow that. Memory bounds it: loads and
+// stores go past the L2, where nothing would be found again (the next call's
+// workgroups are on other dies). 18829 rows in place, halves, on memory that is in no
+// cache: 32 and 8 heads of 128 67 us, 5.8 TB/s; 20 and 20 of 64, whose halves are half a line each, 44 us, 4.4 TB/s
+// (through the L2 59; one piece of a thread at a time 47; lines whole and the halves
+// exchanged between lanes 48; workgroups of two or four rows 44). 64 rows: 2.9 us.
 //
 // The angle is reduced in 64 bits: position * frequency / 2 pi, less its whole
 // turns, has an absolute error of 2^-52 of the number of turns; the rest, at most
@@ -51,6 +56,20 @@ struct alignas(N <= 2 ? sizeof(T) : sizeof(T) * N) Few {
   T v[N];
 };
 
+constexpr int kRopeThreads = 256, kRopeAhead = 2;   // pieces of a thread that are on their way together
+
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+template <class V>
+__device__ __forceinline__ V get(const V* from) {
+  if constexpr (sizeof(V) == 16) return __builtin_bit_cast(V, __builtin_nontemporal_load(reinterpret_cast<const Words*>(from)));
+  else return *from;
+}
+template <class V>
+__device__ __forceinline__ void put(V* to, const V& v) {
+  if constexpr (sizeof(V) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words, v), reinterpret_cast<Words*>(to));
+  else *to = v;
+}
+
 struct RopeArgs {
   c4s_rope_desc d;
   int parts;   // workgroups of a row
@@ -58,12 +77,12 @@ struct RopeArgs {
 
 // T: of the tensors; N: values a piece; PAIRS: the layout.
 template <class T, int N, bool PAIRS>
-__global__ __launch_bounds__(256) void k_rope(RopeArgs f) {
+__global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
   __shared__ float cs[kRopePairs], sn[kRopePairs];
   const c4s_rope_desc& a = f.d;
   const int row = blockIdx.x / f.parts, part = blockIdx.x % f.parts;
   const int half = a.rot_dim / 2;
-  const int turned = PAIRS ? a.rot_dim / N : half / N;          // pieces of a head that are turned; the others
+  const int turned = (PAIRS ? a.rot_dim : half) / N;  // pieces of a head that are turned; the others
   const int per = turned + (a.head_dim - a.rot_dim) / N;        // (copied) follow them
   const int heads = (a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0), all = heads * per;
   const int step = blockDim.x * f.parts;
@@ -71,7 +90,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs f) {
   struct Piece {
     const T* from;
     T* to;
-    int pair;    // the first one it has; -1: copied
+    int at;    // its first value's place in the head; -1: copied
   };
   auto piece = [&](int i) {
     const int head = i / per, p = i - head * per;
@@ -81,18 +100,23 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs f) {
     const T* from = static_cast<const T*>(is_q ? a.q : a.k) + r * (is_q ? a.ldq : a.ldk) + (int64_t)h * a.head_dim;
     T* to = static_cast<T*>(is_q ? a.q_out : a.k_out) + r * (is_q ? a.ldq_out : a.ldk_out) + (int64_t)h * a.head_dim;
     const int at = p < turned ? p * N : a.rot_dim + (p - turned) * N;
-    return Piece{from + at, to + at, p < turned ? (PAIRS ? at / 2 : at) : -1};
+    return Piece{from + at, to + at, p < turned ? at : -1};
   };
   using V = Few<T, N>;
-  int i = part * blockDim.x + threadIdx.x;
-  Piece now{};
-  V x{}, y{};
-  auto load = [&] {
-    now = piece(i);
-    x = *reinterpret_cast<const V*>(now.from);
-    if (!PAIRS && now.pair >= 0) y = *reinterpret_cast<const V*>(now.from + half);
+  Piece now[kRopeAhead];
+  V x[kRopeAhead], y[kRopeAhead];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kRopeAhead; ++u) {
+      const int i = i0 + u * step;
+      if (i >= all) continue;
+      now[u] = piece(i);
+      x[u] = get(reinterpret_cast<const V*>(now[u].from));
+      if (!PAIRS && now[u].at >= 0) y[u] = get(reinterpret_cast<const V*>(now[u].from + half));
+    }
   };
-  if (i < all) load();
+  int i = part * blockDim.x + threadIdx.x;
+  load(i);
 
   const int64_t pos = position_of(a, row);
   if (pos < 0) return;
@@ -106,30 +130,36 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs f) {
   }
   __syncthreads();
   while (i < all) {
-    if (now.pair < 0) {
-      if (now.to != now.from) *reinterpret_cast<V*>(now.to) = x;
-    } else if (PAIRS) {
+#pragma unroll
+    for (int u = 0; u < kRopeAhead; ++u) {
+      if (i + u * step >= all) continue;
+      const int at = now[u].at;
+      T* const to = now[u].to;
       V o;
+      if (at < 0) {
+        if (to != now[u].from) put(reinterpret_cast<V*>(to), x[u]);
+      } else if constexpr (PAIRS) {
 #pragma unroll
-      for (int j = 0; j < N; j += 2) {
-        const float c = cs[now.pair + j / 2], s = sn[now.pair + j / 2], u = (float)x.v[j], w = (float)x.v[j + 1];
-        o.v[j] = (T)(u * c - w * s);
-        o.v[j + 1] = (T)(u * s + w * c);
-      }
-      *reinterpret_cast<V*>(now.to) = o;
-    } else {
-      V o, e;
+        for (int j = 0; j < N; j += 2) {
+          const float c = cs[(at + j) / 2], s = sn[(at + j) / 2], v = (float)x[u].v[j], w = (float)x[u].v[j + 1];
+          o.v[j] = (T)(v * c - w * s);
+          o.v[j + 1] = (T)(v * s + w * c);
+        }
+        put(reinterpret_cast<V*>(to), o);
+      } else {
+        V e;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float c = cs[now.pair + j], s = sn[now.pair + j], u = (float)x.v[j], w = (float)y.v[j];
-        o.v[j] = (T)(u * c - w * s);
-        e.v[j] = (T)(u * s + w * c);
+        for (int j = 0; j < N; ++j) {
+          const float c = cs[at + j], s = sn[at + j], v = (float)x[u].v[j], w = (float)y[u].v[j];
+          o.v[j] = (T)(v * c - w * s);
+          e.v[j] = (T)(v * s + w * c);
+        }
+        put(reinterpret_cast<V*>(to), o);
+        put(reinterpret_cast<V*>(to + half), e);
       }
-      *reinterpret_cast<V*>(now.to) = o;
-      *reinterpret_cast<V*>(now.to + half) = e;
     }
-    i += step;
-    if (i < all) load();
+    i += kRopeAhead * step;
+    load(i);
   }
 }
 
@@ -137,10 +167,16 @@ template <class T, int N, bool PAIRS>
 hipError_t rope(const c4s_rope_desc& a, hipStream_t s) {
   const int per = (PAIRS ? a.rot_dim : a.rot_dim / 2) / N + (a.head_dim - a.rot_dim) / N;
   const int64_t all = (int64_t)((a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0)) * per;
-  const int threads = (int)std::min<int64_t>((all + 63) / 64 * 64, 256);
-  // rows alone fill the chip, or every thread has one piece
-  const int parts = a.n_rows >= 1024 ? 1 : (int)std::min<int64_t>((all + threads - 1) / threads, std::max(2048 / a.n_rows, 1));
-  hipLaunchKernelGGL((k_rope<T, N, PAIRS>), dim3((unsigned)(a.n_rows * parts)), dim3(threads), 0, s, RopeArgs{a, parts});
+  // few rows: every thread has one piece; rows that fill the chip: kRopeAhead, in as many even rounds as that takes
+  int parts = 1;
+  int64_t threads = std::min<int64_t>(all, kRopeThreads);
+  if (a.n_rows < 1024) {
+    parts = (int)std::min<int64_t>((all + kRopeThreads - 1) / kRopeThreads, std::max(2048 / a.n_rows, 1));
+  } else {
+    const int64_t rounds = (all + kRopeAhead * kRopeThreads - 1) / (kRopeAhead * kRopeThreads);
+    threads = (all + rounds * kRopeAhead - 1) / (rounds * kRopeAhead);
+  }
+  hipLaunchKernelGGL((k_rope<T, N, PAIRS>), dim3((unsigned)(a.n_rows * parts)), dim3((unsigned)((threads + 63) / 64 * 64)), 0, s, RopeArgs{a, parts});
   return hipGetLastError();
 }
 
