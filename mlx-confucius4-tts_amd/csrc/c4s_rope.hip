@@ -4,12 +4,13 @@
 // position into cosines and sines, once for all heads, and leave them in LDS
 // while every thread's first pieces of queries or keys are on their way. A piece is
 // eight bf16 or four floats (of either half of the pairs, with C4S_ROPE_HALF), or
-// single pairs where sizes or alignment do not allow that. Memory bounds it: loads and
-// stores go past the L2, where nothing would be found again (the next call's
-// workgroups are on other dies). 18829 rows in place, halves, on memory that is in no
-// cache: 32 and 8 heads of 128 67 us, 5.8 TB/s; 20 and 20 of 64, whose halves are half a line each, 44 us, 4.4 TB/s
-// (through the L2 59; one piece of a thread at a time 47; lines whole and the halves
-// exchanged between lanes 48; workgroups of two or four rows 44). 64 rows: 2.9 us.
+// single pairs where sizes or alignment do not allow that. Memory bounds it: stores go
+// past the L2, where nothing would be found again (the next call's workgroups are on
+// other dies). 18829 rows in place, halves, from the last-level cache, where the product
+// before leaves them / from memory: 20 and 20 heads of 64 34 us, 5.6 TB/s / 45 (a half is
+// half a line there); 32 and 8 of 128 59, 6.5 TB/s / 77. (Stores through the L2: 46 / 59 for heads of 64.
+// Loads past the caches as well: 43 / 44, and 66 / 67 for heads of 128. One piece of a thread at a time 47 from memory;
+// lines whole and the halves exchanged between lanes 48; workgroups of two or four rows 44.) 64 rows: 2.9 us.
 //
 // The angle is reduced in 64 bits: position * frequency / 2 pi, less its whole
 // turns, has an absolute error of 2^-52 of the number of turns; the rest, at most
@@ -60,11 +61,6 @@ constexpr int kRopeThreads = 256, kRopeAhead = 2;   // pieces of a thread that a
 
 typedef uint32_t Words __attribute__((ext_vector_type(4)));
 template <class V>
-__device__ __forceinline__ V get(const V* from) {
-  if constexpr (sizeof(V) == 16) return __builtin_bit_cast(V, __builtin_nontemporal_load(reinterpret_cast<const Words*>(from)));
-  else return *from;
-}
-template <class V>
 __device__ __forceinline__ void put(V* to, const V& v) {
   if constexpr (sizeof(V) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words, v), reinterpret_cast<Words*>(to));
   else *to = v;
@@ -111,8 +107,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
       const int i = i0 + u * step;
       if (i >= all) continue;
       now[u] = piece(i);
-      x[u] = get(reinterpret_cast<const V*>(now[u].from));
-      if (!PAIRS && now[u].at >= 0) y[u] = get(reinterpret_cast<const V*>(now[u].from + half));
+      x[u] = *reinterpret_cast<const V*>(now[u].from);
+      if (!PAIRS && now[u].at >= 0) y[u] = *reinterpret_cast<const V*>(now[u].from + half);
     }
   };
   int i = part * blockDim.x + threadIdx.x;
