@@ -96,8 +96,9 @@ typedef struct c4s_pages {
   int32_t page_size;         /* 16, 32, 64, 128 or 256 */
 } c4s_pages;
 
-/* lens[b] += n_new[b] (below 0: 0), with the pages for it: the free ones with the
- * lowest numbers, to the sequences in order. What is not to be had, or lies behind
+/* lens[b] += n_new[b] (below 0: 0; all of them together, and every length, stay below
+ * 2^31), with the pages for it: the free ones with the lowest numbers, to the sequences
+ * in order. What is not to be had, or lies behind
  * max_pages, is counted in missing; its entries stay -1, and the cache drops what is
  * written there.
  * rows_off, row_pos and row_slot describe the new tokens as packed rows: the offsets

@@ -61,10 +61,33 @@ struct GrowArgs {
   c4s_pages p;
   c4s_grow g;
   int shift;
+  bool maps;   // the new rows' maps are the one workgroup's work too
 };
+
+// Position and slot of row r, the sequences' first rows at off.
+__device__ __forceinline__ void map_row(const GrowArgs& f, const int32_t* off, int r) {
+  const c4s_pages& p = f.p;
+  int lo = 0, hi = p.n_seqs;
+  while (hi - lo > 1) {   // eight parts a step
+    const int step = (hi - lo + 7) / 8;
+    int behind = 0;
+#pragma unroll
+    for (int j = 1; j < 8; ++j) behind += (lo + j * step < hi) & (off[min(lo + j * step, hi - 1)] <= r);
+    lo += behind * step;
+    hi = min(lo + step, hi);
+  }
+  const int pos = p.lens[lo] - (off[lo + 1] - r), at = pos >> f.shift;
+  if (f.g.row_pos) f.g.row_pos[r] = pos;
+  if (!f.g.row_slot) return;
+  const int page = pos >= 0 && at < p.max_pages ? p.block_table[lo * p.table_ld + at] : -1;
+  f.g.row_slot[r] = page < 0 || page >= p.n_pages ? -1 : (page << f.shift) + (pos & ((1 << f.shift) - 1));
+}
 
 constexpr int kHash = 2 * kPagesSeqs;   // places of the table of shared pages
 constexpr int kBatch = 16384;           // pages in LDS at a time
+// Rows whose maps that workgroup writes; more have a kernel of their own. 64 sequences, new tokens each, with a trim,
+// us: 16 11.3 (own kernel 12.2), 32 12.9 (13.4), 64 16.7 (14.9), 256 32 (18.6).
+constexpr int kMapRows = 2048;
 
 __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
   __shared__ union {
@@ -201,9 +224,9 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
     for (int rank = begin; rank < end; rank += step) row[rank] = there ? lds.give.page[rank - first] : -1;
   };
   // Few: a page a thread, which searches its sequence; many: sixteen threads a sequence, which write its entries next to
-  // each other.
+  // each other. (4000 sequences, one page each, with a trim: 35 us, by sixteen 51; 1000 of three 27 and 29, of 13 39 and 31.)
   auto give = [&](int first, int count, bool there) {
-    if (count <= 2 * kGrowThreads) {
+    if (count <= 2 * kGrowThreads || count <= 4 * n) {
       for (int i = tid; i < count; i += kGrowThreads) {
         int lo = 0, hi = n;   // the last sequence that begins at or before it (those that ask for none begin with the next)
         while (hi - lo > 1) {
@@ -280,28 +303,18 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
       if (g.row_slot) g.row_slot[b] = is_page(here[b]) ? (here[b] << shift) + (len & (ps - 1)) : -1;
     }
   }
+  if (!f.maps) return;
+  int32_t* off = lds.give.page;   // (no page is handed out any more)
+  static_assert(kPagesSeqs < kBatch, "the rows' offsets in LDS");
+  for (int b = tid; b <= n; b += kGrowThreads) off[b] = g.rows_off[b];
+  __syncthreads();
+  for (int row = tid; row < min(g.n_rows, off[n]); row += kGrowThreads) map_row(f, off, row);
 }
 
 // Rows of several new tokens a sequence: positions and slots.
 __global__ __launch_bounds__(256) void k_row_maps(GrowArgs f) {
-  const c4s_pages& p = f.p;
-  const c4s_grow& g = f.g;
   const int r = blockIdx.x * 256 + threadIdx.x;
-  if (r >= g.n_rows || r >= g.rows_off[p.n_seqs]) return;
-  int lo = 0, hi = p.n_seqs;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 7) / 8;
-    int behind = 0;
-#pragma unroll
-    for (int j = 1; j < 8; ++j) behind += (lo + j * step < hi) & (g.rows_off[min(lo + j * step, hi - 1)] <= r);
-    lo += behind * step;
-    hi = min(lo + step, hi);
-  }
-  const int pos = p.lens[lo] - (g.rows_off[lo + 1] - r), at = pos >> f.shift;
-  if (g.row_pos) g.row_pos[r] = pos;
-  if (!g.row_slot) return;
-  const int page = at < p.max_pages ? p.block_table[lo * p.table_ld + at] : -1;
-  g.row_slot[r] = page < 0 || page >= p.n_pages ? -1 : (page << f.shift) + (pos & ((1 << f.shift) - 1));
+  if (r < f.g.n_rows && r < f.g.rows_off[f.p.n_seqs]) map_row(f, f.g.rows_off, r);
 }
 
 // A wave a sequence.
@@ -397,10 +410,11 @@ int shift_of(int page_size) {
 }  // namespace
 
 hipError_t launch_pages_grow(const c4s_pages& p, const c4s_grow& g, hipStream_t s) {
-  const GrowArgs f{p, g, shift_of(p.page_size)};
+  const bool maps = g.n_new && g.n_rows && (g.row_pos || g.row_slot);
+  const GrowArgs f{p, g, shift_of(p.page_size), maps && g.n_rows <= kMapRows};
   hipLaunchKernelGGL(k_pages_grow, dim3(1), dim3(kGrowThreads), 0, s, f);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !g.n_new || g.n_rows == 0 || (!g.row_pos && !g.row_slot)) return e;
+  if (e != hipSuccess || !maps || f.maps) return e;
   hipLaunchKernelGGL(k_row_maps, dim3((g.n_rows + 255) / 256), dim3(256), 0, s, f);
   return hipGetLastError();
 }

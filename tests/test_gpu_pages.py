@@ -84,6 +84,28 @@ def test_sizes(gpu_ctx, n, pages_n):
     _grow(gpu_ctx, pool, pages, [r.randint(0, 90) for _ in range(n)], True, room=3)
 
 
+def test_rows_of_many_tokens(gpu_ctx):
+    """Maps that the one workgroup writes, and maps of their own kernel, at the border between them."""
+    for n, new, room in ((3, 2000, None), (64, 32, None), (64, 33, None), (4096, 1, 4096), (200, 10, 2049), (1, 9000, 70)):
+        print(f"maps n={n} new={new} room={room}", flush=True)
+        pool = B.Pool(n, 700, 12000, 16)
+        pages = pool.device()
+        for step in range(2):
+            _grow(gpu_ctx, pool, pages, [new + (b + step) % 2 for b in range(n)], step == 1, room=room)
+
+
+def test_more_tokens_than_numbers(gpu_ctx):
+    """What no table holds is counted nowhere sensible, and written nowhere."""
+    for room in (50, 5000):
+        pages = c4s.Pages.empty(3, 4, 40, 16)
+        off, pos, slot = i32([0] * 4), i32([-9] * room), i32([-9] * room)
+        gpu_ctx.pages_grow(pages, i32([2 ** 31 - 1, 7, 2 ** 31 - 1]), off, pos, slot)
+        gpu_ctx.pages_grow(pages, i32([2 ** 31 - 1, 7, 2 ** 31 - 1]), off, pos, slot)
+        assert pages.lens.tolist() == [2 ** 31 - 1, 14, 2 ** 31 - 1]
+        assert pages.block_table.tolist() == [[0, 1, 2, 3], [4, -1, -1, -1], [5, 6, 7, 8]]
+        assert pages.refs.tolist() == [1] * 9 + [0] * 31
+
+
 def test_beams_that_part(gpu_ctx):
     """Who copies a shared last page: all but the last of its holders, all of them where one does not go on, nobody
     where it is full."""
