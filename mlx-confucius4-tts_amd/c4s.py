@@ -775,24 +775,29 @@ class Context:
         or in place. pairs: dims 2 i and 2 i + 1 go together, else i and i + len(freq). Positions: pos (int32 [rows]), or
         the last ones of lens[b] with rows_off as kv_append has them."""
         x = k if q is None else q
-        _need(x is not None and (lens is not None or pos is not None), "rope: needs q or k, and lens or pos")
+        if x is None or (lens is None and pos is None):
+            raise ValueError("rope: needs q or k, and lens or pos")
         shape, dev = x.shape, self.device
-        rows, _, dim = shape
+        rows, heads, dim = shape
         freq_n = freq.numel()
         fp = _words(freq, freq_n, _Torch.f64, "rope: freq must be a float64 vector", dev)
-        t = ldq = ldqo = ldk = ldko = qp = qop = kp = kop = heads = kv_heads = 0
-        if q is not None:
-            heads = shape[1]
+        ldq = ldqo = ldk = ldko = qp = qop = kp = kop = kv_heads = 0
+        if q is None:
+            heads = 0
+        else:
             qp, ldq, t = _heads(q, shape, "rope: q must be bfloat16 or float32 [rows][heads][head_dim], a row contiguous", dev, True)
             qop, ldqo, to = (qp, ldq, t) if q_out is None else _heads(q_out, shape, "rope: q_out must have q's shape and dtype, a row contiguous", dev)
-            _need(t == to, "rope: q_out must have q's dtype")
+            if t != to:
+                raise ValueError("rope: q_out must have q's dtype")
         if k is not None:
             ks = k.shape
-            _need(ks[0] == rows and ks[2] == dim, "rope: k must have q's rows and head_dim")
-            kv_heads = ks[1]
+            k_rows, kv_heads, k_dim = ks
             kp, ldk, tk = _heads(k, ks, "rope: k must be bfloat16 or float32 [rows][heads][head_dim], a row contiguous", dev, True)
             kop, ldko, to = (kp, ldk, tk) if k_out is None else _heads(k_out, ks, "rope: k_out must have k's shape and dtype, a row contiguous", dev)
-            _need(tk == to and (q is None or tk == t), "rope: q, k and their outputs must have one dtype")
+            if k_rows != rows or k_dim != dim:
+                raise ValueError("rope: k must have q's rows and head_dim")
+            if tk != to or (q is not None and tk != t):
+                raise ValueError("rope: q, k and their outputs must have one dtype")
             t = tk
         n = 0 if lens is None else lens.numel()
         rc = _lib.c4s_rope(
