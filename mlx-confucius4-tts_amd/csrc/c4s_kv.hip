@@ -12,11 +12,13 @@
 //
 // Memory bounds both for prompts, and both move more than they need. 24 prompts of
 // 70 to 1500 tokens, 20 heads of 64, 8-bit, calls back to back: the read needs 179 MB
-// (62 of codes and scales, 117 of rows) and takes 41 us, 4.4 TB/s, in which 93 and
-// 159 MB pass, 6.1 TB/s; the write needs 148 MB (96 of rows, 51 of codes and scales)
-// and takes 51 us, 2.9 TB/s, in which 97 and 65 MB pass. What the write adds are the
+// (62 of codes and scales, 117 of rows) and takes 37 us, 4.8 TB/s, in which 93 and
+// 117 MB pass; the write needs 148 MB (96 of rows, 51 of codes and scales) and takes
+// 51 us, 2.9 TB/s, in which 97 and 65 MB pass. What the write adds are the
 // lines of pages that a tile's ends leave half full; the VALU, which computes the
 // codes, is busy half of the time, and which of the two costs more is not known.
+// In 4 bits (18829 rows like those, from memory / from the last-level cache) the write's 121 MB
+// take 39 / 30 us, the read's as many 25 / 25, 4.9 TB/s; 64 rows 4.1 and 4.6.
 
 #include <hip/hip_runtime.h>
 
@@ -318,86 +320,95 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_append(KvArgs c, KvRowsArgs 
   });
 }
 
+// Four lanes a row; in large tiles eight, with two rows each, so that a store is a whole line (with four, past the caches,
+// 158 MB are written where 117 are needed: the prompts above 50 us for 42 from memory, in 4 bits 30 for 26).
 template <int STORE, int PIECES, int TILE>
 __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs rows) {
   constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
+  constexpr int kLanes = TILE == 64 ? 8 : 4, kRows = kLanes / 4, kPieces = PIECES / kRows;
   __shared__ Tile<TILE> tile;
   __shared__ Values<STORE, PIECES, TILE> values;
   tile.find(c, rows);
-  const int row = threadIdx.x / 4, l = threadIdx.x % 4, dim = c.dim, ps = 1 << c.page_shift;
+  const int l = threadIdx.x % kLanes, dim = c.dim, ps = 1 << c.page_shift;
   const int head = blockIdx.x % c.n_heads;
-  const int64_t r = (int64_t)(blockIdx.x / c.n_heads) * TILE + row;
-  const Place p = tile.at[row];
-  const int64_t slot = (p.page * c.n_heads + head) * (int64_t)ps + p.at;
-  float scale[2] = {1.0f, 1.0f};
-  if (Q8 && p.page >= 0) {
-    scale[0] = c.k_scale[slot];
-    scale[1] = c.v_scale[slot];
-  }
-  uint32_t e[2][Q4 ? PIECES : 1];
-  if (Q4 && p.page >= 0) {
-    const int64_t first = (p.page * c.n_heads + head) * (int64_t)(dim / 32) * ps + p.at;
+  const auto row_of = [&](int h) { return (int)threadIdx.x / kLanes + TILE / kRows * h; };
+  float scale[2][kRows];
+  uint32_t e[2][kRows][Q4 ? kPieces : 1];
+  Piece raw[2][kRows][kPieces];   // without a page: zeros
+  bool mine[kRows], has[kRows];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      if (32 * i >= dim) break;
-      e[0][i] = reinterpret_cast<const uint8_t*>(c.k_scale)[first + ((uint32_t)i << c.page_shift)];
-      e[1][i] = reinterpret_cast<const uint8_t*>(c.v_scale)[first + ((uint32_t)i << c.page_shift)];
+  for (int h = 0; h < kRows; ++h) {
+    const Place p = tile.at[row_of(h)];
+    const int64_t slot = (p.page * c.n_heads + head) * (int64_t)ps + p.at;
+    // a row between two sequences' rows, or behind the last, is not the call's to write
+    const int64_t r = (int64_t)(blockIdx.x / c.n_heads) * TILE + row_of(h);
+    mine[h] = r < rows.n_rows && (!rows.off || (r >= rows.off[0] && r < rows.off[c.n_seqs]));
+    has[h] = p.page >= 0;
+    scale[0][h] = scale[1][h] = 1.0f;
+    if (Q8 && p.page >= 0) {
+      scale[0][h] = c.k_scale[slot];
+      scale[1][h] = c.v_scale[slot];
     }
-  }
-  Piece raw[2][PIECES];   // without a page: zeros
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
-    const int d = 32 * i + 8 * l;
-    raw[0][i] = raw[1][i] = Piece{};
-    if (p.page < 0 || d >= dim) continue;
-    if (Q4) {
-      raw[0][i][0] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.k) + (slot * dim + d) / 2);
-    } else if (Q8) {
-      const Codes w = *reinterpret_cast<const Codes*>(static_cast<const uint8_t*>(c.k) + slot * dim + d);
-      raw[0][i] = Piece{w[0], w[1], 0, 0};
-    } else {
-      raw[0][i] = *reinterpret_cast<const Piece*>(static_cast<const uint16_t*>(c.k) + slot * dim + d);
+    for (int i = 0; i < kPieces; ++i) {
+      const int d = 8 * (kLanes * i + l);
+      raw[0][h][i] = raw[1][h][i] = Piece{};
+      if (p.page < 0 || d >= dim) continue;
+      if (Q4) {
+        const int64_t at = (p.page * c.n_heads + head) * (int64_t)(dim / 32) * ps + p.at + ((uint32_t)(d / 32) << c.page_shift);
+        e[0][h][i] = reinterpret_cast<const uint8_t*>(c.k_scale)[at];
+        e[1][h][i] = reinterpret_cast<const uint8_t*>(c.v_scale)[at];
+        raw[0][h][i][0] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.k) + (slot * dim + d) / 2);
+      } else if (Q8) {
+        const Codes w = *reinterpret_cast<const Codes*>(static_cast<const uint8_t*>(c.k) + slot * dim + d);
+        raw[0][h][i] = Piece{w[0], w[1], 0, 0};
+      } else {
+        raw[0][h][i] = *reinterpret_cast<const Piece*>(static_cast<const uint16_t*>(c.k) + slot * dim + d);
+      }
     }
   }
   const int wide = Q4 ? dim / 2 : dim;   // of a page's rows of positions
   values.template move<false>(tile, wide, c.page_shift, [&](const Place& q) {
     return static_cast<uint8_t*>(c.v) + ((q.page * c.n_heads + head) * (int64_t)ps * wide + q.at) * (STORE == C4S_KV_BF16 ? 2 : 1);
   });
-  // a row between two sequences' rows, or behind the last, is not the call's to write
-  const bool mine = r < rows.n_rows && (!rows.off || (r >= rows.off[0] && r < rows.off[c.n_seqs]));
   __syncthreads();
-  if (!mine) return;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    void* out = which ? rows.v : rows.k;
-    const int64_t o = r * (which ? rows.ldv : rows.ldk) + head * dim;
+  for (int h = 0; h < kRows; ++h) {
+    const int row = row_of(h);
+    const int64_t r = (int64_t)(blockIdx.x / c.n_heads) * TILE + row;
+    if (!mine[h]) continue;
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int d = 32 * i + 8 * l;
-      if (d >= dim) continue;
-      Piece w = raw[which][i];
-      if (which && p.page >= 0) {
+    for (int which = 0; which < 2; ++which) {
+      void* out = which ? rows.v : rows.k;
+      const int64_t o = r * (which ? rows.ldv : rows.ldk) + head * dim;
 #pragma unroll
-        for (int j = 0; j < (Q4 ? 1 : (Q8 ? 2 : 4)); ++j) w[j] = values.piece(row, d)[j];
-      }
-      if (Q4 && p.page >= 0) w = values4(w[0], scale4(e[which][i]));
-      float v[8];
+      for (int i = 0; i < kPieces; ++i) {
+        const int d = 8 * (kLanes * i + l);
+        if (d >= dim) continue;
+        Piece w = raw[which][h][i];
+        if (which && has[h]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = Q8 ? (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale[which]
-                  : __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-      // past the caches, which keeps the pages in them (41 us for 52)
-      if (rows.f32) {
-        typedef float Quad __attribute__((ext_vector_type(4)));
-        Quad* q = reinterpret_cast<Quad*>(static_cast<float*>(out) + o + d);
-        __builtin_nontemporal_store(Quad{v[0], v[1], v[2], v[3]}, q);
-        __builtin_nontemporal_store(Quad{v[4], v[5], v[6], v[7]}, q + 1);
-      } else {
-        if (Q8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, Pair{(__bf16)v[2 * j], (__bf16)v[2 * j + 1]});
+          for (int j = 0; j < (Q4 ? 1 : (Q8 ? 2 : 4)); ++j) w[j] = values.piece(row, d)[j];
         }
-        __builtin_nontemporal_store(w, reinterpret_cast<Piece*>(static_cast<uint16_t*>(out) + o + d));
+        if (Q4 && has[h]) w = values4(w[0], scale4(e[which][h][i]));
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[j] = Q8 ? (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale[which][h]
+                    : __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+        // past the caches, which keeps the pages in them (41 us for 52)
+        if (rows.f32) {
+          typedef float Quad __attribute__((ext_vector_type(4)));
+          Quad* q = reinterpret_cast<Quad*>(static_cast<float*>(out) + o + d);
+          __builtin_nontemporal_store(Quad{v[0], v[1], v[2], v[3]}, q);
+          __builtin_nontemporal_store(Quad{v[4], v[5], v[6], v[7]}, q + 1);
+        } else {
+          if (Q8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, Pair{(__bf16)v[2 * j], (__bf16)v[2 * j + 1]});
+          }
+          __builtin_nontemporal_store(w, reinterpret_cast<Piece*>(static_cast<uint16_t*>(out) + o + d));
+        }
       }
     }
   }
