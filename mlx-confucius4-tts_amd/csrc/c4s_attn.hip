@@ -183,6 +183,7 @@ struct FewArgs {
   int chunk, splits, tiles;   // positions a chunk (a multiple of 256); chunks at most; row tiles
   uint32_t* arrived;          // [n_seqs][tiles][key heads]
   float* part;                // [n_seqs][tiles][key heads][splits][kRows][dim + 4]
+  bool neighbours;
 };
 
 // DH: the head's dims rounded up to 64, 128 or 256; FULL: they are that many.
@@ -208,8 +209,15 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = lane % 16, g = lane / 16;
   const int dim = FULL ? DH : a.c.dim;
   // blockIdx.x: (tile, chunk, key head), the heads of one chunk next to each other
-  const int head = blockIdx.x % a.c.n_heads, split = blockIdx.x / a.c.n_heads % f.splits, tile = blockIdx.x / a.c.n_heads / f.splits;
-  const int seq = blockIdx.y;
+  uint32_t block = blockIdx.x;
+  int seq = blockIdx.y;
+  if (Q4 && f.neighbours) {   // four blocks next to each other on one die: they share lines of scales
+    uint32_t at = blockIdx.y * gridDim.x + blockIdx.x;
+    if (at < (gridDim.x * gridDim.y & ~31u)) at = (at & ~31u) + at % 8 * 4 + at % 32 / 8;
+    seq = at / gridDim.x;
+    block = at - seq * gridDim.x;
+  }
+  const int head = block % a.c.n_heads, split = block / a.c.n_heads % f.splits, tile = block / a.c.n_heads / f.splits;
   const int shift = a.c.page_shift, ps = 1 << shift;
   // The chunk's part of the table (-1: no page), asked for while the lengths are on their way.
   __shared__ int32_t pages[kMaxPages + 16];
@@ -842,6 +850,9 @@ FewArgs few_args(const AttnArgs& a) {
   chunk = std::max(chunk, (cap + kMaxParts - 1) / kMaxParts + 255) / 256 * 256;
   f.chunk = (int)std::min<int64_t>(std::max<int64_t>(chunk, 256), (int64_t)kMaxPages << a.c.page_shift);
   f.splits = (int)std::max<int64_t>((cap + f.chunk - 1) / f.chunk, 1);
+  // heads whose scales of a page share a line of 128 bytes (64 rows of 50 to 1500, 20 heads of 64, pages of 16, from
+  // memory: 69 MB read for 81, 17.0 us for 17.9)
+  f.neighbours = ((a.c.dim / 32) << a.c.page_shift) < 128 && groups * f.splits < INT32_MAX;
   return f;
 }
 
