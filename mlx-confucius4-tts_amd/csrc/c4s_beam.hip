@@ -507,14 +507,14 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_states(BeamArgs f) {
   }
 }
 
-// How a row is cut: into slices for 3072 waves together, twelve a CU, of 1 to kMostChunks chunks. In us, for 2048 / 3072 /
-// 4096 / 6144 waves: 24 groups of 8 rows of 151936 bf16 27.2 / 26.2 / 27.4 / 35.4, fp32 30.8 / 31.0 / 32.5 / 39.9; 192 rows
+// How a row is cut: into slices for twelve waves a CU together, of 1 to kMostChunks chunks. In us, for 8 / 12 / 16 / 24
+// waves a CU: 24 groups of 8 rows of 151936 bf16 27.2 / 26.2 / 27.4 / 35.4, fp32 30.8 / 31.0 / 32.5 / 39.9; 192 rows
 // 24.3 / 20.7 / 21.1 / 26.8; 256 groups of 4 of 32000 25.1 / 23.4 / 23.2 / 30.3.
 BeamArgs beam_args(const c4s_beam& a) {
   BeamArgs f{};
   f.a = a;
   const int64_t rows = (int64_t)a.n_groups * a.width, chunks = (a.vocab + kChunk - 1) / kChunk;
-  const int64_t slices = std::max(std::min(std::max<int64_t>(3072 / rows, 1), chunks), (chunks + kMostChunks - 1) / kMostChunks);
+  const int64_t slices = std::max(std::min(std::max<int64_t>(12 * 256 / rows, 1), chunks), (chunks + kMostChunks - 1) / kMostChunks);
   f.chunks = (int)((chunks + slices - 1) / slices);
   f.slices = (int)((chunks + f.chunks - 1) / f.chunks);
   f.wgs = (a.width * f.slices + kBeamWaves - 1) / kBeamWaves;
