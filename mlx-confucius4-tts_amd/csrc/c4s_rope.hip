@@ -66,6 +66,12 @@ __device__ __forceinline__ void put(V* to, const V& v) {
   else *to = v;
 }
 
+// Values of a piece that is not turned: single ones beside single pairs, as their number may be odd.
+template <int N, bool PAIRS>
+__host__ __device__ constexpr int copied() {
+  return PAIRS && N == 2 ? 1 : N;
+}
+
 struct RopeArgs {
   c4s_rope_desc d;
   int parts;   // workgroups of a row
@@ -79,7 +85,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
   const int row = blockIdx.x / f.parts, part = blockIdx.x % f.parts;
   const int half = a.rot_dim / 2;
   const int turned = (PAIRS ? a.rot_dim : half) / N;  // pieces of a head that are turned; the others
-  const int per = turned + (a.head_dim - a.rot_dim) / N;        // (copied) follow them
+  constexpr int kCopy = copied<N, PAIRS>();
+  const int per = turned + (a.head_dim - a.rot_dim) / kCopy;    // (copied) follow them
   const int heads = (a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0), all = heads * per;
   const int step = blockDim.x * f.parts;
 
@@ -95,7 +102,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
     const int64_t r = row;
     const T* from = static_cast<const T*>(is_q ? a.q : a.k) + r * (is_q ? a.ldq : a.ldk) + (int64_t)h * a.head_dim;
     T* to = static_cast<T*>(is_q ? a.q_out : a.k_out) + r * (is_q ? a.ldq_out : a.ldk_out) + (int64_t)h * a.head_dim;
-    const int at = p < turned ? p * N : a.rot_dim + (p - turned) * N;
+    const int at = p < turned ? p * N : a.rot_dim + (p - turned) * kCopy;
     return Piece{from + at, to + at, p < turned ? at : -1};
   };
   using V = Few<T, N>;
@@ -107,7 +114,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
       const int i = i0 + u * step;
       if (i >= all) continue;
       now[u] = piece(i);
-      x[u] = *reinterpret_cast<const V*>(now[u].from);
+      if (kCopy == N || now[u].at >= 0) x[u] = *reinterpret_cast<const V*>(now[u].from);
+      else x[u].v[0] = *now[u].from;
       if (!PAIRS && now[u].at >= 0) y[u] = *reinterpret_cast<const V*>(now[u].from + half);
     }
   };
@@ -133,7 +141,9 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
       T* const to = now[u].to;
       V o;
       if (at < 0) {
-        if (to != now[u].from) put(reinterpret_cast<V*>(to), x[u]);
+        if (to == now[u].from) continue;
+        if (kCopy == N) put(reinterpret_cast<V*>(to), x[u]);
+        else *to = x[u].v[0];
       } else if constexpr (PAIRS) {
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
@@ -161,7 +171,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
 
 template <class T, int N, bool PAIRS>
 hipError_t rope(const c4s_rope_desc& a, hipStream_t s) {
-  const int per = (PAIRS ? a.rot_dim : a.rot_dim / 2) / N + (a.head_dim - a.rot_dim) / N;
+  const int per = (PAIRS ? a.rot_dim : a.rot_dim / 2) / N + (a.head_dim - a.rot_dim) / copied<N, PAIRS>();
   const int64_t all = (int64_t)((a.q ? a.n_heads : 0) + (a.k ? a.n_kv_heads : 0)) * per;
   // few rows: every thread has one piece; rows that fill the chip: kRopeAhead, in as many even rounds as that takes
   int parts = 1;

@@ -34,6 +34,9 @@ CASES = [  # new, past, heads, kv_heads, dim, rot, dtype
     ([1500], [5], 2, 1, 64, 64, "bf16"),               # a row a workgroup
     ([20], [2 ** 31 - 30], 2, 1, 64, 64, "f32"),
     ([3], [1], 1, 1, 1024, 1024, "bf16"),
+    ([3], [5], 2, 1, 7, 4, "bf16"),                    # heads of odd sizes
+    ([4], [9], 3, 2, 33, 10, "f32"),
+    ([1100], [0], 1, 1, 3, 2, "f32"),
 ]
 
 
