@@ -119,6 +119,8 @@ __global__ __launch_bounds__(kGrowThreads) void k_pages_grow(GrowArgs f) {
       if (word + 1 < words) bits.y = p.free_bits[word + 1];
       if (word + 2 < words) bits.z = p.free_bits[word + 2];
     }
+    const int last = words - 1 - word;   // bits behind the last page count for nothing
+    if (last >= 0 && last < 4 && p.n_pages % 32) (last == 0 ? bits.x : last == 1 ? bits.y : last == 2 ? bits.z : bits.w) &= (1u << p.n_pages % 32) - 1;
   };
   load_bits(4 * tid);
 

@@ -118,6 +118,10 @@ ATTN = [  # new, past, heads, kv_heads, dim, page
     ([5, 1], [33, 260], 3, 3, 160, 128),
     ([1, 8], [90, 1000], 16, 2, 64, 256),
     ([2, 1], [300, 20], 7, 1, 224, 64),
+    ([2, 1, 0, 2], [70, 300, 5, 0], 3, 3, 64, 16),
+    ([4, 3, 1], [100, 9, 0], 5, 5, 128, 32),
+    ([1, 1], [65, 2], 9, 3, 160, 16),
+    ([3], [1000], 2, 2, 256, 128),
 ]
 
 
@@ -128,6 +132,35 @@ def test_attn_few_rows(gpu_ctx, new, past, heads, kv_heads, dim, page):
     cache = B.Cache4([n + p for n, p in zip(new, past)], kv_heads, dim, page, seed=dim + page, junk=True)
     q, out, lse = _run_attn(gpu_ctx, cache, new, heads, spread=0.7)
     _check_attn(cache, q, out, lse, new, heads)
+
+
+@pytest.mark.parametrize("new,heads", [([1, 1], 3), ([2, 1], 3), ([1, 1], 12), ([5, 1], 6)])
+def test_attn_scales(gpu_ctx, new, heads):
+    """No scale, negative ones, and scores that differ by hundreds, so that every block has a new greatest one; values
+    of very different sizes beside each other."""
+    for scale, spread, rising in ((0.0, 0.7, False), (-0.25, 0.7, False), (0.125, 5.0, False), (0.125, 1.0, True), (-0.125, 1.0, True)):
+        print(f"attn4 scales {new} {heads} {scale} {spread} {rising}", flush=True)
+        cache = B.Cache4([900, 333], 3, 64, 16, seed=21, junk=True)
+        if rising:     # the first block of a key grows with its position, and so does the score of a q with ones there
+            for b, n in enumerate(cache.lens):
+                for p in range(n):
+                    code, e = B.quantise4(torch.full((3, 32), float(p + 1)).to(BF))
+                    pg, at = int(cache.table[b, p // 16]), p % 16
+                    cache.t["k"][pg, :, at, :16] = code[:, 0::2] | code[:, 1::2] << 4
+                    cache.t["k_scale"][pg, :, 0, at] = e[:, 0]
+        for pg in range(cache.n_pages):
+            cache.t["v_scale"][pg, :, 1] = torch.where(cache.t["v_scale"][pg, :, 1] < 253, 40 + 20 * (pg % 11), cache.t["v_scale"][pg, :, 1]).to(torch.uint8)
+        g = torch.Generator().manual_seed(22)
+        q = (torch.randn((sum(new), heads, 64), generator=g) * spread).to(BF)
+        if rising:
+            q[..., :32] = 1.0
+        out = torch.empty((sum(new), heads, 64), dtype=BF, device="cuda")
+        off = _packed(new, True)
+        gpu_ctx.attn(q.cuda(), cache.cuda(), torch.tensor(cache.lens, dtype=I32).cuda(), out, rows_off=None if off is None else off.cuda(),
+                     max_new=max(new), scale=scale)
+        want, _, mag, _ = L.attn(cache, q, new, heads, scale)
+        # scores of up to 500 in float32: 64 products' sum, 8 roundings of 2^-24 at most in a tree, the scale's: 3e-4 of a weight
+        _close(out, want, (6e-4 if rising else 1e-4 if spread < 1 else 3e-4) * mag)
 
 
 PROMPTS = [  # new, past, heads, kv_heads, dim, page

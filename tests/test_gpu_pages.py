@@ -106,6 +106,16 @@ def test_more_tokens_than_numbers(gpu_ctx):
         assert pages.refs.tolist() == [1] * 9 + [0] * 31
 
 
+def test_bits_behind_the_last_page(gpu_ctx):
+    """They name no pages."""
+    for n_pages in (3, 33, 70, 120, 127):
+        pages = c4s.Pages.empty(2, 200, n_pages, 16)
+        pages.free_bits.fill_(-1)
+        gpu_ctx.pages_grow(pages, i32([16 * 50, 16 * 100]))
+        assert sorted(p for p in pages.block_table.flatten().tolist() if p >= 0) == list(range(min(n_pages, 150)))
+        assert pages.refs.tolist() == [1] * n_pages and int(pages.missing) == 150 - n_pages
+
+
 def test_beams_that_part(gpu_ctx):
     """Who copies a shared last page: all but the last of its holders, all of them where one does not go on, nobody
     where it is full."""
