@@ -196,7 +196,7 @@ struct FewArgs {
 // scales join the weights, a product a row and block of 32 dims (a scale of 2^-127 counts as 0 there); the weights then
 // go through LDS, as pairs of bf16 for each such block, into the second product's operand. The codes themselves need no
 // scale there: two positions' bytes give a dim's pair by an exchange of nibbles and one conversion. 64 rows of 50 to 1500
-// positions, 20 heads of 64: 18.0 us (as with more rows 22.4; its 36 MB in 6.4); 64 of 4000, 5 heads of 256: 95 (119).
+// positions, 20 heads of 64: 17.5 us (as with more rows 22.4); 64 of 4000, 5 heads of 256: 92 (119).
 template <int DH, int STORE, bool FULL, int KEYS, int ROWS>
 __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) void k_attn_few(FewArgs f) {
   constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;

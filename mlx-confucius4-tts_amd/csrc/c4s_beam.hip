@@ -10,7 +10,9 @@
 // The last workgroup of a group to arrive joins the slices' sums (in the slices'
 // order). Its threads look at the slices' first places alone: the width-th best of a
 // wave's threads' best bounds what can win, and the few places that reach the bound
-// are ranked together.
+// are ranked together. 24 groups of 8 rows of 151936, bf16: 25.5 us, of which the slices
+// take 18 (8.8 in the mean, memory and VALU together; 58 MB alone would take 10) and the
+// join 7.6; 64 of 4 of 8194, fp32, penalty and temperature: 15.5, a chain of waits.
 // A second kernel brings the states into their new order, a thread a column: it
 // reads that of all rows before it writes one, so that outputs may be the inputs.
 // (In the first kernel's last workgroups it was a chain of waits: 9 us of 33 for 64
