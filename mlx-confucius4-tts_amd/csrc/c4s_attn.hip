@@ -905,7 +905,10 @@ hipError_t few_by_store(const FewArgs& f, hipStream_t s) {
 // 64 of 20 to 100 21.5 / 19).
 // Weights for codes have the values' scales in them, none is exact, and the error
 // would come to 1.5 times: those enter as pairs (8 prompts of 2048, 20 heads of 64:
-// 224 us for 185, 1.0 times). The weights' sum is taken before the rounding, in fp32
+// 224 us for 185, 1.0 times). So do those for 4-bit pages, so that a token's row is as
+// exact inside a prompt as it is as a step (once / pairs, us: 12 of 500 to 2100, 20 heads of
+// 64, 119 / 143, 1.3 times the output's own rounding against 1.0; 8 of 2048 171 / 200; 2 of 4096, 32 on 8 of 128, 331 / 412; 4 of
+// 2000, 5 of 256, 87 / 104). The weights' sum is taken before the rounding, in fp32
 // (from the matrix engine, of the rounded weights, it would be cheaper and lse off by 3e-4).
 constexpr int kBlock = 64;         // positions
 constexpr int kSegment = 16384;    // positions whose pages LDS holds at a time
@@ -930,7 +933,7 @@ __device__ __forceinline__ int value_piece(int r, int p) {
 }
 
 // (In 4 bits a thread's piece is 16 codes: 16 dims of a key, or 8 positions of a pair of dims. They are in LDS as the
-// bf16 values that they stand for, and from there on such pages are bf16 pages.)
+// bf16 values that they stand for, and from there on such pages are bf16 pages, but for the pairs of weights.)
 template <int DH, int STORE, int NB, int W, int OCC>
 __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
   constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
@@ -1185,14 +1188,17 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
           for (int j = 0; j < 16; ++j) s[b][j / 4][j % 4] = j < from ? -__builtin_inff() : s[b][j / 4][j % 4];
       }
       auto value = [&](int d, int st) { return *reinterpret_cast<const uint4*>(vl + value_piece(16 * d + c, 2 * g + st)); };
-      constexpr bool kAhead = DH == 64;   // two dim tiles' values asked for before the weights, the others' before the products
+      // Two dim tiles' values asked for before the weights, the others' before the products (4-bit pages, whose pieces on
+      // their way and pairs of weights have the registers: 204 us without for 212, 8 of 2048, 20 heads of 64).
+      constexpr bool kAhead = DH == 64 && !Q4;
       uint4 va[kAhead ? 4 : 1];
       if constexpr (kAhead) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) va[i] = value(i / 2, i % 2);
         __builtin_amdgcn_sched_barrier(0);
       }
-      uint32_t p[NB][8], rest[NB][Q8 ? 8 : 1];
+      constexpr bool kPairs = Q8 || Q4;
+      uint32_t p[NB][8], rest[NB][kPairs ? 8 : 1];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         float top = fmaxf(s[b][0][0], s[b][0][1]);
@@ -1218,13 +1224,13 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
             y *= vs[1];
           }
           p[b][j / 2] = pack(x, y);
-          if constexpr (Q8) rest[b][j / 2] = pack(x - low(p[b][j / 2]), y - high(p[b][j / 2]));
+          if constexpr (kPairs) rest[b][j / 2] = pack(x - low(p[b][j / 2]), y - high(p[b][j / 2]));
         }
       }
       auto quad = [](const uint32_t* w) { return make_uint4(w[0], w[1], w[2], w[3]); };
       auto add = [&](f32x4& to, uint4 v, int b, int st) {
         to = mfma(v, quad(p[b] + 4 * st), to);
-        if constexpr (Q8) to = mfma(v, quad(rest[b] + 4 * st), to);
+        if constexpr (kPairs) to = mfma(v, quad(rest[b] + 4 * st), to);
       };
       if constexpr (kAhead) {
 #pragma unroll
@@ -1258,7 +1264,7 @@ __global__ __launch_bounds__(64 * W, OCC) void k_attn_many(ManyArgs f) {
         }
       }
       int strange = 0;
-      if (!kAhead || edge_of(t)) {
+      if (DH > 64 || edge_of(t)) {
 #pragma unroll
         for (int w = 0; w < W; ++w) strange |= odd[buf][w];
       }
@@ -1317,13 +1323,13 @@ hipError_t many_by_store(const AttnArgs& a, hipStream_t s) {
 // 1000, 640, 21 / 30; 2 of 600, 1520, 17.9 / 18.9; 4 of 300 over 500, 1520, 27 / 24; 64 of 48 and of 64 over 300,
 // three and four tiles a sequence, 35 / 39 and 45 / 42; 8 heads of 128: 2 of 200 over 1000, 800, 43 / 65; 2 of 400 over 400, 1600, 48 / 48; 5 heads of 256: 4
 // of 200 over 200, 500, 30 / 29; 4 of 500 over 500, 1260, 107 / 59. 4-bit codes, 20 heads of 64: 4 of 128 over 1000, 640,
-// 16 / 23; 2 of 600, 1520, 15.2 / 15.5; 4 of 300 over 500, 1520, 21 / 19; 64 of 48 over 300, three tiles a sequence, 29 / 33; 8 heads
-// of 128: 2 of 400 over 400, 1600, 35 / 38; 4 of 300 over 500, 2400, 51 / 39; 5 heads of 256: 64 of 17 over 300, 640, 30 / 34;
-// 64 of 48 over 300, 960, 41 / 41.
+// 16.6 / 27; 2 of 600, 1520, 15.0 / 17.4; 4 of 300 over 500, 1520, 21.0 / 21.0; 64 of 48 and of 64 over 300, three and four tiles a
+// sequence, 29 / 38 and 37 / 39; 8 heads of 128: 2 of 400 over 400, 1600, 36 / 44; 4 of 300 over 500, 2400, 50 / 46; 5 heads of
+// 256: 64 of 17 over 300, 640, 28 / 37; of 48, 960, 40 / 46; of 64, 1280, 49 / 47.
 bool many_pays(const AttnArgs& a) {
   const int64_t tiles = ((int64_t)a.max_new * a.shared + kRows - 1) / kRows, all = tiles * a.c.n_heads * a.c.n_seqs;
   if (a.c.store != C4S_KV_BF16 && a.c.dim <= 128) return tiles > 3 && all > 1500;
-  return tiles > 1 && all > 700;
+  return tiles > 1 && all > (a.c.store == C4S_KV_Q4 ? 1100 : 700);
 }
 
 }  // namespace
