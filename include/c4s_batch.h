@@ -140,10 +140,14 @@ int c4s_kv_copy(c4s_ctx* ctx, const c4s_kv_cache* cache, const int32_t* copies, 
  * temperature, as c4s_sample_rows applies them, every row r = g * width + j offers its
  * group for every token v the total
  *   score[r] + z[v] - log sum_u exp z[u]
- * (in 64 bits; -inf where score or z is, and where it would be NaN, as for all of a row with NaN or +inf among its
+ * (-inf where score or z is, and where it would be NaN, as for all of a row with NaN or +inf among its
  * z), a row that is done only its stop token, with its score as it is. The `width` largest totals of a group, equal ones by the lowest
  * (j, v), become its rows: parent j, token v, out_score the total, out_done whether the
  * parent was done or v is the stop token.
+ * Totals are in 64 bits, of exponentials in 32: a row's log sum is off by up to
+ *   2^-22 (1.5 + the mean of |z - the row's largest|, weighted by exp z),
+ * 4e-7 to 2e-6, for all its tokens alike, and by a little else in a call of another number
+ * of rows. Two rows' totals that lie nearer to each other may come in either order.
  * hist_bits and the states are carried along: row g * width + i of each output is row
  * g * width + out_parent[..] of its input, and out_hist_bits then has the token added,
  * unless the row was or is done. Outputs may be their inputs themselves.

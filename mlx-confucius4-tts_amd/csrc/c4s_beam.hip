@@ -19,8 +19,12 @@
 // groups of 4 with 1757 words a row, 40 of 85 for 24 of 8 with 5348.)
 //
 // Orders are on (value, index) pairs, equal values by the lower index, so results
-// do not depend on how rows are cut, but for the sums' rounding: exp(z - m) as
-// 2^((z - m) log2 e) is off by 2^-23 |z - m| of itself, least where it counts most.
+// do not depend on how rows are cut, but for the sums' rounding. An exponential is one of 32
+// bits: exp(z - m) as 2^((z - m) log2 e) is off by 2^-22.8 |z - m| + 2^-23 of itself, least where it
+// counts most. A chunk's 16 are added in pairs (2^-22), and all that follows, the chunks' sums and
+// what scales them when the maximum rises, is in 64 bits. (One running sum in 32 bits, up to 512 additions
+// that may all round the same way, was off by 1.4e-5, and 24 groups of 8 rows of 151936, bf16, without states, took 26.3 us for
+// 27.6; with the library's exp for the scaling 28.2.)
 // (One fused operation, z log2 e - m log2 e, would save a tenth of the VALU's work and
 // overflow on a row whose logits are all the type's lowest value.)
 
@@ -41,6 +45,7 @@ constexpr int kPer = 16, kChunk = 64 * kPer;   // values of a lane, and of a wav
 constexpr int kMostChunks = 32;                // of a slice
 constexpr int kQueue = 128;                    // a lane's chunks that wait to be looked at
 constexpr int kFound = 1024;                   // places that are ranked together
+constexpr int kStats = 2;                      // words of a part in front of its keys
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -50,7 +55,7 @@ struct BeamArgs {
   uint32_t* arrived;     // [n_groups]
   int state_wgs;         // workgroups of a group's states
   int32_t* joined;       // [rows] the token that joins a row's history, -1: none; with states
-  uint64_t* parts;       // [rows][slices][1 + width]: maximum and sum, keys
+  uint64_t* parts;       // [rows][slices][kStats + width]: maximum, sum (in 64 bits), keys
 };
 
 __device__ __forceinline__ void wave_order() {   // this wave's writes to LDS before its reads behind it
@@ -79,6 +84,23 @@ __device__ __forceinline__ Total total_of(double t, int at) {   // what is not a
 }
 __device__ __forceinline__ double total_value(const Total& x) {
   return __longlong_as_double((long long)(x.t >> 63 ? x.t ^ 1ull << 63 : ~x.t));
+}
+
+// exp y, y <= 0 (below -700, where it no longer counts, 2^-1010): 2^n exp r with |r| up to log 2 / 2, whose series'
+// first missing term is r^9 / 9! < 2e-10.
+__device__ __forceinline__ double exp_below(double y) {
+  const double x = y > -700.0 ? y * 1.4426950408889634 : -1010.0;
+  const double n = rint(x), r = (x - n) * 0.6931471805599453;
+  double p = 1.0 / 40320.0;
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)n);
 }
 
 // A number that at least n of the wave's lanes reach, and the n-th largest of them but for its last bits (0: fewer
@@ -187,7 +209,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, W = a.width, V = a.vocab;
   const int group = blockIdx.x / f.wgs, units = W * f.slices, unit = blockIdx.x % f.wgs * kBeamWaves + wave;
   const int64_t row0 = (int64_t)group * W;
-  const int words = 1 + W;
+  const int words = kStats + W;
 
   if (unit < units) {
     const int64_t row = row0 + unit / f.slices;
@@ -212,7 +234,8 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
     const bool idle = (a.done && a.done[row]) || a.score[row] == -__builtin_inff();   // its logits do not matter
     if (!idle) {
       uint32_t (*chunk_tops)[64] = lds.wave.tops[wave];
-      float m = -__builtin_inff(), sum = 0.0f;
+      float m = -__builtin_inff();
+      double sum = 0.0;
       uint32_t most = 0;   // key of the lane's largest value; 0: it has none
       float z[kPer];
       auto chunk = [&](int which, int v0, int at) {
@@ -231,15 +254,21 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
         chunk_tops[at][lane] = key;
         most = max(most, key);
         if (top > m) {
-          sum *= __builtin_amdgcn_exp2f((m - top) * kLog2e);
+          sum *= exp_below((double)m - (double)top);
           m = top;
         }
         if (m > -__builtin_inff()) {
+          float e[kPer];
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) sum += __builtin_amdgcn_exp2f((z[i] - m) * kLog2e);
+          for (int i = 0; i < kPer; ++i) e[i] = __builtin_amdgcn_exp2f((z[i] - m) * kLog2e);
+#pragma unroll
+          for (int n = kPer / 2; n; n /= 2)
+#pragma unroll
+            for (int i = 0; i < n; ++i) e[i] += e[i + n];
+          sum += (double)e[0];
         } else {
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) sum = z[i] != z[i] ? z[i] : sum;   // NaN among the logits is NaN here
+          for (int i = 0; i < kPer; ++i) sum = z[i] != z[i] ? (double)z[i] : sum;   // NaN among the logits is NaN here
         }
       };
       for (int v0 = begin, at = 0; v0 < end; v0 += 2 * kChunk, at += 2) {
@@ -309,13 +338,15 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       }
       // the slice's maximum, sum and list
       const float top = wave_max_dpp(m);
-      const float s = (float)wave_sum_dpp((double)(m == top ? sum : sum * __builtin_amdgcn_exp2f((m - top) * kLog2e)));
+      const double s = wave_sum_dpp(m == top ? sum : sum * exp_below((double)m - (double)top));
       uint64_t* part = f.parts + (row * f.slices + slice) * words;
       uint64_t w = 0;
       if (lane < kept) w = list[lane];
-      if (lane < W) __hip_atomic_store(part + 1 + lane, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (lane == 0)
-        __hip_atomic_store(part, (uint64_t)__float_as_uint(top) << 32 | __float_as_uint(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (lane < W) __hip_atomic_store(part + kStats + lane, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (lane == 0) {
+        __hip_atomic_store(part, (uint64_t)__float_as_uint(top), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(part + 1, (uint64_t)__double_as_longlong(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
   }
   if (!last_to_arrive(f.arrived + group, f.wgs)) return;
@@ -326,16 +357,18 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   const int tid = threadIdx.x;
   uint64_t first[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) first[i] = tid < units && i < W ? word(tid, 1 + i) : 0;
+  for (int i = 0; i < 4; ++i) first[i] = tid < units && i < W ? word(tid, kStats + i) : 0;
   // A wave has every fourth row; of up to 64 slices all sums are on their way.
   constexpr int kRowsOfWave = kBeamWidth / kBeamWaves;
-  const uint64_t none = (uint64_t)__float_as_uint(-__builtin_inff()) << 32;
-  uint64_t stat[kRowsOfWave];
+  float most[kRowsOfWave];
+  double part[kRowsOfWave];
+  auto stats = [&](int i, int j, int s) {
+    const bool there = j < W && s < f.slices;
+    most[i] = there ? __uint_as_float((uint32_t)word(j * f.slices + s, 0)) : -__builtin_inff();
+    part[i] = there ? __longlong_as_double((long long)word(j * f.slices + s, 1)) : 0.0;
+  };
 #pragma unroll
-  for (int i = 0; i < kRowsOfWave; ++i) {
-    const int j = wave + kBeamWaves * i;
-    stat[i] = j < W && lane < f.slices ? word(j * f.slices + lane, 0) : none;
-  }
+  for (int i = 0; i < kRowsOfWave; ++i) stats(i, wave + kBeamWaves * i, lane);
   if (tid < W) {
     score[tid] = a.score[row0 + tid];
     done[tid] = a.done ? a.done[row0 + tid] : 0;
@@ -348,11 +381,10 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
     float m = -__builtin_inff();
     double sum = 0.0;
     for (int s0 = 0; s0 < f.slices; s0 += 64) {
-      if (s0) stat[i] = s0 + lane < f.slices ? word(j * f.slices + s0 + lane, 0) : none;
-      const float mine = __uint_as_float((uint32_t)(stat[i] >> 32)), part = __uint_as_float((uint32_t)stat[i]);
-      const float t = fmaxf(m, wave_max_dpp(mine));
-      const double more = wave_sum_dpp((double)(mine == t ? part : part * __builtin_amdgcn_exp2f((mine - t) * kLog2e)));
-      sum = (m == t ? sum : sum * (double)__builtin_amdgcn_exp2f((m - t) * kLog2e)) + more;
+      if (s0) stats(i, j, s0 + lane);
+      const float t = fmaxf(m, wave_max_dpp(most[i]));
+      const double more = wave_sum_dpp(most[i] == t ? part[i] : part[i] * exp_below((double)most[i] - (double)t));
+      sum = (m == t ? sum : sum * exp_below((double)m - (double)t)) + more;
       m = t;
     }
     if (lane == 0) {
@@ -375,7 +407,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   {
     Total mine = no_total();
     for (int u = tid; u < units; u += kBeamThreads) {
-      const Total t = total(u, 0, u < kBeamThreads ? first[0] : word(u, 1));
+      const Total t = total(u, 0, u < kBeamThreads ? first[0] : word(u, kStats));
       if (t.beats(mine)) mine = t;
     }
     // (of a total's bits the upper half: a bound a little lower does as well)
@@ -389,7 +421,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
     for (int at0 = 0; at0 < W; at0 += 4) {   // places are in order: behind one that does not reach the bound none does
       uint64_t k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = at0 == 0 && u < kBeamThreads ? first[i] : (at0 + i < W ? word(u, 1 + at0 + i) : 0);
+      for (int i = 0; i < 4; ++i) k[i] = at0 == 0 && u < kBeamThreads ? first[i] : (at0 + i < W ? word(u, kStats + at0 + i) : 0);
       bool more = true;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -425,7 +457,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       Total mine = no_total();
       for (int u = threadIdx.x; u < units; u += kBeamThreads)
         for (int at = 0; at < W; ++at) {
-          const Total t = total(u, at, word(u, 1 + at));
+          const Total t = total(u, at, word(u, kStats + at));
           if (!t.at) break;
           if (i == 0 || last.beats(t)) {
             if (t.beats(mine)) mine = t;
@@ -530,14 +562,14 @@ BeamArgs beam_args(const c4s_beam& a) {
 
 LayerSpace beam_space(const c4s_beam& a) {
   const BeamArgs f = beam_args(a);
-  return {a.n_groups, (int64_t)a.n_groups * a.width * (f.slices * (1 + a.width) * 2 + 1)};
+  return {a.n_groups, (int64_t)a.n_groups * a.width * (f.slices * (kStats + a.width) * 2 + 1)};
 }
 
 hipError_t launch_beam(const c4s_beam& a, uint32_t* counters, float* space, hipStream_t s) {
   BeamArgs f = beam_args(a);
   f.arrived = counters;
   f.parts = reinterpret_cast<uint64_t*>(space);
-  f.joined = f.state_wgs ? reinterpret_cast<int32_t*>(f.parts + (int64_t)a.n_groups * a.width * f.slices * (1 + a.width)) : nullptr;
+  f.joined = f.state_wgs ? reinterpret_cast<int32_t*>(f.parts + (int64_t)a.n_groups * a.width * f.slices * (kStats + a.width)) : nullptr;
   const dim3 grid((unsigned)(a.n_groups * f.wgs)), block(kBeamThreads);
   if (a.dtype == C4S_DTYPE_BF16) hipLaunchKernelGGL(k_beam<true>, grid, block, 0, s, f);
   else hipLaunchKernelGGL(k_beam<false>, grid, block, 0, s, f);
