@@ -18,6 +18,9 @@
 // (In the first kernel's last workgroups it was a chain of waits: 9 us of 33 for 64
 // groups of 4 with 1757 words a row, 40 of 85 for 24 of 8 with 5348.)
 //
+// Logits that differ can have one total: beside a score of -1e30 all have, and so have some far smaller than the row's
+// largest. Where a list's last place is such a one, the tied tokens are looked for once more (to know that takes up to
+// 0.4 us).
 // Orders are on (value, index) pairs, equal values by the lower index, so results
 // do not depend on how rows are cut, but for the sums' rounding. An exponential is one of 32
 // bits: exp(z - m) as 2^((z - m) log2 e) is off by 2^-22.8 |z - m| + 2^-23 of itself, least where it
@@ -198,12 +201,16 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       uint16_t queue[kBeamWaves][kQueue];           // chunk * 64 + lane
     } wave;
     Total found[kFound];
+    struct {
+      int32_t token[kBeamWidth][kBeamWidth];   // of each row the lowest that tie for the last places
+      int32_t n[kBeamWidth];
+    } ties;
   } lds;
   __shared__ Total won[kBeamWidth];
   __shared__ uint32_t bounds[kBeamWaves];
   __shared__ double logs[kBeamWidth];                    // the rows' log sum exp(z - tops)
   __shared__ float score[kBeamWidth], tops[kBeamWidth];
-  __shared__ int n_found;
+  __shared__ int n_found, merged;
   __shared__ uint8_t done[kBeamWidth];
   const c4s_beam& a = f.a;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, W = a.width, V = a.vocab;
@@ -373,7 +380,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
     score[tid] = a.score[row0 + tid];
     done[tid] = a.done ? a.done[row0 + tid] : 0;
   }
-  if (tid == 0) n_found = 0;
+  if (tid == 0) n_found = merged = 0;
 #pragma unroll
   for (int i = 0; i < kRowsOfWave; ++i) {
     const int j = wave + kBeamWaves * i;
@@ -394,14 +401,22 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
   }
   __syncthreads();
 
+  auto lost = [&](int j) { return !(score[j] > -__builtin_inff()) | (logs[j] != logs[j]); };   // all of row j's totals are -inf
+  auto total_at = [&](int j, float z, int v) {
+    return total_of(z == -__builtin_inff() ? -__builtin_inf() : (double)score[j] + (((double)z - (double)tops[j]) - logs[j]), j * V + v);
+  };
   // Place `at` of slice u, whose key is k where the row's logits matter.
   auto total = [&](int u, int at, uint64_t k) {
     const int j = u / f.slices;
     if (done[j]) return u == j * f.slices && at == 0 ? total_of(score[j], j * V + a.stop_token) : no_total();
-    if (!(score[j] > -__builtin_inff()) | (logs[j] != logs[j])) return u == j * f.slices && at < V ? total_of(-__builtin_inf(), j * V + at) : no_total();
-    if (!k) return no_total();
-    const float z = key_value(k);
-    return total_of(z == -__builtin_inff() ? -__builtin_inf() : (double)score[j] + (((double)z - (double)tops[j]) - logs[j]), j * V + key_token(k));
+    if (lost(j)) return u == j * f.slices && at < V ? total_of(-__builtin_inf(), j * V + at) : no_total();
+    return k ? total_at(j, key_value(k), key_token(k)) : no_total();
+  };
+  // Whether the slice whose last place this is may have left out lower tokens of the same total: its logit's total is
+  // that of the next lower number too.
+  auto merges = [&](int u, uint64_t k, const Total& t) {
+    const int j = u / f.slices;
+    return !done[j] && !lost(j) && key_value(k) > -__builtin_inff() && total_at(j, kfloat((uint32_t)(k >> 32) - 1), 0).t == t.t;
   };
   Total* found = lds.found;
   {
@@ -430,6 +445,7 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
         if (more) {
           const int n = atomicAdd(&n_found, 1);
           if (n < kFound) found[n] = t;
+          if (at0 + i == W - 1 && merges(u, k[i], t)) merged = 1;
         }
       }
       if (!more) break;
@@ -458,11 +474,8 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
       for (int u = threadIdx.x; u < units; u += kBeamThreads)
         for (int at = 0; at < W; ++at) {
           const Total t = total(u, at, word(u, kStats + at));
-          if (!t.at) break;
-          if (i == 0 || last.beats(t)) {
-            if (t.beats(mine)) mine = t;
-            break;
-          }
+          if (!t.at || t.t < mine.t) break;
+          if ((i == 0 || last.beats(t)) && t.beats(mine)) mine = t;
         }
       __syncthreads();
       found[threadIdx.x] = mine;
@@ -477,6 +490,56 @@ __global__ __launch_bounds__(kBeamThreads, 4) void k_beam(BeamArgs f) {
     }
   }
   __syncthreads();
+  if (merged) {
+    // Of different logits with equal totals a slice's list has the highest logits, but the lowest tokens come first. The last
+    // place's total is right, and so are the places above it, of which a list leaves out none: the row's tokens with that
+    // very total, looked for in all its logits, fill the others. A wave takes every fourth row. (This is seldom, and slow
+    // where ties are few: 0.5 ms for a row of 151936 bf16, 3 us for one of 8194.)
+    const uint64_t tie = won[W - 1].t;
+    for (int j = wave; j < W; j += kBeamWaves) {
+      int32_t* tied = lds.ties.token[j];
+      int n = 0;
+      if (done[j]) {
+        n = total_of(score[j], 0).t == tie;
+        if (n && lane == 0) tied[0] = a.stop_token;
+      } else if (lost(j)) {
+        n = tie == kTotalNegInf ? min(W, V) : 0;
+        if (lane < n) tied[lane] = lane;
+      } else {
+        const Logits<BF16> x(a, row0 + j);
+        constexpr int kSome = Logits<BF16>::kSome;
+        for (int v0 = 0; v0 < V && n < W; v0 += 64 * kSome) {
+          const int v = v0 + kSome * lane;
+          float z[kSome];
+          x.value(x.raw(v, V), x.bits(v, V), z);
+          int before = n;   // those of the lanes before
+          uint32_t mine = 0;
+#pragma unroll
+          for (int i = 0; i < kSome; ++i) {
+            const bool same = v + i < V && total_at(j, z[i], 0).t == tie;
+            const uint64_t some = __ballot(same);
+            before += lanes_before(some, lane);
+            n += __popcll(some);
+            mine |= same ? 1u << i : 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < kSome; ++i) {
+            const int place = before + __popc(mine & ((1u << i) - 1));
+            if ((mine >> i & 1) && place < W) tied[place] = v + i;
+          }
+        }
+      }
+      if (lane == 0) lds.ties.n[j] = min(n, W);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int at = 0;
+      while (won[at].t > tie) ++at;
+      for (int j = 0; j < W; ++j)
+        for (int i = 0; i < lds.ties.n[j] && at < W; ++i) won[at++] = Total{tie, ~(uint32_t)(j * V + lds.ties.token[j][i])};
+    }
+    __syncthreads();
+  }
   if (tid < W) {
     const Total t = won[tid];
     const int at = (int)~t.at, parent = at / V, token = at - parent * V;
