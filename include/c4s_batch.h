@@ -34,9 +34,10 @@ extern "C" {
  * position p is turned by the angle t = p * freq[i], and scaled:
  *   a' = scale (a cos t - b sin t),  b' = scale (a sin t + b cos t)
  * C4S_ROPE_HALF: pair i is dims i and i + rot_dim / 2; C4S_ROPE_PAIRS: dims 2 i and
- * 2 i + 1. The other dims are copied. freq is in 64 bits, and so are the angles
- * until they are reduced to a part of a turn: at position 10^6 a frequency rounded
- * to 32 bits would be off by 0.06 radians. Negated frequencies turn back.
+ * 2 i + 1. The other dims are copied. freq is in 64 bits, and angles are reduced to a
+ * part of a turn with what their products lose, so that 2^-26 of a turn is all they are
+ * off by at every position (a frequency below 1 that is rounded to 32 bits is off by up to
+ * 0.03 radians at position 10^6). Negated frequencies turn back.
  * (Contexts longer than a model was trained with: freq and scale as it wants them.)
  *
  * q and k have n_rows rows, row r's head h at q + r * ldq + h * head_dim (strides in

@@ -8,13 +8,16 @@
 // past the L2, where nothing would be found again (the next call's workgroups are on
 // other dies). 18829 rows in place, halves, from the last-level cache, where the product
 // before leaves them / from memory: 20 and 20 heads of 64 34 us, 5.6 TB/s / 45 (a half is
-// half a line there); 32 and 8 of 128 59, 6.5 TB/s / 77. (Stores through the L2: 46 / 59 for heads of 64.
+// half a line there); 32 and 8 of 128 59, 6.5 TB/s / 77. 20 and 20 heads of 64 in floats, of twice the bytes, 77 from memory, 5.0 TB/s.
+// (Stores through the L2: 46 / 59 for heads of 64.
 // Loads past the caches as well: 43 / 44, and 66 / 67 for heads of 128. One piece of a thread at a time 47 from memory;
 // lines whole and the halves exchanged between lanes 48; workgroups of two or four rows 44.) 64 rows: 2.9 us.
 //
-// The angle is reduced in 64 bits: position * frequency / 2 pi, less its whole
-// turns, has an absolute error of 2^-52 of the number of turns; the rest, at most
-// half a turn, is exact enough in 32 bits (2^-25 of a turn, 2e-7 radians).
+// The angle is reduced in twice 64 bits: what the product position * frequency and its division by 2 pi (a
+// constant of two parts) lose in their last place is added to what is left of the whole turns, of which there may be
+// 2^28 and more. That rest, at most half a turn, is exact enough in 32 bits (2^-26 of a turn, 1e-7 radians). With 64 bits alone the
+// error was more than 2^-52 of the number of turns: 3e-7 radians at frequency 1 and position 2^31, 3e-4 at
+// frequency 1000. The calls take as long as before.
 
 #include <hip/hip_runtime.h>
 
@@ -56,6 +59,15 @@ template <class T, int N>
 struct alignas(N <= 2 ? sizeof(T) : sizeof(T) * N) Few {
   T v[N];
 };
+
+// pos * freq / 2 pi less its whole turns.
+__device__ __forceinline__ double part_of_turn(double pos, double freq) {
+  constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnRest = -0x1.6b01ec5417056p-57;   // 1 / 2 pi
+  const double angle = pos * freq, angle_rest = fma(pos, freq, -angle);
+  const double turns = angle * kTurn;
+  const double rest = fma(angle, kTurn, -turns) + (angle * kTurnRest + angle_rest * kTurn);
+  return turns - rint(turns) + rest;
+}
 
 constexpr int kRopeThreads = 256, kRopeAhead = 2;   // pieces of a thread that are on their way together
 
@@ -125,10 +137,8 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs f) {
   const int64_t pos = position_of(a, row);
   if (pos < 0) return;
   for (int p = threadIdx.x; p < half; p += blockDim.x) {
-    double turns = (double)pos * a.freq[p] * 0.15915494309189535;
-    turns -= rint(turns);
     float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
+    sincospif(2.0f * (float)part_of_turn((double)pos, a.freq[p]), &s, &c);
     cs[p] = c * a.scale;
     sn[p] = s * a.scale;
   }
