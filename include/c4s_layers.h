@@ -145,8 +145,8 @@ enum { C4S_KV_BF16 = 0, C4S_KV_Q8 = 1, C4S_KV_Q4 = 2 };
 typedef struct c4s_kv_cache {
   void* k;
   void* v;                      /* both 16-byte aligned */
-  void* k_scale;                /* float (C4S_KV_Q8) or uint8_t (C4S_KV_Q4), 16-byte aligned */
-  void* v_scale;
+  float* k_scale;               /* C4S_KV_Q8; C4S_KV_Q4: uint8_t, cast. 16-byte aligned */
+  float* v_scale;
   const int32_t* block_table;   /* [n_seqs][table_ld] */
   int64_t table_ld;
   int32_t n_seqs;               /* up to 65535 */

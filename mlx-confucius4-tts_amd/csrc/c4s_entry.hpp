@@ -19,7 +19,7 @@ inline int launched(c4s_ctx* ctx, hipError_t e, const char* what) {
   return e == hipSuccess ? C4S_OK : hip_fail(ctx, e, what);
 }
 
-// Runs `body` with the context's device current; nothing is thrown through the ABI.
+// Runs `body`; nothing is thrown through the ABI.
 template <class Body>
 int entry(c4s_ctx* ctx, const void* desc, const char* what, Body body) {
   if (!ctx) return C4S_EINVAL;
@@ -79,8 +79,8 @@ inline int check_cache(c4s_ctx* ctx, const c4s_kv_cache* c) {
 inline KvArgs to_args(const c4s_kv_cache* c) {
   int shift = 0;
   while ((1 << shift) < c->page_size) ++shift;
-  return KvArgs{c->k,       c->v,          static_cast<float*>(c->k_scale), static_cast<float*>(c->v_scale), c->block_table, c->table_ld, c->n_seqs,
-                     c->max_pages, c->n_pages, shift, c->n_kv_heads, c->head_dim, c->store};
+  return KvArgs{c->k,       c->v,          c->k_scale,    c->v_scale,    c->block_table, c->table_ld, c->n_seqs,
+                c->max_pages, c->n_pages, shift, c->n_kv_heads, c->head_dim, c->store};
 }
 
 }  // namespace c4s
