@@ -127,7 +127,8 @@ int c4s_linear(c4s_ctx* ctx, const c4s_linear_desc* lin, void* stream);
  * times as large (2^-127 at least), a code the nearest (of two the even one); the 32
  * read back as NaN where one is not finite (e = 255). All values are bf16 numbers but 4
  * or 6 times 2^126, which read back as infinite, or count in c4s_attn as what they are.
- * There values of a scale of 2^-127 may count as 0.
+ * There values below 2^-80 may lose bits, and those below 2^-110 count as 0: their scales
+ * join the weights.
  * (The values lie with their positions next to each other because that is how
  * the product of weights and values reads them: no transpose in the decode.)
  *
@@ -181,7 +182,8 @@ int c4s_kv_read(c4s_ctx* ctx, const c4s_kv_cache* cache, const c4s_kv_rows* rows
  *   out[r][h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[r][h] . k_j),
  * with the keys and values of head h / (n_heads / n_kv_heads); a row that sees
  * nothing is zero. Values that are not finite matter only to rows that see them
- * (those read inf or NaN).
+ * (those read inf or NaN). Sums are in 32 bits, of weights up to 2^8 before they are divided:
+ * values above 2^99 may overflow.
  * Refused (C4S_EINVAL): max_pages above 1024 together with more than 262144 of
  * (sequence, key head, 16 of its new rows' query heads), where few rows a sequence
  * have their positions' parts joined, or with more than 16777215 of (such a one of

@@ -193,7 +193,8 @@ struct FewArgs {
 // the rows repeated four times: each lane group has all of a tile's scores, and takes those of another tile, so that
 // a lane has one position's scores, of ROWS rows. What the weights are relative to lies up to 2^kFewSlack above the
 // greatest, so that a vote finds nothing to do in most blocks, sums stay a lane's own until the end, and the values'
-// scales join the weights, a product a row and block of 32 dims (a scale of 2^-127 counts as 0 there); the weights then
+// scales join the weights, a product a row and block of 32 dims (where that leaves bf16's range, below 2^-126, the weight's
+// low half and then all of it counts as 0); the weights then
 // go through LDS, as pairs of bf16 for each such block, into the second product's operand. The codes themselves need no
 // scale there: two positions' bytes give a dim's pair by an exchange of nibbles and one conversion. 64 rows of 50 to 1500
 // positions, 20 heads of 64: 17.5 us (as with more rows 22.4); 64 of 4000, 5 heads of 256: 92 (119).

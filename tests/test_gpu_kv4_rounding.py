@@ -55,3 +55,14 @@ def test_padding_and_missing_pages_with_wide_heads(gpu_ctx):
     empty = torch.isinf(L.attn(cache, q, new, heads, 0.0625, first)[1])
     assert empty.any() and (out.cpu()[empty] == 0).all()
     _check_attn(cache, q, out, lse, new, heads, first=first)
+
+
+@pytest.mark.parametrize("byte", [47, 221])
+@pytest.mark.parametrize("new,past,heads,kv_heads,dim", [([1, 1], [300, 20], 3, 3, 64), ([1, 1], [300, 20], 12, 3, 128), ([6, 1], [300, 20], 5, 5, 256),
+                                                         ([150, 80], [40, 3], 80, 80, 64)])
+def test_values_as_small_and_as_large_as_attention_has_them(gpu_ctx, byte, new, past, heads, kv_heads, dim):
+    """All scales 2^-80, or 2^94: values up to 2^96.6."""
+    cache = B.Cache4([n + p for n, p in zip(new, past)], kv_heads, dim, 16, seed=dim, junk=True)
+    cache.t["v_scale"][cache.t["v_scale"] != 255] = byte
+    q, out, lse = _run_attn(gpu_ctx, cache, new, heads, spread=0.7)
+    _check_attn(cache, q, out, lse, new, heads)
