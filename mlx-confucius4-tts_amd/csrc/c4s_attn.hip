@@ -197,7 +197,7 @@ struct FewArgs {
 // low half and then all of it counts as 0); the weights then
 // go through LDS, as pairs of bf16 for each such block, into the second product's operand. The codes themselves need no
 // scale there: two positions' bytes give a dim's pair by an exchange of nibbles and one conversion. 64 rows of 50 to 1500
-// positions, 20 heads of 64: 17.5 us (as with more rows 22.4); 64 of 4000, 5 heads of 256: 92 (119).
+// positions, 20 heads of 64: 17.4 us (as with more rows 21.8); 64 of 4000, 10 query heads on 5 of 256: 92 (111).
 template <int DH, int STORE, bool FULL, int KEYS, int ROWS>
 __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) void k_attn_few(FewArgs f) {
   constexpr bool Q8 = STORE == C4S_KV_Q8, Q4 = STORE == C4S_KV_Q4;
@@ -839,7 +839,7 @@ __global__ __launch_bounds__(kAttnThreads, DH == 64 ? 3 : (DH == 128 ? 2 : 1)) v
 // for 512 / 1024 / 2048: 64 rows of 1024, 8 heads of 128: 54 / 72 / 68 (8-bit 32
 // / 41 / 44); 8 rows of 2000, 20 heads of 64: 17.7 / 18.5 / 19.9; 6 rows of 12000
 // to 50001, 8 heads of 128, 8-bit: 95 / 94 / 87. With 4-bit pages, of half the bytes, pieces of 2560: the last 46 us
-// (with 1280 48), 64 of 4000, 5 heads of 256, 95 (107).
+// (with 1280 48), 64 of 4000, 10 query heads on 5 of 256, 92 (103).
 FewArgs few_args(const AttnArgs& a) {
   FewArgs f{};
   f.a = a;

@@ -10,9 +10,9 @@
 // The last workgroup of a group to arrive joins the slices' sums (in the slices'
 // order). Its threads look at the slices' first places alone: the width-th best of a
 // wave's threads' best bounds what can win, and the few places that reach the bound
-// are ranked together. 24 groups of 8 rows of 151936, bf16: 25.5 us, of which the slices
-// take 18 (8.8 in the mean, memory and VALU together; 58 MB alone would take 10) and the
-// join 7.6; 64 of 4 of 8194, fp32, penalty and temperature: 15.5, a chain of waits.
+// are ranked together. 24 groups of 8 rows of 151936, bf16: 27.7 us; when it was 25.5, the slices
+// took 18 (8.8 in the mean, memory and VALU together; 58 MB alone would take 10; why the last
+// end so late is not known) and the join 7.6. 64 of 4 of 8194, fp32: 13.7, a chain of waits.
 // A second kernel brings the states into their new order, a thread a column: it
 // reads that of all rows before it writes one, so that outputs may be the inputs.
 // (In the first kernel's last workgroups it was a chain of waits: 9 us of 33 for 64
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(kBeamThreads) void k_beam_states(BeamArgs f) {
 }
 
 // How a row is cut: into slices for twelve waves a CU together, of 1 to kMostChunks chunks. In us, for 8 / 12 / 16 / 24
-// waves a CU: 24 groups of 8 rows of 151936 bf16 27.2 / 26.2 / 27.4 / 35.4, fp32 30.8 / 31.0 / 32.5 / 39.9; 192 rows
+// waves a CU (with sums in 32 bits): 24 groups of 8 rows of 151936 bf16 27.2 / 26.2 / 27.4 / 35.4, fp32 30.8 / 31.0 / 32.5 / 39.9; 192 rows
 // 24.3 / 20.7 / 21.1 / 26.8; 256 groups of 4 of 32000 25.1 / 23.4 / 23.2 / 30.3.
 BeamArgs beam_args(const c4s_beam& a) {
   BeamArgs f{};

@@ -1,7 +1,8 @@
 // The paged key-value cache: rows written as bf16 or as 8- or 4-bit codes, and
 // read back (include/c4s_layers.h has the layout).
 //
-// Both kernels take tiles of packed rows of one head, four lanes a row. Keys keep
+// Both kernels take tiles of packed rows of one head, four lanes a row (a read in large
+// tiles eight, with two rows each). Keys keep
 // their order: pieces of eight dims go to and from the page as they are. Values
 // lie in the page with their positions next to each other, so a tile of them
 // passes through LDS. Four rows of a tile that are positions 4 i .. 4 i + 3 of a
@@ -396,7 +397,8 @@ __global__ __launch_bounds__(4 * TILE, 4) void k_kv_read(KvArgs c, KvRowsArgs ro
         for (int j = 0; j < 8; ++j)
           v[j] = Q8 ? (float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * scale[which][h]
                     : __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-        // past the caches, which keeps the pages in them (41 us for 52)
+        // past the caches, which keeps the pages in them (18829 rows, 20 heads of 64, from memory: 8-bit 30 us for 40, 4-bit 25
+        // for 37, bf16 39 for 46)
         if (rows.f32) {
           typedef float Quad __attribute__((ext_vector_type(4)));
           Quad* q = reinterpret_cast<Quad*>(static_cast<float*>(out) + o + d);

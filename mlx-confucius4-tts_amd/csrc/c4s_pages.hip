@@ -9,8 +9,8 @@
 // Who shares a last page with whom is found in a hash table in LDS. Nothing depends on
 // the order in which threads come, so tables are the same in every run.
 // A step's call is a chain of a few dependent reads (64 sequences: 8.5 us, 2.7 of them
-// the launch; a trim 3.6, a fork of 64 groups of 4 5.4); thousands of pages keep the
-// one workgroup's VALU and LDS busy.
+// the launch; a trim 3.6, a fork of 64 groups of 4 5.4). With thousands of pages, too, its waves
+// wait for half of the time: VALU 57 % busy, LDS 23 %.
 
 #include <hip/hip_runtime.h>
 
